@@ -69,6 +69,20 @@ class MoeEp(C.Structure):
                 ("peers", C.POINTER(EpPeers))]
 
 
+class PagedKv(C.Structure):
+    """glq_paged_kv_t"""
+    _fields_ = [("k_pages", vp), ("v_pages", vp), ("k_scale", vp), ("v_scale", vp), ("table", vp), ("table_stride", C.c_int64),
+                ("dtype", C.c_int32), ("n_pages", C.c_int32), ("n_kv", C.c_int32), ("head_dim", C.c_int32), ("page", C.c_int32),
+                ("max_pages", C.c_int32)]
+
+
+class PagedRows(C.Structure):
+    """glq_paged_rows_t"""
+    _fields_ = [("start", vp), ("q_start", vp), ("start_stride", C.c_int32), ("B", C.c_int32), ("rows", C.c_int32),
+                ("max_new", C.c_int32)]
+
+
+KV_I8, KV_E4M3 = 0, 1
 MOE_PHASE_ALL, MOE_PHASE_EXPERTS, MOE_PHASE_COMBINE, MOE_PHASE_EXCHANGE = 0, 1, 2, 3
 MOE_EP_NO_ZERO_FILL = 1
 
@@ -124,6 +138,12 @@ _SIGS = {
                                   vp, vp, vp]),
     "glq_moe_forward_ep": (C.c_int, [C.POINTER(MoeDesc), vp, C.c_int, vp, vp, vp, vp, vp, C.c_size_t, vp, C.c_size_t,
                                      vp, vp, vp, vp, C.POINTER(MoeEp)]),
+    "glq_paged_append": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedRows), vp, C.c_int64, vp, C.c_int64, vp, C.c_int64, vp, C.c_int64,
+                                   C.c_int, vp, vp, C.c_int, vp, vp, C.c_float, vp]),
+    "glq_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedKv), C.POINTER(PagedRows), C.c_int]),
+    "glq_paged_attention": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedRows), vp, C.c_int64, vp, C.c_int64, C.c_int, C.c_float, vp,
+                                      C.c_size_t, vp]),
+    "glq_paged_read": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedRows), vp, vp, vp]),
 }
 
 _lib = None

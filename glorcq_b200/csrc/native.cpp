@@ -50,7 +50,11 @@ struct Api {
     GLQ_FN(glq_moe_workspace_bytes)                                                                                 \
     GLQ_FN(glq_moe_counters)                                                                                        \
     GLQ_FN(glq_moe_forward_ep)                                                                                      \
-    GLQ_FN(glq_add_rmsnorm)
+    GLQ_FN(glq_add_rmsnorm)                                                                                         \
+    GLQ_FN(glq_paged_append)                                                                                        \
+    GLQ_FN(glq_paged_attention_workspace_bytes)                                                                     \
+    GLQ_FN(glq_paged_attention)                                                                                     \
+    GLQ_FN(glq_paged_read)
     GLQ_FNS
 #undef GLQ_FN
 } api;
@@ -609,6 +613,161 @@ PyObject* py_add_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- paged key/value cache in 8 bits ---------------------------------------------------------------------------
+// The descriptors of a call from its tensors: codes (pages, heads, tokens, channels) of keys and values, their scales (pages, heads),
+// page table (B, max_pages), start (B,) or (1,), q_start (B + 1,) or None.
+struct PagedCall {
+    glq_paged_kv_t kv;
+    glq_paged_rows_t rows;
+    const at::Tensor* pages;
+};
+const at::Tensor& beside(PyObject* o, const char* name, at::ScalarType dtype, const char* dtype_name, const at::Tensor& with) {
+    const at::Tensor& t = tensor(o, name);
+    need(t, name, dtype, dtype_name);
+    if (t.device() != with.device()) fail(std::string(name) + " must be on the device of the pages");
+    return t;
+}
+PagedCall paged_call(PyObject* const* a, int64_t n_rows, int64_t max_new) {
+    PagedCall c;
+    std::memset(&c.kv, 0, sizeof(c.kv));
+    std::memset(&c.rows, 0, sizeof(c.rows));
+    const at::Tensor& kp = tensor(a[0], "k_pages");
+    const at::ScalarType t = kp.scalar_type();
+    if (t != at::kChar && t != at::kFloat8_e4m3fn) fail("k_pages must be torch.int8 or torch.float8_e4m3fn");
+    need(kp, "k_pages", t, "");
+    if (kp.dim() != 4) fail("k_pages must be (pages, heads, tokens, channels)");
+    const at::Tensor& vpg = beside(a[1], "v_pages", t, "of the type of k_pages", kp);
+    const at::Tensor &ks = beside(a[2], "k_scale", at::kFloat, "torch.float32", kp), &vs = beside(a[3], "v_scale", at::kFloat, "torch.float32", kp);
+    const at::Tensor& table = tensor(a[4], "page_table");
+    if (!table.is_cuda() || table.device() != kp.device() || table.scalar_type() != at::kInt || table.dim() != 2 ||
+        (table.size(1) > 1 && table.stride(1) != 1))
+        fail("page_table must be (sequences, pages) torch.int32 rows on the device of the pages");
+    const at::Tensor& start = beside(a[5], "start", at::kLong, "torch.int64", kp);
+    const at::Tensor* qs = a[6] == Py_None ? nullptr : &beside(a[6], "q_start", at::kInt, "torch.int32", kp);
+    const int64_t B = table.size(0), pages = kp.size(0), heads = kp.size(1);
+    if (vpg.sizes() != kp.sizes()) fail("k_pages and v_pages must have one shape");
+    if (ks.dim() != 2 || ks.size(0) != pages || ks.size(1) != heads || vs.sizes() != ks.sizes()) fail("k_scale and v_scale must be (pages, heads)");
+    if (start.dim() != 1 || (start.size(0) != 1 && start.size(0) != B)) fail("start must have one value, or one for each sequence");
+    if (qs && (qs->dim() != 1 || qs->size(0) != B + 1)) fail("q_start must have a value for each sequence and one more");
+    if (!qs && (B == 0 ? n_rows != 0 : n_rows % B != 0)) fail("without q_start every sequence has as many rows as the others");
+    constexpr int64_t most = INT32_MAX;
+    if (n_rows > most || B > most || pages > most || table.size(1) > most || kp.size(2) > most || kp.size(3) > most || heads > most) fail("sizes must fit 32 bits");
+    c.kv.k_pages = kp.data_ptr();
+    c.kv.v_pages = vpg.data_ptr();
+    c.kv.k_scale = static_cast<float*>(ks.data_ptr());
+    c.kv.v_scale = static_cast<float*>(vs.data_ptr());
+    c.kv.table = static_cast<const int32_t*>(table.const_data_ptr());
+    c.kv.table_stride = B > 1 ? table.stride(0) : std::max<int64_t>(table.size(1), 1);
+    c.kv.dtype = t == at::kChar ? GLQ_KV_I8 : GLQ_KV_E4M3;
+    c.kv.n_pages = (int32_t)pages;
+    c.kv.n_kv = (int32_t)heads;
+    c.kv.page = (int32_t)kp.size(2);
+    c.kv.head_dim = (int32_t)kp.size(3);
+    c.kv.max_pages = (int32_t)table.size(1);
+    c.rows.start = start.const_data_ptr<int64_t>();
+    c.rows.start_stride = start.size(0) == 1 ? 0 : 1;
+    c.rows.q_start = qs ? qs->const_data_ptr<int32_t>() : nullptr;
+    c.rows.B = (int32_t)B;
+    c.rows.rows = (int32_t)n_rows;
+    c.rows.max_new = (int32_t)std::min(max_new < 0 ? n_rows : max_new, n_rows);
+    c.pages = &kp;
+    return c;
+}
+// fp16 rows (N, heads, head size) with any distance between rows
+int64_t paged_rows(const at::Tensor& x, const char* name, const PagedCall& c, int64_t n_rows, int64_t heads) {
+    const int64_t D = c.kv.head_dim;
+    if (!x.is_cuda() || x.device() != c.pages->device()) fail(std::string(name) + " must be a CUDA tensor on the device of the pages");
+    if (x.scalar_type() != at::kHalf) fail(std::string(name) + " must be torch.float16");
+    if (x.dim() != 3 || x.size(0) != n_rows || x.size(2) != D || (heads >= 0 && x.size(1) != heads))
+        fail(std::string(name) + " must be (rows, heads, head size)");
+    if (n_rows > 0 && x.size(1) > 0 && (x.stride(2) != 1 || (x.size(1) > 1 && x.stride(1) != D))) fail(std::string(name) + ": the heads of a row must be consecutive");
+    return n_rows > 1 ? x.stride(0) : std::max<int64_t>(x.size(1), 1) * D;
+}
+cudaStream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// q or None, k, v, cos or None, sin or None, <cache: 5 tensors>, start, q_start or None, q_norm or None, k_norm or None, eps, q_out or None
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        nargs_are(n, 16);
+        const at::Tensor *q = tensor_or_none(a[0], "q"), *cos = tensor_or_none(a[3], "cos"), *sin = tensor_or_none(a[4], "sin");
+        const at::Tensor &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
+        const int64_t N = k.dim() > 0 ? k.size(0) : 0;
+        const PagedCall c = paged_call(a + 5, N, -1);
+        const int64_t ldk = paged_rows(k, "k", c, N, c.kv.n_kv), ldv = paged_rows(v, "v", c, N, c.kv.n_kv);
+        const int64_t ldq = q ? paged_rows(*q, "q", c, N, -1) : 0;
+        if (!cos != !sin) fail("cos and sin come together");
+        if (cos) {
+            beside(a[3], "cos", at::kFloat, "torch.float32", *c.pages);
+            beside(a[4], "sin", at::kFloat, "torch.float32", *c.pages);
+            if (cos->dim() != 2 || cos->size(1) != c.kv.head_dim / 2 || sin->sizes() != cos->sizes()) fail("cos and sin must be (positions, head size / 2)");
+            if (cos->size(0) < (int64_t)c.kv.max_pages * c.kv.page || cos->size(0) > INT32_MAX) fail("cos and sin must have a row for every position that the page table holds");
+        }
+        const at::Tensor* norms[2];
+        for (int i = 0; i < 2; ++i) {
+            norms[i] = a[12 + i] == Py_None ? nullptr : &beside(a[12 + i], i ? "k_norm" : "q_norm", at::kHalf, "torch.float16", *c.pages);
+            if (norms[i] && norms[i]->numel() != c.kv.head_dim) fail("q_norm and k_norm must have a value for each channel of a head");
+        }
+        if (q && !norms[0] != !norms[1]) fail("q_norm and k_norm come together");
+        const float eps = number(a[14]);
+        c10::cuda::OptionalCUDAGuard guard(c.pages->device());
+        at::Tensor out;
+        int64_t ldo = 0;
+        if (q) {
+            out = a[15] == Py_None ? empty({N, q->size(1), q->size(2)}, at::kHalf, *q) : tensor(a[15], "q_out");
+            ldo = paged_rows(out, "q_out", c, N, q->size(1));
+        }
+        const cudaStream_t st = stream_of(*c.pages);
+        if (N > 0 && c.rows.B > 0) launch(st, "paged_append", [&] {
+            return api.glq_paged_append(&c.kv, &c.rows, ptr(q), ldq, k.const_data_ptr(), ldk, v.const_data_ptr(), ldv,
+                                        q ? out.mutable_data_ptr() : nullptr, ldo, q ? (int)q->size(1) : 0, static_cast<const float*>(ptr(cos)),
+                                        static_cast<const float*>(ptr(sin)), cos ? (int)cos->size(0) : 0, ptr(norms[0]), ptr(norms[1]), eps, st);
+        });
+        if (!q) Py_RETURN_NONE;
+        return wrap(out);
+    });
+}
+
+// q, <cache: 5 tensors>, start, q_start or None, max_new (below 0: not known), scale, out or None
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&] {
+        nargs_are(n, 11);
+        const at::Tensor& q = tensor(a[0], "q");
+        const int64_t N = q.dim() > 0 ? q.size(0) : 0;
+        const PagedCall c = paged_call(a + 1, N, integer(a[8]));
+        const int64_t ldq = paged_rows(q, "q", c, N, -1);
+        const int heads = (int)q.size(1);
+        if (heads <= 0 || heads % c.kv.n_kv) fail("q must have a multiple of the cache's heads");
+        const float scale = number(a[9]);
+        c10::cuda::OptionalCUDAGuard guard(c.pages->device());
+        at::Tensor out = a[10] == Py_None ? empty({N, q.size(1), q.size(2)}, at::kHalf, q) : tensor(a[10], "out");
+        const int64_t ldo = paged_rows(out, "out", c, N, heads);
+        const cudaStream_t st = stream_of(*c.pages);
+        // partial results: a buffer of the call's own (captured calls each have theirs, as calls on several streams do)
+        const size_t bytes = api.glq_paged_attention_workspace_bytes(&c.kv, &c.rows, heads);
+        const at::Tensor ws = bytes ? empty({(int64_t)bytes}, at::kByte, q) : at::Tensor();
+        if (N > 0 && c.rows.B > 0) launch(st, "paged_attention", [&] {
+            return api.glq_paged_attention(&c.kv, &c.rows, q.const_data_ptr(), ldq, out.mutable_data_ptr(), ldo, heads, scale,
+                                           bytes ? ws.mutable_data_ptr() : nullptr, bytes, st);
+        });
+        return wrap(out);
+    });
+}
+
+// <cache: 5 tensors>, start, q_start or None, rows -> keys, values (rows, heads, head size)
+PyObject* py_paged_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&] {
+        nargs_are(n, 8);
+        const int64_t N = integer(a[7]);
+        if (N < 0) fail("rows must not be negative");
+        const PagedCall c = paged_call(a, N, -1);
+        c10::cuda::OptionalCUDAGuard guard(c.pages->device());
+        at::Tensor k = empty({N, c.kv.n_kv, c.kv.head_dim}, at::kHalf, *c.pages), v = empty({N, c.kv.n_kv, c.kv.head_dim}, at::kHalf, *c.pages);
+        const cudaStream_t st = stream_of(*c.pages);
+        if (N > 0 && c.rows.B > 0) launch(st, "paged_read", [&] { return api.glq_paged_read(&c.kv, &c.rows, k.mutable_data_ptr(), v.mutable_data_ptr(), st); });
+        return Py_BuildValue("NN", wrap(k), wrap(v));
+    });
+}
+
 PyObject* py_bind(PyObject*, PyObject* d) {   // {entry point: address}
 #define GLQ_FN(name)                                                                              \
     if (PyObject* v = PyDict_GetItemString(d, #name)) api.name = reinterpret_cast<decltype(api.name)>(PyLong_AsVoidPtr(v)); \
@@ -633,6 +792,7 @@ PyObject* py_names(PyObject*, PyObject*) {
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(workspace), FAST(layer), FAST(linear), FAST(group), FAST(grouped_linear), FAST(turbo_matmul),
                          FAST(turbo_grouped_gemv), FAST(gptq_matmul), FAST(block), FAST(block_scratch), FAST(moe), FAST(add_rmsnorm),
+                         FAST(paged_append), FAST(paged_attention), FAST(paged_read),
                          {"bind", py_bind, METH_O, nullptr}, {"names", py_names, METH_NOARGS, nullptr},
                          {"clear_workspaces", py_clear_workspaces, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "glorcq_b200._native", nullptr, -1, methods};

@@ -1,0 +1,632 @@
+// Paged key/value cache in 8 bits: writing new tokens (glq_paged_append), attention (glq_paged_attention) and reading rows
+// back (glq_paged_read).  include/glorcq_b200.h has the definitions, paged.cuh what the kernels share.
+#include <algorithm>
+
+#include "paged.cuh"
+
+using namespace glq;
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Append.  A block of a page and head is one CTA's: its scale needs the largest value of all new tokens before a code can be written.  The values
+// are computed twice (second time from the first-level cache) unless one pass of the CTA covers them.  Two halves of a row that the
+// rotation mixes belong to one lane: lane c of HD / 16 has channels 8c .. 8c+7 and HD/2 + 8c .. .  Bound by memory.
+// ---------------------------------------------------------------------------------------------
+constexpr int kAppendThreads = 128;
+
+struct AppendParams {
+    PagedKv kv;
+    PagedRows r;
+    const __half *q, *k, *v, *q_norm, *k_norm;
+    __half* q_out;
+    const float *cos, *sin;
+    long long ldq, ldk, ldv, ldqo;
+    int n_heads, page_items, cos_rows;
+    float eps;
+};
+
+struct RowHalves {
+    float a[8], b[8];      // first half's channels, second half's
+};
+__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
+    __align__(16) __half h[8];
+    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __half2float(h[i]);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
+    __align__(16) __half h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = __float2half_rn(f[i]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
+// Norm and rotation of one row by its HD / 16 lanes, in fp32; products and sums rounded one by one, so that they do not depend on
+// what the compiler contracts.  pos < 0: no rotation.
+template <int HD>
+__device__ __forceinline__ void norm_rotate(RowHalves& x, const __half* norm, float eps, const float* cos, const float* sin, int pos, int c) {
+    constexpr int LPR = HD / 16;
+    if (norm) {
+        float ss = 0.f, wa[8], wb[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
+#pragma unroll
+        for (int d = LPR / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        const float r = rsqrtf(ss / HD + eps);
+        load8(norm + 8 * c, wa);
+        load8(norm + HD / 2 + 8 * c, wb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x.a[i] = x.a[i] * r * wa[i];
+            x.b[i] = x.b[i] * r * wb[i];
+        }
+    }
+    if (cos && pos >= 0) {
+        __align__(16) float cs[8], sn[8];
+        const float4* cp = reinterpret_cast<const float4*>(cos + (size_t)pos * (HD / 2) + 8 * c);
+        const float4* sp = reinterpret_cast<const float4*>(sin + (size_t)pos * (HD / 2) + 8 * c);
+        reinterpret_cast<float4*>(cs)[0] = cp[0];
+        reinterpret_cast<float4*>(cs)[1] = cp[1];
+        reinterpret_cast<float4*>(sn)[0] = sp[0];
+        reinterpret_cast<float4*>(sn)[1] = sp[1];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = __fsub_rn(__fmul_rn(x.a[i], cs[i]), __fmul_rn(x.b[i], sn[i]));
+            x.b[i] = __fadd_rn(__fmul_rn(x.b[i], cs[i]), __fmul_rn(x.a[i], sn[i]));
+            x.a[i] = a;
+        }
+    }
+}
+
+template <int DT> __device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv) {
+    uint2 w = make_uint2(0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w.x |= to_code<DT>(__fmul_rn(f[i], inv)) << (8 * i);
+        w.y |= to_code<DT>(__fmul_rn(f[i + 4], inv)) << (8 * i);
+    }
+    return w;
+}
+
+template <int HD, int DT>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
+    constexpr int LPR = HD / 16, RPP = kAppendThreads / LPR;       // lanes of a row, rows of a pass
+    const int tid = threadIdx.x, c = tid % LPR, slot = tid / LPR;
+    after_launch_ahead();
+    const int block_items = p.page_items * 2 * p.kv.n_kv;
+    if ((int)blockIdx.x >= block_items) {                          // queries: 2 RPP (row, head) pairs
+        const long long total = (long long)p.r.N * p.n_heads;
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u) {
+            const long long i = ((long long)((int)blockIdx.x - block_items) * 2 + u) * RPP + slot;
+            const bool live = i < total;
+            const int row = live ? (int)(i / p.n_heads) : 0, h = live ? (int)(i - (long long)row * p.n_heads) : 0;
+            // rows in front of the first sequence or behind the last are not touched
+            const int b = last_from(p.r.B, row, [&](int b) { return rows_from(p.r, b); });
+            const int2 own = rows_of(p.r, b);
+            const bool mine = live && row >= own.x && row - own.x < own.y;
+            RowHalves x = {};
+            if (mine) {
+                const __half* src = p.q + row * p.ldq + h * HD + 8 * c;
+                load8(src, x.a);
+                load8(src + HD / 2, x.b);
+            }
+            const long long at = mine ? (long long)start_of(p.r, b, p.kv.capacity) + (row - own.x) : 0;
+            norm_rotate<HD>(x, p.q_norm, p.eps, p.cos, p.sin, (int)min(at, (long long)p.cos_rows - 1), c);
+            if (mine) {
+                __half* dst = p.q_out + row * p.ldqo + h * HD + 8 * c;
+                store8(dst, x.a);
+                store8(dst + HD / 2, x.b);
+            }
+        }
+        return;
+    }
+    const int hz = blockIdx.x % (2 * p.kv.n_kv), item = blockIdx.x / (2 * p.kv.n_kv);
+    const int h = hz >> 1;
+    const bool is_k = (hz & 1) == 0;
+    // sequence b's blocks are items rows / page + 2 b ..: n rows lie in at most (n - 2) / page + 2 pages
+    auto first = [&](int b) { return (rows_from(p.r, b) >> p.kv.page_shift) + 2 * b; };
+    const int b = last_from(p.r.B, item, first);
+    if (item < first(b)) return;       // (rows in front of the first sequence)
+    const int2 own = rows_of(p.r, b);
+    const int start = start_of(p.r, b, p.kv.capacity);
+    const int j = item - first(b) + (start >> p.kv.page_shift);
+    const int at = j << p.kv.page_shift;
+    if (own.y == 0 || (long long)at >= (long long)start + own.y) return;
+    const int phys = page_of(p.kv, b, j);
+    if (phys < 0) return;
+    const int s0 = max(start - at, 0), s1 = (int)min((long long)start + own.y - at, (long long)p.kv.page);
+    const size_t block = (size_t)phys * p.kv.n_kv + h;
+    unsigned char* codes = (is_k ? p.kv.k : p.kv.v) + block * ((size_t)HD << p.kv.page_shift);
+    float* scale_at = (is_k ? p.kv.k_scale : p.kv.v_scale) + block;
+    const __half* src = (is_k ? p.k : p.v) + (long long)(own.x + at - start) * (is_k ? p.ldk : p.ldv) + h * HD + 8 * c;
+    const long long ld = is_k ? p.ldk : p.ldv;
+    const float old = *scale_at;
+
+    RowHalves x;
+    auto row_values = [&](int s) {
+        x = RowHalves{};
+        if (s < s1) {
+            load8(src + s * ld, x.a);
+            load8(src + s * ld + HD / 2, x.b);
+        }
+        if (is_k) norm_rotate<HD>(x, p.k_norm, p.eps, p.cos, p.sin, s < s1 ? at + s : -1, c);
+    };
+    float big = 0.f;
+    for (int s = s0; s < s1; s += RPP) {       // (whole warps stay together for the norm's shuffles)
+        row_values(s + slot);
+        if (s + slot < s1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float u = fabsf(x.a[i]), w = fabsf(x.b[i]);
+                big = fmaxf(big, u <= FLT_MAX ? u : 0.f);
+                big = fmaxf(big, w <= FLT_MAX ? w : 0.f);
+            }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+    __shared__ float red[kAppendThreads / 32];
+    if ((tid & 31) == 0) red[tid >> 5] = big;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) big = fmaxf(big, red[w]);
+    const float need = big / kCodeMax<DT>;
+    float scale = need;
+    if (s0 > 0 && old > 0.f) {
+        scale = old;
+        if (need > old) {
+            int e0, e1;
+            const float m0 = frexpf(old, &e0), m1 = frexpf(need, &e1);
+            const int n = e1 - e0 + (m1 > m0 ? 1 : 0);
+            scale = ldexpf(old, n);
+            const float down = ldexpf(1.f, -n);
+            for (int w = tid; w < s0 * (HD / 4); w += kAppendThreads) {
+                uint32_t v = reinterpret_cast<uint32_t*>(codes)[w], o = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o |= to_code<DT>(code_value<DT>((v >> (8 * i)) & 0xffu) * down) << (8 * i);
+                reinterpret_cast<uint32_t*>(codes)[w] = o;
+            }
+        }
+    }
+    if (tid == 0 && scale != old) *scale_at = scale;
+    const float inv = scale > 0.f ? 1.f / scale : 0.f;
+    const bool again = s1 - s0 > RPP;
+    for (int s = s0; s < s1; s += RPP) {
+        if (again) row_values(s + slot);
+        if (s + slot < s1) {
+            unsigned char* dst = codes + (size_t)(s + slot) * HD + 8 * c;
+            *reinterpret_cast<uint2*>(dst) = codes8<DT>(x.a, inv);
+            *reinterpret_cast<uint2*>(dst + HD / 2) = codes8<DT>(x.b, inv);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Read: HD / 16 lanes a (row, head), keys and values.  Bound by memory.
+// ---------------------------------------------------------------------------------------------
+struct ReadParams {
+    PagedKv kv;
+    PagedRows r;
+    __half *k_out, *v_out;
+};
+constexpr int kReadThreads = 256;
+
+template <int HD, int DT>
+__global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const ReadParams p) {
+    constexpr int LPR = HD / 16, RPP = kReadThreads / LPR;
+    const int c = threadIdx.x % LPR;
+    const long long i = (long long)blockIdx.x * RPP + threadIdx.x / LPR;
+    after_launch_ahead();
+    if (i >= (long long)p.r.N * p.kv.n_kv) return;
+    const int row = (int)(i / p.kv.n_kv), h = (int)(i - (long long)row * p.kv.n_kv);
+    const int b = last_from(p.r.B, row, [&](int b) { return rows_from(p.r, b); });
+    const int2 own = rows_of(p.r, b);
+    if (row < own.x || row - own.x >= own.y) return;
+    const long long at = (long long)start_of(p.r, b, p.kv.capacity) + (row - own.x);
+    const int phys = at < p.kv.capacity ? page_of(p.kv, b, (int)(at >> p.kv.page_shift)) : -1;
+    uint4 kw = make_uint4(0u, 0u, 0u, 0u), vw = kw;
+    float ks = 0.f, vs = 0.f;
+    if (phys >= 0) {
+        const size_t block = (size_t)phys * p.kv.n_kv + h;
+        const size_t off = ((block << p.kv.page_shift) + (at & (p.kv.page - 1))) * HD + 16 * c;
+        kw = *reinterpret_cast<const uint4*>(p.kv.k + off);
+        vw = *reinterpret_cast<const uint4*>(p.kv.v + off);
+        ks = p.kv.k_scale[block] * kCodeUnit<DT>;
+        vs = p.kv.v_scale[block] * kCodeUnit<DT>;
+    }
+    auto put = [&](const uint4& w, float s, __half* out) {
+        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+        __align__(16) __half2 o[8];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint32_t lo, hi;
+            codes_to_half<DT>(in[u], lo, hi);
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), d = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            o[2 * u] = __floats2half2_rn(a.x * s, a.y * s);
+            o[2 * u + 1] = __floats2half2_rn(d.x * s, d.y * s);
+        }
+        uint4* dst = reinterpret_cast<uint4*>(out + ((size_t)row * p.kv.n_kv + h) * HD + 16 * c);
+        dst[0] = reinterpret_cast<const uint4*>(o)[0];
+        dst[1] = reinterpret_cast<const uint4*>(o)[1];
+    };
+    put(kw, ks, p.k_out);
+    put(vw, vs, p.v_out);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention of few rows a key/value head (a decoded token: the heads of the group).  A warp takes 16 tokens a step; scores S^T
+// = K q^T and outputs O^T += V^T P^T on m16n8k16 with the tokens resp. channels as M and eight rows (token of the call, head of the group) as N, so that codes
+// go from 16-byte loads through a few register instructions into fragments:
+//   keys    lane (g, t) loads tokens g and g + 8, 16-byte pieces t, t + 4, ..: any assignment of channels to k positions serves, as
+//           long as q's fragments have the same.
+//   values  lane (g, t) loads piece g of tokens 2t, 2t+1, 2t+8, 2t+9, the k positions of its fragment; bytes of two tokens are
+//           interleaved, then expanded.
+//   P       movmatrix transposes the scores' fragment (tokens by g) into the second product's (tokens by t).
+// Scales: c = ks * scale * log2(e) multiplies a score; vs goes into the exponent, w = 2^(c s + log2 vs - m), so that probabilities are rounded
+// to fp16 relative to the largest contribution; the sum of the softmax is that of w / vs in fp32.  The maximum m is raised only when a score
+// exceeds it by 2^8 (w stays below 256 in fp16), by a vote, so that a step has no shuffles as a rule.
+// ---------------------------------------------------------------------------------------------
+constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32;
+
+struct AttnParams {
+    PagedKv kv;
+    PagedRows r;
+    const __half* q;
+    __half* out;
+    long long ldq, ldo;
+    int n_heads, group;
+    float scale2;           // softmax scale * log2(e) * kCodeUnit
+};
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+__device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; -inf -> 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// codes that one CTA alone reads: not kept in the first-level cache
+template <int WORDS> __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t* w) {
+    if (WORDS == 4)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+    else if (WORDS == 2)
+        asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    else
+        asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+}
+
+template <int HD, int DT, int NB>
+__global__ void __launch_bounds__(kRowsThreads, HD == 256 || NB == 2 ? 1 : 2) paged_attention_rows_kernel(const AttnParams p) {
+    constexpr int R = 8 * NB;                       // rows of a block
+    constexpr int KW = HD / 16, VW = HD / 32;       // code words of a lane: per key row, per value row
+    constexpr int KC = KW < 4 ? KW : 4, VC = VW < 4 ? VW : 4;       // words of one load
+    extern __shared__ float sm_rows[];
+    float* sm_o = sm_rows;                                         // [warp][R][HD]
+    float* sm_m = sm_o + kRowsWarps * R * HD;                      // [warp][R], then weights
+    float* sm_l = sm_m + kRowsWarps * R;                           // [warp][R]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y;
+    after_launch_ahead();
+    // row blocks of sequence b: from rows * group / R + b on
+    auto first = [&](int b) { return (int)((long long)rows_from(p.r, b) * p.group / R) + b; };
+    const int b = last_from(p.r.B, (int)blockIdx.x, first);
+    if ((int)blockIdx.x < first(b)) return;       // (rows in front of the first sequence)
+    const int2 own = rows_of(p.r, b);
+    const int r0 = ((int)blockIdx.x - first(b)) * R, n_rows = min(own.y * p.group - r0, R);
+    if (n_rows <= 0) return;
+    const int start = start_of(p.r, b, p.kv.capacity);
+    const int limit_all = min(start + (r0 + n_rows - 1) / p.group, p.kv.capacity - 1);       // the last key that a row sees
+    const int n_tiles = limit_all / 16 + 1;
+
+    uint32_t qf[NB][KW][2];
+    int limit[NB][2];
+    float m[NB][2], l[NB][2], o[NB][2 * VW][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int r = r0 + 8 * n + g;
+        const bool live = 8 * n + g < n_rows;
+        const __half* src = p.q + (long long)(own.x + (live ? r / p.group : 0)) * p.ldq + (h * p.group + (live ? r % p.group : 0)) * HD;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const int ch = KW < 4 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
+            const uint2 v = live ? *reinterpret_cast<const uint2*>(src + ch) : make_uint2(0u, 0u);
+            qf[n][w][0] = v.x;
+            qf[n][w][1] = v.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int rr = 8 * n + 2 * t + e;
+            limit[n][e] = rr < n_rows ? min(start + (r0 + rr) / p.group, p.kv.capacity - 1) : -1;
+            m[n][e] = -1e30f;
+            l[n][e] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * VW; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+    }
+    const int limit_low = min(start + r0 / p.group, p.kv.capacity - 1);       // keys up to here are seen by every live row
+
+    uint32_t kw[2][KW], vw[4][VW];
+    float ks, vs;
+    auto lookup = [&](int tile) { return tile < n_tiles ? page_of(p.kv, b, tile * 16 >> p.kv.page_shift) : -1; };
+    auto load_k = [&](int tile, int phys) {
+        ks = 0.f;
+        if (phys >= 0) {
+            const size_t block = (size_t)phys * p.kv.n_kv + h;
+            ks = p.kv.k_scale[block];
+            const unsigned char* src = p.kv.k + ((block << p.kv.page_shift) + ((tile * 16) & (p.kv.page - 1)) + g) * HD + t * 4 * KC;
+#pragma unroll
+            for (int c = 0; c < KW / KC; ++c) {
+                load_words<KC>(src + 64 * c, &kw[0][KC * c]);
+                load_words<KC>(src + 8 * HD + 64 * c, &kw[1][KC * c]);
+            }
+        }
+    };
+    auto load_v = [&](int tile, int phys) {
+        vs = 0.f;
+        if (phys >= 0) {
+            const size_t block = (size_t)phys * p.kv.n_kv + h;
+            vs = p.kv.v_scale[block];
+            const unsigned char* src = p.kv.v + ((block << p.kv.page_shift) + ((tile * 16) & (p.kv.page - 1)) + 2 * t) * HD + g * 4 * VC;
+#pragma unroll
+            for (int c = 0; c < VW / VC; ++c)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) load_words<VC>(src + ((u & 1) + 8 * (u >> 1)) * HD + 128 * c, &vw[u][VC * c]);
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < KW; ++w) kw[u][w] = 0u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vw[u][w] = 0u;
+
+    int phys = lookup(warp), phys1 = lookup(warp + kRowsWarps);
+    load_k(warp, phys);
+    load_v(warp, phys);
+    for (int tile = warp; tile < n_tiles; tile += kRowsWarps) {
+        float s[NB][4];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_half<DT>(kw[0][w], a0, a2);
+            codes_to_half<DT>(kw[1][w], a1, a3);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) mma16816(s[n], a0, a1, a2, a3, qf[n][w][0], qf[n][w][1]);
+        }
+        const float c = ks * p.scale2, vscale = vs;
+        const int phys2 = lookup(tile + 2 * kRowsWarps);
+        load_k(tile + kRowsWarps, phys1);
+        const float lv = vscale > 0.f ? log2f(vscale) : 0.f, iv = vscale > 0.f ? 1.f / vscale : 1.f;
+        // w of token g (+ 8) and rows 2t, 2t + 1 of each block of rows
+        uint32_t pf[NB][2];
+        const bool masked = tile * 16 + 15 > limit_low || phys < 0;
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int tok = tile * 16 + g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] = s[n][e] * c + lv;
+                if (masked && (phys < 0 || tok + 8 * (e >> 1) > limit[n][e & 1])) s[n][e] = -INFINITY;
+            }
+            const float hi0 = fmaxf(s[n][0], s[n][2]), hi1 = fmaxf(s[n][1], s[n][3]);
+            if (__any_sync(0xffffffffu, hi0 > m[n][0] + 8.f || hi1 > m[n][1] + 8.f)) {
+                float x0 = fmaxf(hi0, m[n][0]), x1 = fmaxf(hi1, m[n][1]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+                }
+                const float f0 = exp2_fast(m[n][0] - x0), f1 = exp2_fast(m[n][1] - x1);
+                m[n][0] = x0;
+                m[n][1] = x1;
+                l[n][0] *= f0;
+                l[n][1] *= f1;
+#pragma unroll
+                for (int i = 0; i < 2 * VW; ++i) {
+                    o[n][i][0] *= f0;
+                    o[n][i][1] *= f1;
+                    o[n][i][2] *= f0;
+                    o[n][i][3] *= f1;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = exp2_fast(s[n][e] - m[n][e & 1]);
+            l[n][0] += (s[n][0] + s[n][2]) * iv;
+            l[n][1] += (s[n][1] + s[n][3]) * iv;
+            pf[n][0] = transpose8x8(vscale > 0.f ? pack_half2(s[n][0], s[n][1]) : 0u);
+            pf[n][1] = transpose8x8(vscale > 0.f ? pack_half2(s[n][2], s[n][3]) : 0u);
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t sel = half ? 0x7362u : 0x5140u;
+                uint32_t a0, a1, a2, a3;
+                codes_to_half<DT>(prmt(vw[0][w], vw[1][w], sel), a0, a1);
+                codes_to_half<DT>(prmt(vw[2][w], vw[3][w], sel), a2, a3);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) mma16816(o[n][2 * w + half], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+            }
+        }
+        load_v(tile + kRowsWarps, phys1);
+        phys = phys1;
+        phys1 = phys2;
+    }
+    // the warps' results meet in shared memory
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+            const int r = 8 * n + 2 * t + e;
+            if (g == 0) {
+                sm_m[warp * R + r] = m[n][e];
+                sm_l[warp * R + r] = l[n][e];
+            }
+            float* dst = sm_o + (warp * R + r) * HD;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+                const int ch = VW < 4 ? 4 * VW * g + 4 * w : 128 * (w / 4) + 16 * g + 4 * (w % 4);
+                *reinterpret_cast<float4*>(dst + ch) = make_float4(o[n][2 * w][e], o[n][2 * w][e + 2], o[n][2 * w + 1][e], o[n][2 * w + 1][e + 2]);
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n_rows * (HD / 4); i += kRowsThreads) {
+        const int r = i / (HD / 4), ch = i % (HD / 4) * 4;
+        float mx = -1e30f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) mx = fmaxf(mx, sm_m[w * R + r]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) {
+            const float f = exp2_fast(sm_m[w * R + r] - mx);
+            const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * R + r) * HD + ch);
+            sum += sm_l[w * R + r] * f;
+            acc.x += v.x * f;
+            acc.y += v.y * f;
+            acc.z += v.z * f;
+            acc.w += v.w * f;
+        }
+        const float inv = sum > 0.f ? kCodeUnit<DT> / sum : (sum == 0.f ? 0.f : sum);      // (not-a-number stays)
+        __half2 o2[2] = {__floats2half2_rn(acc.x * inv, acc.y * inv), __floats2half2_rn(acc.z * inv, acc.w * inv)};
+        const int rr = r0 + r;
+        __half* dst = p.out + (long long)(own.x + rr / p.group) * p.ldo + (h * p.group + rr % p.group) * HD + ch;
+        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o2);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int check_cache(const glq_paged_kv_t* kv, const glq_paged_rows_t* r) {
+    if (!kv || !r || !kv->k_pages || !kv->v_pages || !kv->k_scale || !kv->v_scale || !kv->table || !r->start) return GLQ_ERR_ARG;
+    if (kv->dtype != GLQ_KV_I8 && kv->dtype != GLQ_KV_E4M3) return GLQ_ERR_UNSUPPORTED;
+    if (kv->head_dim != 32 && kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256) return GLQ_ERR_UNSUPPORTED;
+    if (kv->page != 16 && kv->page != 32 && kv->page != 64 && kv->page != 128) return GLQ_ERR_UNSUPPORTED;
+    if (kv->n_pages <= 0 || kv->n_kv <= 0 || kv->max_pages <= 0 || kv->table_stride < kv->max_pages) return GLQ_ERR_ARG;
+    if ((long long)kv->max_pages * kv->page >= 1 << 30 || kv->n_kv > 1024) return GLQ_ERR_UNSUPPORTED;
+    if (r->B < 0 || r->rows < 0 || r->rows >= 1 << 28 || (r->start_stride != 0 && r->start_stride != 1)) return GLQ_ERR_ARG;
+    if (!r->q_start && r->B > 0 && r->rows % r->B != 0) return GLQ_ERR_ARG;
+    if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages)) return GLQ_ERR_ALIGN;
+    return GLQ_OK;
+}
+PagedKv device_kv(const glq_paged_kv_t* kv) {
+    int shift = 0;
+    while ((1 << shift) < kv->page) ++shift;
+    return {static_cast<unsigned char*>(kv->k_pages), static_cast<unsigned char*>(kv->v_pages), kv->k_scale, kv->v_scale, kv->table,
+            kv->table_stride, kv->n_pages, kv->n_kv, kv->page, shift, kv->max_pages, kv->max_pages * kv->page};
+}
+PagedRows device_rows(const glq_paged_rows_t* r) {
+    return {reinterpret_cast<const long long*>(r->start), r->q_start, r->B, r->rows, r->q_start ? 0 : r->rows / r->B, r->start_stride};
+}
+
+// f<head size, code type>()
+template <class F> int by_type(const glq_paged_kv_t* kv, F&& f) {
+#define GLQ_PAGED_CASE(HD)                                                                             \
+    case HD:                                                                                           \
+        return kv->dtype == GLQ_KV_I8 ? f(std::integral_constant<int, HD>{}, std::integral_constant<int, kI8>{}) \
+                                      : f(std::integral_constant<int, HD>{}, std::integral_constant<int, kE4M3>{});
+    switch (kv->head_dim) {
+        GLQ_PAGED_CASE(32)
+        GLQ_PAGED_CASE(64)
+        GLQ_PAGED_CASE(128)
+        GLQ_PAGED_CASE(256)
+    }
+#undef GLQ_PAGED_CASE
+    return GLQ_ERR_UNSUPPORTED;
+}
+
+}  // namespace
+
+extern "C" int glq_paged_append(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                                const void* v, int64_t ldv, void* q_out, int64_t ldqo, int n_heads, const float* cos, const float* sin,
+                                int cos_rows, const void* q_norm, const void* k_norm, float eps, void* stream) {
+    const int bad = check_cache(kv, rows);
+    if (bad != GLQ_OK) return bad;
+    if (rows->rows == 0 || rows->B == 0) return GLQ_OK;
+    if (!k || !v || (q && (!q_out || n_heads <= 0)) || (!cos != !sin) || (!q_norm != !k_norm && q)) return GLQ_ERR_ARG;
+    if (cos && cos_rows < kv->max_pages * kv->page) return GLQ_ERR_ARG;
+    const int width = kv->n_kv * kv->head_dim;
+    if (ldk < width || ldv < width || (q && (ldq < (int64_t)n_heads * kv->head_dim || ldqo < (int64_t)n_heads * kv->head_dim))) return GLQ_ERR_ARG;
+    if (ldk % 8 || ldv % 8 || (q && (ldq % 8 || ldqo % 8))) return GLQ_ERR_ALIGN;
+    for (const void* ptr : {k, v, q, (const void*)q_out, (const void*)cos, (const void*)sin, q_norm, k_norm})
+        if (!aligned16(ptr)) return GLQ_ERR_ALIGN;
+    return by_type(kv, [&](auto hd, auto dt) {
+        constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
+        AppendParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<const __half*>(k),
+                       static_cast<const __half*>(v), static_cast<const __half*>(q_norm), static_cast<const __half*>(k_norm),
+                       static_cast<__half*>(q_out), cos, sin, ldq, ldk, ldv, ldqo, n_heads, 0, cos_rows, eps};
+        const long long items = (long long)rows->rows / kv->page + 2ll * rows->B, per = 2 * (kAppendThreads / (HD / 16));
+        const long long grid = items * 2 * kv->n_kv + (q ? ((long long)rows->rows * n_heads + per - 1) / per : 0);
+        if (items * 2 * kv->n_kv > 0x3fffffffll || grid > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
+        p.page_items = (int)items;
+        return launch_kernel(true, paged_append_kernel<HD, DT>, dim3((unsigned)grid), dim3(kAppendThreads), 0,
+                             reinterpret_cast<cudaStream_t>(stream), p) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
+    });
+}
+
+extern "C" int glq_paged_read(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, void* k_out, void* v_out, void* stream) {
+    const int bad = check_cache(kv, rows);
+    if (bad != GLQ_OK) return bad;
+    if (rows->rows == 0 || rows->B == 0) return GLQ_OK;
+    if (!k_out || !v_out) return GLQ_ERR_ARG;
+    if (!aligned16(k_out) || !aligned16(v_out)) return GLQ_ERR_ALIGN;
+    return by_type(kv, [&](auto hd, auto dt) {
+        constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
+        const ReadParams p{device_kv(kv), device_rows(rows), static_cast<__half*>(k_out), static_cast<__half*>(v_out)};
+        const long long grid = ((long long)rows->rows * kv->n_kv + kReadThreads / (HD / 16) - 1) / (kReadThreads / (HD / 16));
+        if (grid > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
+        return launch_kernel(true, paged_read_kernel<HD, DT>, dim3((unsigned)grid), dim3(kReadThreads), 0, reinterpret_cast<cudaStream_t>(stream),
+                             p) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
+    });
+}
+
+extern "C" size_t glq_paged_attention_workspace_bytes(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
+    (void)kv, (void)rows, (void)n_heads;
+    return 0;
+}
+
+extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, void* out,
+                                   int64_t ldo, int n_heads, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    (void)workspace, (void)workspace_bytes;
+    const int bad = check_cache(kv, rows);
+    if (bad != GLQ_OK) return bad;
+    if (rows->rows == 0 || rows->B == 0) return GLQ_OK;
+    if (!q || !out || n_heads <= 0 || n_heads % kv->n_kv != 0 || (rows->q_start && rows->max_new < 0)) return GLQ_ERR_ARG;
+    if (ldq < (int64_t)n_heads * kv->head_dim || ldo < (int64_t)n_heads * kv->head_dim) return GLQ_ERR_ARG;
+    if (ldq % 8 || ldo % 8 || !aligned16(q) || !aligned16(out)) return GLQ_ERR_ALIGN;
+    if ((long long)rows->rows * n_heads > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
+    return by_type(kv, [&](auto hd, auto dt) {
+        constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
+        const int group = n_heads / kv->n_kv;
+        const AttnParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<__half*>(out), ldq, ldo, n_heads,
+                           group, scale * 1.4426950408889634f * kCodeUnit<DT>};
+        const int most = rows->q_start ? std::min(rows->max_new, rows->rows) : rows->rows / rows->B;
+        auto run = [&](auto nb) {
+            constexpr int NB = decltype(nb)::value, R = 8 * NB;
+            constexpr size_t smem = (size_t)kRowsWarps * R * (HD + 2) * sizeof(float);
+            static SmemLimit limit;
+            auto* kern = paged_attention_rows_kernel<HD, DT, NB>;
+            const long long blocks = (long long)rows->rows * group / R + rows->B;
+            if (blocks > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
+            if (reserve_smem(reinterpret_cast<const void*>(kern), limit, smem) != cudaSuccess) return GLQ_ERR_CUDA;
+            return launch_kernel(true, kern, dim3((unsigned)blocks, (unsigned)kv->n_kv), dim3(kRowsThreads), smem,
+                                 reinterpret_cast<cudaStream_t>(stream), p) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
+        };
+        return (long long)most * group <= 8 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
+    });
+}

@@ -15,7 +15,9 @@ kernel over the row-major vocabulary matrix with the greedy arg-max folded in). 
 0..T-1 runs its norms, rotary embedding and cache write in ``glq_rope_prefill`` and its causal attention in
 ``glq_attn_prefill`` (head sizes 64 and 128; prompts of 2048 tokens and more, where the library's kernel is
 measurably faster, and prompts appended to a filled cache go through ``scaled_dot_product_attention``).  The first
-layer norm, the embedding lookup and the logits of a whole prompt are plain library calls.
+layer norm, the embedding lookup and the logits of a whole prompt are plain library calls.  Over a ``PagedKVCache`` (keys and values in
+8 bits, a length of its own for every sequence) decode steps and prompts alike go through ``paged_append`` and
+``paged_attention``.
 """
 
 from __future__ import annotations
@@ -31,6 +33,7 @@ import os
 
 from . import _lib, tiled
 from .moe_block import GraphCompatibleMoeBlock
+from .paged_cache import PagedKVCache
 from .quantized_linear import GLoRCQLinear
 
 # Prompts of at least this many tokens hand their causal attention to the library call instead of
@@ -54,6 +57,15 @@ class StaticKVCache:
     def reset(self):
         self.k.zero_()
         self.v.zero_()
+
+    def snapshot(self, n):
+        """What the first ``n`` positions hold, for ``restore``."""
+        return self.k[:, :, :, :n].clone(), self.v[:, :, :, :n].clone()
+
+    def restore(self, kept):
+        n = kept[0].shape[3]
+        self.k[:, :, :, :n].copy_(kept[0])
+        self.v[:, :, :, :n].copy_(kept[1])
 
     def update(self, layer, k_new, v_new, cache_position):
         """Write (B, kv_heads, T, D) at positions cache_position (T,) and return the layer's full buffers."""
@@ -115,6 +127,8 @@ class _Attention(nn.Module):
     def forward(self, x, cache_position, cache: StaticKVCache, cos, sin, kv_len=None):
         c = self.cfg
         B, T, _ = x.shape
+        if isinstance(cache, PagedKVCache):
+            return self._paged(x, cache_position, cache)
         if T == 1 and cache_position.numel() == 1 and c.head_dim in (32, 64, 128, 256):
             # decode step: norms, rotary embedding, cache write and attention over the live positions in
             # one launch; the position stays on the device (graph replay)
@@ -185,6 +199,22 @@ class _Attention(nn.Module):
         k = k * cs + _rotate_half(k) * sn
         k_all, v_all = cache.update(self.layer_idx, k, v, cache_position)
         return self._prompt_attention(q, k, v, k_all, v_all, cache, cache_position, kv_len, B, T)
+
+    def _paged(self, x, start, cache):
+        """Over a paged cache, T tokens a sequence behind the start[b] that are there: two launches beside the projections for a
+        decode step as for a prompt."""
+        c = self.cfg
+        B, T, _ = x.shape
+        rows = x.reshape(B * T, -1).contiguous()
+        if self._qkv is not None:
+            q, k, v = self._qkv.forward(rows)
+        else:
+            q = self.q_proj(rows)
+            k, v = self._kv.forward(rows) if self._kv is not None else (self.k_proj(rows), self.v_proj(rows))
+        q = q.view(B * T, c.num_attention_heads, c.head_dim)
+        k, v = (t.view(B * T, c.num_key_value_heads, c.head_dim) for t in (k, v))
+        q = cache.append(self.layer_idx, q, k, v, start, B, q_norm=self.q_norm, k_norm=self.k_norm, eps=c.rms_norm_eps)
+        return self.o_proj(cache.attend(self.layer_idx, q, start, B).view(B, T, -1))
 
     def _prompt_attention(self, q, k, v, k_all, v_all, cache, cache_position, kv_len, B, T):
         c = self.cfg
@@ -337,7 +367,8 @@ class GLoRCQDecoder(nn.Module):
     def forward(self, input_ids=None, cache_position=None, past_key_values=None, use_cache=True, return_dict=False,
                 logits_to_keep=0, **_unused):
         """``logits_to_keep`` = k > 0 computes the logits of the last k positions only (the greedy loop needs
-        one); 0 keeps them all, as the transformers models do by default."""
+        one); 0 keeps them all, as the transformers models do by default.  ``cache_position``: the positions of the T tokens, the same
+        for all sequences; with a ``PagedKVCache`` (T > 1: consecutive ones) also (B,) for T = 1 or (B, T), a sequence's own."""
         c = self.config
         B, T = input_ids.shape
         if past_key_values is None:
@@ -346,13 +377,24 @@ class GLoRCQDecoder(nn.Module):
             past_key_values = self._own_cache
         if cache_position is None:
             cache_position = torch.arange(T, device=input_ids.device)
-        cos, sin = self._tables(past_key_values.max_cache_len, input_ids.device)
+        paged = isinstance(past_key_values, PagedKVCache)
+        if paged:
+            if T > past_key_values.max_cache_len:
+                raise RuntimeError(f"{T} tokens are more than the cache's {past_key_values.max_cache_len} positions")
+            if cache_position.numel() == T:
+                start = cache_position.reshape(-1)[:1]
+            elif cache_position.numel() == B * T:
+                start = cache_position.reshape(B, T)[:, 0]
+            else:
+                raise RuntimeError(f"cache_position has {cache_position.numel()} values for {B} sequences of {T} tokens")
+            cache_position = start.to(torch.int64).contiguous()
+        cos, sin = (None, None) if paged else self._tables(past_key_values.max_cache_len, input_ids.device)
         x = F.embedding(input_ids, self.embed_tokens)
         L = c.num_hidden_layers
         h = F.rms_norm(x, (c.hidden_size,), self.ln1[0], c.rms_norm_eps) if L > 0 else x
         # a prompt (T > 1, eager only): its first position is read back once, so that attention sees the live
         # part of the static cache instead of all of it
-        kv_len = (int(cache_position[0]) + T) if T > 1 else None
+        kv_len = (int(cache_position[0]) + T) if T > 1 and not paged else None
         for l in range(L):
             x, h = _add_rmsnorm(x, self.attn[l](h, cache_position, past_key_values, cos, sin, kv_len), self.ln2[l],
                                 c.rms_norm_eps)

@@ -17,23 +17,32 @@ import torch
 
 from .decoder import StaticKVCache as StaticCache
 from .moe_block import GraphCompatibleMoeBlock
+from .paged_cache import PagedKVCache
 from .parallel import PeerExchange
 
 
 class GLoRCQGraphWrapper:
     """wrapper = GLoRCQGraphWrapper(model, max_batch_size=1, max_seq_len=4096)
-    output_ids, seconds = wrapper.generate(input_ids, max_new_tokens=128)"""
+    output_ids, seconds = wrapper.generate(input_ids, max_new_tokens=128)
 
-    def __init__(self, model, max_batch_size=1, max_seq_len=4096):
+    ``kv_cache`` "int8" or "e4m3": keys and values in 8 bits in pages of ``page_size`` tokens (``PagedKVCache``) instead of the static
+    fp16 cache; ``static_cache_position`` then has a position for every sequence, and ``replay`` takes one for all or a list or tensor
+    of them."""
+
+    def __init__(self, model, max_batch_size=1, max_seq_len=4096, kv_cache="static", page_size=64):
         self.model = model
         self.max_batch_size = max_batch_size
         self.max_seq_len = max_seq_len
         self.device = next(model.parameters()).device
         self.dtype = next(model.parameters()).dtype
-        self.static_cache = StaticCache(config=model.config, max_batch_size=max_batch_size, max_cache_len=max_seq_len,
-                                        device=self.device, dtype=self.dtype)
+        self.paged = kv_cache != "static"
+        if self.paged:
+            self.static_cache = PagedKVCache(model.config, max_batch_size, max_seq_len, self.device, dtype=kv_cache, page_size=page_size)
+        else:
+            self.static_cache = StaticCache(config=model.config, max_batch_size=max_batch_size, max_cache_len=max_seq_len,
+                                            device=self.device, dtype=self.dtype)
         self.static_input_ids = torch.zeros((max_batch_size, 1), dtype=torch.long, device=self.device)
-        self.static_cache_position = torch.zeros((1,), dtype=torch.long, device=self.device)
+        self.static_cache_position = torch.zeros((max_batch_size if self.paged else 1,), dtype=torch.long, device=self.device)
         self.static_logits = None
         self.static_next = None
         # this package's decoder can skip the logits of all prompt positions but the last
@@ -90,7 +99,10 @@ class GLoRCQGraphWrapper:
         assert input_ids.shape[0] == self.max_batch_size, \
             f"Input batch size {input_ids.shape[0]} != graph batch size {self.max_batch_size}"
         self.static_input_ids.copy_(input_ids)
-        self.static_cache_position.fill_(cache_position_val)
+        if isinstance(cache_position_val, (list, tuple, torch.Tensor)):
+            self.static_cache_position.copy_(torch.as_tensor(cache_position_val))
+        else:
+            self.static_cache_position.fill_(cache_position_val)
         self.graph.replay()
         return self.static_logits
 
@@ -115,10 +127,9 @@ class GLoRCQGraphWrapper:
         self._set_moe_graph_mode(True)
         if self.graph is None:
             # capturing runs steps at positions 0 and 10 of the static cache: keep the prompt's entries
-            keep_k, keep_v = self.static_cache.k[:, :, :, :11].clone(), self.static_cache.v[:, :, :, :11].clone()
+            kept = self.static_cache.snapshot(11)
             self.capture_graph()
-            self.static_cache.k[:, :, :, :11].copy_(keep_k)
-            self.static_cache.v[:, :, :, :11].copy_(keep_v)
+            self.static_cache.restore(kept)
             torch.cuda.synchronize()
             prefill_end = time.time()
         for i in range(max_new_tokens - 1):

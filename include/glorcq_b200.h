@@ -430,6 +430,62 @@ int glq_lm_head(const void* x, int64_t ldx, const void* W, int B, int V, int H, 
 int glq_lm_head_rows(const void* x, int64_t ldx, const void* W, int B, int V, int H, void* logits, int64_t ldl,
                      int64_t* argmax_out, void* workspace, size_t workspace_bytes, int32_t* counter, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged key/value cache in 8 bits, with a length of its own for every sequence (the reference decodes over transformers'
+ * static fp16 cache with one position for the whole batch, inference/graph_wrapper.py:41-47, 84-127).
+ *
+ * Pages of one layer: k_pages / v_pages (n_pages, n_kv, page, head_dim) codes, k_scale / v_scale (n_pages, n_kv) fp32;
+ * value = code * scale.  table: row b (table_stride ints apart) lists the physical pages of sequence b in order; an id outside
+ * [0, n_pages) is a page that is not there: nothing is written to it, its tokens are hidden from attention and read as zeros.  Pages may
+ * be shared by sequences that only read them; a page that a call writes belongs to one sequence.
+ *
+ * Rows of a call: sequence b holds start[b * start_stride] tokens before the call (start_stride 0: the same for all) and has
+ * rows q_start[b] .. q_start[b + 1] - 1 of the batch, at positions start, start + 1, ...; q_start NULL: rows / B each.
+ * max_new: at least the most rows of one sequence (host; with q_start NULL not read).  Rows in front of q_start[0] or behind q_start[B] are left as they
+ * are.  A start below zero counts as zero, one above max_pages * page as that; tokens past it are not stored and see all that is.
+ * start, q_start and table are read on the device when the call runs, so that captured calls follow them.
+ *
+ * head_dim 32, 64, 128 or 256; page 16, 32, 64 or 128 tokens; max_pages * page below 2^30; pages and rows 16-byte aligned, leading
+ * dimensions (elements between rows; the heads of a row are consecutive) multiples of 8.
+ * ------------------------------------------------------------------------------------------ */
+#define GLQ_KV_I8 0   /* -127 .. 127 */
+#define GLQ_KV_E4M3 1 /* 8-bit floating point, 4 exponent bits, at most 448 */
+typedef struct glq_paged_kv {
+    void* k_pages; void* v_pages;
+    float* k_scale; float* v_scale;
+    const int32_t* table; int64_t table_stride;
+    int32_t dtype; /* GLQ_KV_* */
+    int32_t n_pages, n_kv, head_dim, page, max_pages;
+} glq_paged_kv_t;
+typedef struct glq_paged_rows {
+    const int64_t* start; const int32_t* q_start;
+    int32_t start_stride, B, rows, max_new;
+} glq_paged_rows_t;
+
+/* New keys and values into the cache and the position rotation of q: every head of q and k is RMS-normed with q_norm / k_norm
+ * ((head_dim,) fp16, both or neither) and rotated (halves, as glq_rope_prefill) by cos / sin (cos_rows, head_dim / 2) fp32 at the
+ * token's position, in fp32; q_out is fp16 (may be q), keys and values are rounded once, to their codes.  cos NULL: no rotation.  q NULL: keys and
+ * values alone.  cos_rows >= max_pages * page.
+ * Scale of a block (one head's tokens of a page), need = largest finite magnitude of the new values / largest code (127, 448):
+ * a block whose first slot the call writes gets need; another keeps its scale while that is at least need, and otherwise has it
+ * doubled until it is, the codes in front of the new ones halved as often (nearest, ties to even).  A block without a scale yet (0) gets need.
+ * Infinities become the largest code, not-a-numbers zero. */
+int glq_paged_append(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, const void* k, int64_t ldk,
+                     const void* v, int64_t ldv, void* q_out, int64_t ldqo, int n_heads, const float* cos, const float* sin, int cos_rows,
+                     const void* q_norm, const void* k_norm, float eps, void* stream);
+
+/* Causal attention of the call's rows over the cache, the call's own tokens (glq_paged_append before it) among it:
+ * out = softmax(scale * q . K^T) V over the keys at positions 0 .. the row's own, head h of n_heads on key/value head
+ * h / (n_heads / n_kv).  q, out fp16 (rows, n_heads, head_dim); a row that sees no key is zero.  Scores, softmax and sums in fp32, the
+ * probabilities rounded to fp16 as the second product's operand.  Workspace contents irrelevant. */
+size_t glq_paged_attention_workspace_bytes(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads);
+int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, void* out, int64_t ldo,
+                        int n_heads, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows of the cache as fp16 = code * scale: row q_start[b] + i of k_out / v_out (rows, n_kv, head_dim) is position start + i of
+ * sequence b. */
+int glq_paged_read(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, void* k_out, void* v_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
