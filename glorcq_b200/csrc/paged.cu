@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const ReadPara
 // to fp16 relative to the largest contribution; the sum of the softmax is that of w / vs in fp32.  The maximum m is raised only when a score
 // exceeds it by 2^8 (w stays below 256 in fp16), by a vote, so that a step has no shuffles as a rule.
 // ---------------------------------------------------------------------------------------------
-constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32;
+constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32, kRowsStep = 16 * kRowsWarps;
 
 struct AttnParams {
     PagedKv kv;
@@ -276,7 +276,33 @@ struct AttnParams {
     long long ldq, ldo;
     int n_heads, group;
     float scale2;           // softmax scale * log2(e) * kCodeUnit
+    float* partial;         // two partial results for each CTA
 };
+
+// weighted values / sum of the weights -> four channels of a result row; a row that saw nothing is zero, not-a-number stays
+__device__ __forceinline__ void store_result(__half* dst, const float4& acc, float sum, float unit) {
+    const float inv = sum > 0.f ? unit / sum : (sum == 0.f ? 0.f : sum);
+    __half2 o[2] = {__floats2half2_rn(acc.x * inv, acc.y * inv), __floats2half2_rn(acc.z * inv, acc.w * inv)};
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
+}
+__device__ __forceinline__ void block_sum2(long long& x, long long& y, long long* sm) {      // kRowsThreads threads, 2 kRowsWarps words
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, d);
+        y += __shfl_xor_sync(0xffffffffu, y, d);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        sm[threadIdx.x >> 5] = x;
+        sm[kRowsWarps + (threadIdx.x >> 5)] = y;
+    }
+    __syncthreads();
+    x = y = 0;
+#pragma unroll
+    for (int w = 0; w < kRowsWarps; ++w) {
+        x += sm[w];
+        y += sm[kRowsWarps + w];
+    }
+}
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t d;
@@ -288,222 +314,355 @@ __device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; -inf -> 0
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// codes that one CTA alone reads: not kept in the first-level cache
-template <int WORDS> __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t* w) {
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
     if (WORDS == 4)
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
     else if (WORDS == 2)
-        asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
     else
-        asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
 }
 
+// Shared memory of paged_attention_rows_kernel.  A warp has a ring of its own: S stages of 16 tokens, keys, then values, then the two scales.  A
+// row's 16-byte pieces are stored at piece ^ swizzle(row), so that the fragments' loads (8 lanes together: two rows and four pieces of the keys, four
+// rows, two apart, and two pieces of the values) meet 32 banks; with 64 channels the values' meet 16.  The rings and the warps' results share the space.
+template <int HD, int NB> struct RowsCfg {
+    static constexpr int R = 8 * NB, PIECES = HD / 16;
+    static constexpr int STAGE = 32 * HD;
+    static constexpr int S = HD == 32 ? 6 : HD == 64 ? 5 : 3;
+    static constexpr int RING = S * STAGE;
+    static constexpr int RESULTS = kRowsWarps * R * (HD + 2) * 4;
+    static constexpr size_t SMEM = (kRowsWarps * RING > RESULTS ? kRowsWarps * RING : RESULTS) + kRowsWarps * S * 8;
+    static constexpr int CTAS = HD == 256 || NB == 2 ? 1 : 2;
+    static __device__ __forceinline__ int key_swizzle(int row) { return HD >= 128 ? (row & 1) << 2 : 0; }
+    static __device__ __forceinline__ int value_swizzle(int row) { return HD >= 128 ? row & 6 : HD == 64 ? (row >> 1) & 3 : 0; }
+};
+
+// rows of a block, HD values and (maximum, sum) each: a CTA's partial results of a segment
+template <int R, int HD> constexpr int kPartial = R * (HD + 2);
+
 template <int HD, int DT, int NB>
-__global__ void __launch_bounds__(kRowsThreads, HD == 256 || NB == 2 ? 1 : 2) paged_attention_rows_kernel(const AttnParams p) {
-    constexpr int R = 8 * NB;                       // rows of a block
+__global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_attention_rows_kernel(const AttnParams p) {
+    using C = RowsCfg<HD, NB>;
+    constexpr int R = C::R, S = C::S;               // rows of a block, stages
     constexpr int KW = HD / 16, VW = HD / 32;       // code words of a lane: per key row, per value row
     constexpr int KC = KW < 4 ? KW : 4, VC = VW < 4 ? VW : 4;       // words of one load
-    extern __shared__ float sm_rows[];
+    extern __shared__ __align__(128) float sm_rows[];
     float* sm_o = sm_rows;                                         // [warp][R][HD]
-    float* sm_m = sm_o + kRowsWarps * R * HD;                      // [warp][R], then weights
+    float* sm_m = sm_o + kRowsWarps * R * HD;                      // [warp][R]
     float* sm_l = sm_m + kRowsWarps * R;                           // [warp][R]
+    __shared__ long long sm_plan[kRowsWarps + 3];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int h = blockIdx.y;
+    const uint32_t ring = smem_addr(sm_rows) + warp * C::RING, scales = smem_addr(sm_rows) + (uint32_t)C::SMEM - (kRowsWarps - warp) * S * 8;
     after_launch_ahead();
-    // row blocks of sequence b: from rows * group / R + b on
-    auto first = [&](int b) { return (int)((long long)rows_from(p.r, b) * p.group / R) + b; };
-    const int b = last_from(p.r.B, (int)blockIdx.x, first);
-    if ((int)blockIdx.x < first(b)) return;       // (rows in front of the first sequence)
-    const int2 own = rows_of(p.r, b);
-    const int r0 = ((int)blockIdx.x - first(b)) * R, n_rows = min(own.y * p.group - r0, R);
-    if (n_rows <= 0) return;
-    const int start = start_of(p.r, b, p.kv.capacity);
-    const int limit_all = min(start + (r0 + n_rows - 1) / p.group, p.kv.capacity - 1);       // the last key that a row sees
-    const int n_tiles = limit_all / 16 + 1;
+    int b;
+    long long off;
+    const long long total = paged_plan<kRowsThreads, R, kRowsStep>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan, b, off);
+    long long left = share_begin(total, blockIdx.x + 1, gridDim.x) - share_begin(total, blockIdx.x, gridDim.x);
 
-    uint32_t qf[NB][KW][2];
-    int limit[NB][2];
-    float m[NB][2], l[NB][2], o[NB][2 * VW][4];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int r = r0 + 8 * n + g;
-        const bool live = 8 * n + g < n_rows;
-        const __half* src = p.q + (long long)(own.x + (live ? r / p.group : 0)) * p.ldq + (h * p.group + (live ? r % p.group : 0)) * HD;
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            const int ch = KW < 4 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
-            const uint2 v = live ? *reinterpret_cast<const uint2*>(src + ch) : make_uint2(0u, 0u);
-            qf[n][w][0] = v.x;
-            qf[n][w][1] = v.y;
+    while (left > 0) {
+        const PagedSeq seq = paged_seq<R, kRowsStep>(p.kv, p.r, p.group, b);
+        if (off >= (long long)seq.blocks * p.kv.n_kv * seq.steps) {
+            ++b;
+            off = 0;
+            continue;
         }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int rr = 8 * n + 2 * t + e;
-            limit[n][e] = rr < n_rows ? min(start + (r0 + rr) / p.group, p.kv.capacity - 1) : -1;
-            m[n][e] = -1e30f;
-            l[n][e] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 2 * VW; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
-    }
-    const int limit_low = min(start + r0 / p.group, p.kv.capacity - 1);       // keys up to here are seen by every live row
+        const int segment = (int)(off / seq.steps), step0 = (int)(off - (long long)segment * seq.steps);
+        const int step1 = (int)min((long long)seq.steps, step0 + left);
+        const int h = segment % p.kv.n_kv, r0 = segment / p.kv.n_kv * R, n_rows = min(seq.own.y * p.group - r0, R);
+        const int2 own = seq.own;
+        const int start = seq.start;
+        left -= step1 - step0;
+        off += step1 - step0;
+        const int limit_all = min(start + (r0 + n_rows - 1) / p.group, p.kv.capacity - 1);       // the last key that a row sees
+        const int n_tiles = min(limit_all / 16 + 1, step1 * kRowsWarps);
 
-    uint32_t kw[2][KW], vw[4][VW];
-    float ks, vs;
-    auto lookup = [&](int tile) { return tile < n_tiles ? page_of(p.kv, b, tile * 16 >> p.kv.page_shift) : -1; };
-    auto load_k = [&](int tile, int phys) {
-        ks = 0.f;
-        if (phys >= 0) {
-            const size_t block = (size_t)phys * p.kv.n_kv + h;
-            ks = p.kv.k_scale[block];
-            const unsigned char* src = p.kv.k + ((block << p.kv.page_shift) + ((tile * 16) & (p.kv.page - 1)) + g) * HD + t * 4 * KC;
+        uint32_t qf[NB][KW][2];
+        int limit[NB][2];
+        float m[NB][2], l[NB][2], o[NB][2 * VW][4];
 #pragma unroll
-            for (int c = 0; c < KW / KC; ++c) {
-                load_words<KC>(src + 64 * c, &kw[0][KC * c]);
-                load_words<KC>(src + 8 * HD + 64 * c, &kw[1][KC * c]);
+        for (int n = 0; n < NB; ++n) {
+            const int r = r0 + 8 * n + g;
+            const bool live = 8 * n + g < n_rows;
+            const __half* src = p.q + (long long)(own.x + (live ? r / p.group : 0)) * p.ldq + (h * p.group + (live ? r % p.group : 0)) * HD;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                const int ch = KW < 4 ? 8 * t + 4 * w : 64 * (w / 4) + 16 * t + 4 * (w % 4);
+                const uint2 v = live ? *reinterpret_cast<const uint2*>(src + ch) : make_uint2(0u, 0u);
+                qf[n][w][0] = v.x;
+                qf[n][w][1] = v.y;
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int rr = 8 * n + 2 * t + e;
+                limit[n][e] = rr < n_rows ? min(start + (r0 + rr) / p.group, p.kv.capacity - 1) : -1;
+                m[n][e] = -1e30f;
+                l[n][e] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * VW; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
         }
-    };
-    auto load_v = [&](int tile, int phys) {
-        vs = 0.f;
-        if (phys >= 0) {
-            const size_t block = (size_t)phys * p.kv.n_kv + h;
-            vs = p.kv.v_scale[block];
-            const unsigned char* src = p.kv.v + ((block << p.kv.page_shift) + ((tile * 16) & (p.kv.page - 1)) + 2 * t) * HD + g * 4 * VC;
+        const int limit_low = min(start + r0 / p.group, p.kv.capacity - 1);       // keys up to here are seen by every live row
+
+        // The warp's tiles are i = 0, 1, ..: tokens 16 (8 (step0 + i) + warp) and 15 more.  Lane k has the page of the tile i + k of the
+        // current 32, asked for together; -1 ends the list or is a page that is not there.
+        const int tile0 = step0 * kRowsWarps + warp, count = tile0 < n_tiles ? (n_tiles - tile0 + kRowsWarps - 1) / kRowsWarps : 0;
+        auto pages_from = [&](int i) { return i + lane < count ? page_of(p.kv, b, (tile0 + (i + lane) * kRowsWarps) * 16 >> p.kv.page_shift) : -1; };
+        int pages = pages_from(0), pages_next = pages_from(32);
+        auto request = [&](int i, int stage, int phys) {
+            if (phys >= 0) {
+                const size_t block = (size_t)phys * p.kv.n_kv + h;
+                const size_t from = ((block << p.kv.page_shift) + (((tile0 + i * kRowsWarps) * 16) & (p.kv.page - 1))) * HD + lane * 16;
+                const uint32_t at = ring + stage * C::STAGE;
+#pragma unroll
+                for (int u = 0; u < (HD + 31) / 32; ++u) {
+                    const int piece = u * 32 + lane, row = piece / C::PIECES, c = piece % C::PIECES;
+                    copy_async_16(at + row * HD + ((c ^ C::key_swizzle(row)) << 4), p.kv.k + from + u * 512);
+                    copy_async_16(at + 16 * HD + row * HD + ((c ^ C::value_swizzle(row)) << 4), p.kv.v + from + u * 512);
+                }
+                if (lane < 2) copy_async_4(scales + stage * 8 + lane * 4, (lane ? p.kv.v_scale : p.kv.k_scale) + block);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i) request(i, i, __shfl_sync(0xffffffffu, pages, i));
+        int stage = 0;
+        for (int i = 0; i < count; ++i) {
+            const int tile = tile0 + i * kRowsWarps;
+            asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+            __syncwarp();
+            const int phys = __shfl_sync(0xffffffffu, pages, i & 31);
+            {       // the stage that the tile before this one has left
+                const int j = i + S - 1;
+                request(j, stage == 0 ? S - 1 : stage - 1, __shfl_sync(0xffffffffu, (j ^ i) & 32 ? pages_next : pages, j & 31));
+            }
+            const uint32_t at = ring + stage * C::STAGE;
+            float ks, vscale;
+            asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vscale) : "r"(scales + stage * 8) : "memory");
+            uint32_t kw[2][KW], vw[4][VW];
+#pragma unroll
+            for (int c = 0; c < KW / KC; ++c)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int row = g + 8 * u;
+                    const uint32_t a = KC == 4 ? ((t + 4 * c) ^ C::key_swizzle(row)) << 4 : t * 8;
+                    lds_words<KC>(at + row * HD + a, &kw[u][KC * c]);
+                }
 #pragma unroll
             for (int c = 0; c < VW / VC; ++c)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) load_words<VC>(src + ((u & 1) + 8 * (u >> 1)) * HD + 128 * c, &vw[u][VC * c]);
+                for (int u = 0; u < 4; ++u) {
+                    const int row = 2 * t + (u & 1) + 8 * (u >> 1);
+                    const uint32_t a = VC == 4 ? ((g + 8 * c) ^ C::value_swizzle(row)) << 4
+                                     : VC == 2 ? (((g >> 1) ^ C::value_swizzle(row)) << 4) + (g & 1) * 8 : g * 4;
+                    lds_words<VC>(at + 16 * HD + row * HD + a, &vw[u][VC * c]);
+                }
+            float s[NB][4];
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                uint32_t a0, a1, a2, a3;
+                codes_to_half<DT>(kw[0][w], a0, a2);
+                codes_to_half<DT>(kw[1][w], a1, a3);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) mma16816(s[n], a0, a1, a2, a3, qf[n][w][0], qf[n][w][1]);
+            }
+            const float c = ks * p.scale2, lv = vscale > 0.f ? log2_fast(vscale) : 0.f, iv = vscale > 0.f ? rcp_fast(vscale) : 1.f;
+            // w of token g (+ 8) and rows 2t, 2t + 1 of each block of rows
+            uint32_t pf[NB][2];
+            const bool masked = tile * 16 + 15 > limit_low || phys < 0;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const int tok = tile * 16 + g;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[n][e] = s[n][e] * c + lv;
+                    if (masked && (phys < 0 || tok + 8 * (e >> 1) > limit[n][e & 1])) s[n][e] = -INFINITY;
+                }
+                const float hi0 = fmaxf(s[n][0], s[n][2]), hi1 = fmaxf(s[n][1], s[n][3]);
+                if (__any_sync(0xffffffffu, hi0 > m[n][0] + 8.f || hi1 > m[n][1] + 8.f)) {
+                    float x0 = fmaxf(hi0, m[n][0]), x1 = fmaxf(hi1, m[n][1]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) {
+                        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+                        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+                    }
+                    const float f0 = exp2_fast(m[n][0] - x0), f1 = exp2_fast(m[n][1] - x1);
+                    m[n][0] = x0;
+                    m[n][1] = x1;
+                    l[n][0] *= f0;
+                    l[n][1] *= f1;
+#pragma unroll
+                    for (int i = 0; i < 2 * VW; ++i) {
+                        o[n][i][0] *= f0;
+                        o[n][i][1] *= f1;
+                        o[n][i][2] *= f0;
+                        o[n][i][3] *= f1;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] = exp2_fast(s[n][e] - m[n][e & 1]);
+                l[n][0] += (s[n][0] + s[n][2]) * iv;
+                l[n][1] += (s[n][1] + s[n][3]) * iv;
+                pf[n][0] = transpose8x8(vscale > 0.f ? pack_half2(s[n][0], s[n][1]) : 0u);
+                pf[n][1] = transpose8x8(vscale > 0.f ? pack_half2(s[n][2], s[n][3]) : 0u);
+            }
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t sel = half ? 0x7362u : 0x5140u;
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_half<DT>(prmt(vw[0][w], vw[1][w], sel), a0, a1);
+                    codes_to_half<DT>(prmt(vw[2][w], vw[3][w], sel), a2, a3);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) mma16816(o[n][2 * w + half], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+                }
+            }
+            if (++stage == S) stage = 0;
+            if ((i & 31) == 31) {
+                pages = pages_next;
+                pages_next = pages_from(i + 33);
+            }
         }
-    };
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int w = 0; w < KW; ++w) kw[u][w] = 0u;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) vw[u][w] = 0u;
-
-    int phys = lookup(warp), phys1 = lookup(warp + kRowsWarps);
-    load_k(warp, phys);
-    load_v(warp, phys);
-    for (int tile = warp; tile < n_tiles; tile += kRowsWarps) {
-        float s[NB][4];
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        // the warps' results meet in shared memory
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            uint32_t a0, a1, a2, a3;
-            codes_to_half<DT>(kw[0][w], a0, a2);
-            codes_to_half<DT>(kw[1][w], a1, a3);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) mma16816(s[n], a0, a1, a2, a3, qf[n][w][0], qf[n][w][1]);
-        }
-        const float c = ks * p.scale2, vscale = vs;
-        const int phys2 = lookup(tile + 2 * kRowsWarps);
-        load_k(tile + kRowsWarps, phys1);
-        const float lv = vscale > 0.f ? log2f(vscale) : 0.f, iv = vscale > 0.f ? 1.f / vscale : 1.f;
-        // w of token g (+ 8) and rows 2t, 2t + 1 of each block of rows
-        uint32_t pf[NB][2];
-        const bool masked = tile * 16 + 15 > limit_low || phys < 0;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            const int tok = tile * 16 + g;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[n][e] = s[n][e] * c + lv;
-                if (masked && (phys < 0 || tok + 8 * (e >> 1) > limit[n][e & 1])) s[n][e] = -INFINITY;
-            }
-            const float hi0 = fmaxf(s[n][0], s[n][2]), hi1 = fmaxf(s[n][1], s[n][3]);
-            if (__any_sync(0xffffffffu, hi0 > m[n][0] + 8.f || hi1 > m[n][1] + 8.f)) {
-                float x0 = fmaxf(hi0, m[n][0]), x1 = fmaxf(hi1, m[n][1]);
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) {
-                    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-                    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+                for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
+                const int r = 8 * n + 2 * t + e;
+                if (g == 0) {
+                    sm_m[warp * R + r] = m[n][e];
+                    sm_l[warp * R + r] = l[n][e];
                 }
-                const float f0 = exp2_fast(m[n][0] - x0), f1 = exp2_fast(m[n][1] - x1);
-                m[n][0] = x0;
-                m[n][1] = x1;
-                l[n][0] *= f0;
-                l[n][1] *= f1;
+                float* dst = sm_o + (warp * R + r) * HD;
 #pragma unroll
-                for (int i = 0; i < 2 * VW; ++i) {
-                    o[n][i][0] *= f0;
-                    o[n][i][1] *= f1;
-                    o[n][i][2] *= f0;
-                    o[n][i][3] *= f1;
+                for (int w = 0; w < VW; ++w) {
+                    const int ch = VW < 4 ? 4 * VW * g + 4 * w : 128 * (w / 4) + 16 * g + 4 * (w % 4);
+                    *reinterpret_cast<float4*>(dst + ch) = make_float4(o[n][2 * w][e], o[n][2 * w][e + 2], o[n][2 * w + 1][e], o[n][2 * w + 1][e + 2]);
                 }
             }
+        __syncthreads();
+        const bool whole = step0 == 0 && step1 == seq.steps;
+        float* part = p.partial + (size_t)(2 * blockIdx.x + (step0 == 0)) * kPartial<R, HD>;
+        for (int i = threadIdx.x; i < n_rows * (HD / 4); i += kRowsThreads) {
+            const int r = i / (HD / 4), ch = i % (HD / 4) * 4;
+            float mx = -1e30f, sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = exp2_fast(s[n][e] - m[n][e & 1]);
-            l[n][0] += (s[n][0] + s[n][2]) * iv;
-            l[n][1] += (s[n][1] + s[n][3]) * iv;
-            pf[n][0] = transpose8x8(vscale > 0.f ? pack_half2(s[n][0], s[n][1]) : 0u);
-            pf[n][1] = transpose8x8(vscale > 0.f ? pack_half2(s[n][2], s[n][3]) : 0u);
-        }
+            for (int w = 0; w < kRowsWarps; ++w) mx = fmaxf(mx, sm_m[w * R + r]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t sel = half ? 0x7362u : 0x5140u;
-                uint32_t a0, a1, a2, a3;
-                codes_to_half<DT>(prmt(vw[0][w], vw[1][w], sel), a0, a1);
-                codes_to_half<DT>(prmt(vw[2][w], vw[3][w], sel), a2, a3);
-#pragma unroll
-                for (int n = 0; n < NB; ++n) mma16816(o[n][2 * w + half], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+            for (int w = 0; w < kRowsWarps; ++w) {
+                const float f = exp2_fast(sm_m[w * R + r] - mx);
+                const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * R + r) * HD + ch);
+                sum += sm_l[w * R + r] * f;
+                acc.x += v.x * f;
+                acc.y += v.y * f;
+                acc.z += v.z * f;
+                acc.w += v.w * f;
+            }
+            if (whole) {
+                store_result(p.out + (long long)(own.x + (r0 + r) / p.group) * p.ldo + (h * p.group + (r0 + r) % p.group) * HD + ch, acc, sum, kCodeUnit<DT>);
+            } else {
+                *reinterpret_cast<float4*>(part + r * HD + ch) = acc;
+                if (ch == 0) *reinterpret_cast<float2*>(part + R * HD + 2 * r) = make_float2(mx, sum);
             }
         }
-        load_v(tile + kRowsWarps, phys1);
-        phys = phys1;
-        phys1 = phys2;
+        __syncthreads();
     }
-    // the warps' results meet in shared memory
+}
+
+// Joins the partial results of segments that several CTAs shared: a CTA a (block of rows, head), a warp a row.  Lane c looks at the
+// maximum and sum of the c-th part, the values are added in the order of the shares, eight parts requested together.
+template <int HD, int DT, int R, int STEP>
+__global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnParams p, int n_cta) {
+    constexpr int VPL = HD / 32;                     // channels of a lane
+    __shared__ long long sm_plan[2 * kRowsWarps];
+    after_launch_ahead();
+    const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto first = [&](int b) { return (int)((long long)rows_from(p.r, b) * p.group / R) + b; };
+    const int b = last_from(p.r.B, (int)blockIdx.x, first);
+    const PagedSeq seq = paged_seq<R, STEP>(p.kv, p.r, p.group, b);
+    const int rb = (int)blockIdx.x - first(b);
+    if (rb < 0 || rb >= seq.blocks) return;
+    // steps of the sequences before b, and of all
+    long long before = 0, total = 0;
+    for (int i = threadIdx.x; i < p.r.B; i += kRowsThreads) {
+        const PagedSeq s = paged_seq<R, STEP>(p.kv, p.r, p.group, i);
+        const long long w = (long long)s.blocks * p.kv.n_kv * s.steps;
+        total += w;
+        if (i < b) before += w;
+    }
+    block_sum2(before, total, sm_plan);
+    const long long u0 = before + ((long long)rb * p.kv.n_kv + h) * seq.steps, u1 = u0 + seq.steps - 1;
+    const int c0 = share_of(total, u0, n_cta), c1 = share_of(total, u1, n_cta);
+    if (c0 == c1) return;
+    const int r0 = rb * R, n_rows = min(seq.own.y * p.group - r0, R);
+    auto part_of = [&](int c) { return p.partial + (size_t)(2 * c + (c == c0)) * kPartial<R, HD>; };
+    for (int r = warp; r < n_rows; r += kRowsWarps) {
+        float mx = -1e30f, sum = 0.f, acc[VPL];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+        for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
+        for (int base = c0; base <= c1; base += 32) {
+            const int c = base + lane;
+            const bool live = c <= c1 && share_begin(total, c, n_cta) < share_begin(total, c + 1, n_cta);
+            const float2 ml = live ? *reinterpret_cast<const float2*>(part_of(c) + R * HD + 2 * r) : make_float2(-1e30f, 0.f);
+            float x = fmaxf(ml.x, mx);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+            for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            const float f = exp2_fast(mx - x), w = exp2_fast(ml.x - x);
+            mx = x;
+            sum = sum * f + warp_sum(ml.y * w);
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], d);
-            const int r = 8 * n + 2 * t + e;
-            if (g == 0) {
-                sm_m[warp * R + r] = m[n][e];
-                sm_l[warp * R + r] = l[n][e];
-            }
-            float* dst = sm_o + (warp * R + r) * HD;
+            for (int i = 0; i < VPL; ++i) acc[i] *= f;
+            const unsigned there = __ballot_sync(0xffffffffu, live);
+            const int n = min(32, c1 - base + 1);
+            for (int k = 0; k < n; k += 8) {
+                float v[8][VPL];
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                const int ch = VW < 4 ? 4 * VW * g + 4 * w : 128 * (w / 4) + 16 * g + 4 * (w % 4);
-                *reinterpret_cast<float4*>(dst + ch) = make_float4(o[n][2 * w][e], o[n][2 * w][e + 2], o[n][2 * w + 1][e], o[n][2 * w + 1][e + 2]);
+                for (int u = 0; u < 8; ++u) {
+                    const float* src = part_of(base + k + u) + r * HD + lane * VPL;
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) v[u][i] = there >> (k + u) & 1u ? src[i] : 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float wu = __shfl_sync(0xffffffffu, w, k + u);
+#pragma unroll
+                    for (int i = 0; i < VPL; ++i) acc[i] += v[u][i] * wu;
+                }
             }
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n_rows * (HD / 4); i += kRowsThreads) {
-        const int r = i / (HD / 4), ch = i % (HD / 4) * 4;
-        float mx = -1e30f, sum = 0.f;
+        const float inv = sum > 0.f ? kCodeUnit<DT> / sum : (sum == 0.f ? 0.f : sum);
+        __half* dst = p.out + (long long)(seq.own.x + (r0 + r) / p.group) * p.ldo + (h * p.group + (r0 + r) % p.group) * HD + lane * VPL;
 #pragma unroll
-        for (int w = 0; w < kRowsWarps; ++w) mx = fmaxf(mx, sm_m[w * R + r]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kRowsWarps; ++w) {
-            const float f = exp2_fast(sm_m[w * R + r] - mx);
-            const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * R + r) * HD + ch);
-            sum += sm_l[w * R + r] * f;
-            acc.x += v.x * f;
-            acc.y += v.y * f;
-            acc.z += v.z * f;
-            acc.w += v.w * f;
-        }
-        const float inv = sum > 0.f ? kCodeUnit<DT> / sum : (sum == 0.f ? 0.f : sum);      // (not-a-number stays)
-        __half2 o2[2] = {__floats2half2_rn(acc.x * inv, acc.y * inv), __floats2half2_rn(acc.z * inv, acc.w * inv)};
-        const int rr = r0 + r;
-        __half* dst = p.out + (long long)(own.x + rr / p.group) * p.ldo + (h * p.group + rr % p.group) * HD + ch;
-        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o2);
+        for (int i = 0; i < VPL; ++i) dst[i] = __float2half_rn(acc[i] * inv);
     }
 }
 
@@ -595,38 +754,64 @@ extern "C" int glq_paged_read(const glq_paged_kv_t* kv, const glq_paged_rows_t* 
     });
 }
 
+// How a call runs, from what the host knows.
+struct AttnPlan {
+    int nb, grid;          // blocks of 8 rows in a row block; CTAs
+};
+int sm_count() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n;
+}
+AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
+    const long long most = rows->q_start ? std::min(rows->max_new, rows->rows) : rows->rows / rows->B;
+    AttnPlan a;
+    a.nb = most * (n_heads / kv->n_kv) <= 8 ? 1 : 2;
+    a.grid = sm_count() * (kv->head_dim == 256 || a.nb == 2 ? 1 : 2);
+    return a;
+}
+int check_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
+    const int bad = check_cache(kv, rows);
+    if (bad != GLQ_OK) return bad;
+    if (n_heads <= 0 || n_heads % kv->n_kv != 0 || (rows->q_start && rows->max_new < 0)) return GLQ_ERR_ARG;
+    if ((long long)rows->rows * n_heads > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
+    return GLQ_OK;
+}
+
 extern "C" size_t glq_paged_attention_workspace_bytes(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
-    (void)kv, (void)rows, (void)n_heads;
-    return 0;
+    if (check_attention(kv, rows, n_heads) != GLQ_OK || rows->rows == 0 || rows->B == 0) return 0;
+    const AttnPlan a = plan_attention(kv, rows, n_heads);
+    return (size_t)a.grid * 2 * (8 * a.nb) * (kv->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, void* out,
                                    int64_t ldo, int n_heads, float scale, void* workspace, size_t workspace_bytes, void* stream) {
-    (void)workspace, (void)workspace_bytes;
-    const int bad = check_cache(kv, rows);
+    const int bad = check_attention(kv, rows, n_heads);
     if (bad != GLQ_OK) return bad;
     if (rows->rows == 0 || rows->B == 0) return GLQ_OK;
-    if (!q || !out || n_heads <= 0 || n_heads % kv->n_kv != 0 || (rows->q_start && rows->max_new < 0)) return GLQ_ERR_ARG;
-    if (ldq < (int64_t)n_heads * kv->head_dim || ldo < (int64_t)n_heads * kv->head_dim) return GLQ_ERR_ARG;
+    if (!q || !out || ldq < (int64_t)n_heads * kv->head_dim || ldo < (int64_t)n_heads * kv->head_dim) return GLQ_ERR_ARG;
     if (ldq % 8 || ldo % 8 || !aligned16(q) || !aligned16(out)) return GLQ_ERR_ALIGN;
-    if ((long long)rows->rows * n_heads > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < glq_paged_attention_workspace_bytes(kv, rows, n_heads)) return GLQ_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return GLQ_ERR_ALIGN;
+    const AttnPlan plan = plan_attention(kv, rows, n_heads);
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return by_type(kv, [&](auto hd, auto dt) {
         constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
         const int group = n_heads / kv->n_kv;
         const AttnParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<__half*>(out), ldq, ldo, n_heads,
-                           group, scale * 1.4426950408889634f * kCodeUnit<DT>};
-        const int most = rows->q_start ? std::min(rows->max_new, rows->rows) : rows->rows / rows->B;
+                           group, scale * 1.4426950408889634f * kCodeUnit<DT>, static_cast<float*>(workspace)};
         auto run = [&](auto nb) {
             constexpr int NB = decltype(nb)::value, R = 8 * NB;
-            constexpr size_t smem = (size_t)kRowsWarps * R * (HD + 2) * sizeof(float);
+            constexpr size_t smem = RowsCfg<HD, NB>::SMEM;
             static SmemLimit limit;
             auto* kern = paged_attention_rows_kernel<HD, DT, NB>;
             const long long blocks = (long long)rows->rows * group / R + rows->B;
             if (blocks > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
             if (reserve_smem(reinterpret_cast<const void*>(kern), limit, smem) != cudaSuccess) return GLQ_ERR_CUDA;
-            return launch_kernel(true, kern, dim3((unsigned)blocks, (unsigned)kv->n_kv), dim3(kRowsThreads), smem,
-                                 reinterpret_cast<cudaStream_t>(stream), p) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
+            if (launch_kernel(true, kern, dim3((unsigned)plan.grid), dim3(kRowsThreads), smem, st, p) != cudaSuccess) return GLQ_ERR_CUDA;
+            return launch_kernel(true, paged_join_kernel<HD, DT, R, kRowsStep>, dim3((unsigned)blocks, (unsigned)kv->n_kv), dim3(kRowsThreads), 0, st,
+                                 p, plan.grid) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
         };
-        return (long long)most * group <= 8 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
+        return plan.nb == 1 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
     });
 }

@@ -66,6 +66,74 @@ __device__ __forceinline__ void after_launch_ahead() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// ---- sharing out the work of an attention call -----------------------------------------------------------------------
+// A segment is a block of rows of one (sequence, key/value head); its work are steps of STEP tokens.  The steps of all segments, counted in
+// order (sequence, block of rows, head), are cut into equal shares, one for each CTA, whatever the lengths: the lengths are on the device, and
+// a batch of 64 sequences of 800 to 8192 tokens takes as long as its sum, not as its longest.  A segment that a share's end cuts leaves
+// partial results, at most two of them per CTA, which paged_join_kernel joins.
+__host__ __device__ __forceinline__ long long share_begin(long long total, int cta, int n_cta) { return total * cta / n_cta; }
+// the CTA in whose share step u lies
+__device__ __forceinline__ int share_of(long long total, long long u, int n_cta) { return (int)(((u + 1) * n_cta + total - 1) / total) - 1; }
+
+struct PagedSeq {
+    int2 own;               // first row, rows
+    int start, steps, blocks;      // tokens before the call; steps and blocks of rows of a head
+};
+template <int R, int STEP> __device__ __forceinline__ PagedSeq paged_seq(const PagedKv& kv, const PagedRows& r, int group, int b) {
+    PagedSeq s;
+    s.own = rows_of(r, b);
+    s.start = start_of(r, b, kv.capacity);
+    s.blocks = (s.own.y * group + R - 1) / R;
+    s.steps = s.own.y > 0 ? (min(s.start + s.own.y, kv.capacity) + STEP - 1) / STEP : 0;
+    return s;
+}
+// All threads of the block; `sm`: THREADS / 32 + 3 long longs.  Returns the total; b0, off0: the sequence, and the step of it, where
+// the share of `cta` begins (nothing, where that is empty).
+template <int THREADS, int R, int STEP>
+__device__ __forceinline__ long long paged_plan(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, long long* sm, int& b0, long long& off0) {
+    constexpr int W = THREADS / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (r.B + THREADS - 1) / THREADS;
+    auto weight = [&](int b) {
+        const PagedSeq s = paged_seq<R, STEP>(kv, r, group, b);
+        return (long long)s.blocks * kv.n_kv * s.steps;
+    };
+    long long mine = 0;
+    for (int i = 0; i < per; ++i)
+        if (tid * per + i < r.B) mine += weight(tid * per + i);
+    long long incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 31) sm[warp] = incl;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        if (w < warp) before += sm[w];
+        total += sm[w];
+    }
+    const long long u0 = share_begin(total, cta, n_cta);
+    long long at = before + incl - mine;
+    if (mine > 0 && u0 >= at && u0 < at + mine) {
+        for (int i = 0;; ++i) {
+            const long long w = weight(tid * per + i);
+            if (u0 < at + w) {
+                sm[W + 1] = tid * per + i;
+                sm[W + 2] = u0 - at;
+                break;
+            }
+            at += w;
+        }
+    }
+    __syncthreads();
+    b0 = (int)sm[W + 1];
+    off0 = sm[W + 2];
+    return total;
+}
+
 // ---- codes --------------------------------------------------------------------------------------------------------
 constexpr int kI8 = GLQ_KV_I8, kE4M3 = GLQ_KV_E4M3;
 template <int DT> constexpr float kCodeMax = DT == kI8 ? 127.f : 448.f;
