@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libglorcq_b200.so")
 NATIVE = os.path.join(HERE, "_native.so")
-SOURCES = ["api.cu", "moe.cu", "attn.cu", "lm_head.cu", "paged.cu"]
+SOURCES = ["api.cu", "moe.cu", "attn.cu", "lm_head.cu", "paged.cu", "paged_prompt.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-shared", "-Xcompiler", "-fPIC", "--use_fast_math=false"]
 

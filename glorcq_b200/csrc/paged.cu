@@ -266,22 +266,12 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const ReadPara
 // to fp16 relative to the largest contribution; the sum of the softmax is that of w / vs in fp32.  The maximum m is raised only when a score
 // exceeds it by 2^8 (w stays below 256 in fp16), by a vote, so that a step has no shuffles as a rule.
 // ---------------------------------------------------------------------------------------------
-constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32, kRowsStep = 16 * kRowsWarps;
-
-struct AttnParams {
-    PagedKv kv;
-    PagedRows r;
-    const __half* q;
-    __half* out;
-    long long ldq, ldo;
-    int n_heads, group;
-    float scale2;           // softmax scale * log2(e) * kCodeUnit
-    float* partial;         // two partial results for each CTA
-};
+constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32;
+template <int NB> using RowsShare = ShareOf<8 * NB, 16 * kRowsWarps, 1, 1>;
 
 // weighted values / sum of the weights -> four channels of a result row; a row that saw nothing is zero, not-a-number stays
 __device__ __forceinline__ void store_result(__half* dst, const float4& acc, float sum, float unit) {
-    const float inv = sum > 0.f ? unit / sum : (sum == 0.f ? 0.f : sum);
+    const float inv = result_factor(sum, unit);
     __half2 o[2] = {__floats2half2_rn(acc.x * inv, acc.y * inv), __floats2half2_rn(acc.z * inv, acc.w * inv)};
     *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
 }
@@ -308,21 +298,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
     return d;
-}
-__device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; -inf -> 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float log2_fast(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp_fast(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
@@ -355,12 +330,10 @@ template <int HD, int NB> struct RowsCfg {
     static __device__ __forceinline__ int value_swizzle(int row) { return HD >= 128 ? row & 6 : HD == 64 ? (row >> 1) & 3 : 0; }
 };
 
-// rows of a block, HD values and (maximum, sum) each: a CTA's partial results of a segment
-template <int R, int HD> constexpr int kPartial = R * (HD + 2);
-
 template <int HD, int DT, int NB>
 __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_attention_rows_kernel(const AttnParams p) {
     using C = RowsCfg<HD, NB>;
+    using Share = RowsShare<NB>;
     constexpr int R = C::R, S = C::S;               // rows of a block, stages
     constexpr int KW = HD / 16, VW = HD / 32;       // code words of a lane: per key row, per value row
     constexpr int KC = KW < 4 ? KW : 4, VC = VW < 4 ? VW : 4;       // words of one load
@@ -372,25 +345,12 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_addr(sm_rows) + warp * C::RING, scales = smem_addr(sm_rows) + (uint32_t)C::SMEM - (kRowsWarps - warp) * S * 8;
     after_launch_ahead();
-    int b;
-    long long off;
-    const long long total = paged_plan<kRowsThreads, R, kRowsStep>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan, b, off);
-    long long left = share_begin(total, blockIdx.x + 1, gridDim.x) - share_begin(total, blockIdx.x, gridDim.x);
+    Pieces<Share> piece;
+    piece.template begin<kRowsThreads>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan);
 
-    while (left > 0) {
-        const PagedSeq seq = paged_seq<R, kRowsStep>(p.kv, p.r, p.group, b);
-        if (off >= (long long)seq.blocks * p.kv.n_kv * seq.steps) {
-            ++b;
-            off = 0;
-            continue;
-        }
-        const int segment = (int)(off / seq.steps), step0 = (int)(off - (long long)segment * seq.steps);
-        const int step1 = (int)min((long long)seq.steps, step0 + left);
-        const int h = segment % p.kv.n_kv, r0 = segment / p.kv.n_kv * R, n_rows = min(seq.own.y * p.group - r0, R);
-        const int2 own = seq.own;
-        const int start = seq.start;
-        left -= step1 - step0;
-        off += step1 - step0;
+    while (piece.next(p.kv, p.r, p.group)) {
+        const int b = piece.x.b, r0 = piece.x.r0, n_rows = piece.x.n_rows, start = piece.x.start, h = piece.h, step0 = piece.step0, step1 = piece.step1;
+        const int2 own = piece.x.own;
         const int limit_all = min(start + (r0 + n_rows - 1) / p.group, p.kv.capacity - 1);       // the last key that a row sees
         const int n_tiles = min(limit_all / 16 + 1, step1 * kRowsWarps);
 
@@ -569,8 +529,8 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
                 }
             }
         __syncthreads();
-        const bool whole = step0 == 0 && step1 == seq.steps;
-        float* part = p.partial + (size_t)(2 * blockIdx.x + (step0 == 0)) * kPartial<R, HD>;
+        const bool whole = piece.whole();
+        float* part = partial_of<Share, HD>(p.partial, blockIdx.x, step0 == 0);
         for (int i = threadIdx.x; i < n_rows * (HD / 4); i += kRowsThreads) {
             const int r = i / (HD / 4), ch = i % (HD / 4) * 4;
             float mx = -1e30f, sum = 0.f;
@@ -598,34 +558,34 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
     }
 }
 
-// Joins the partial results of segments that several CTAs shared: a CTA a (block of rows, head), a warp a row.  Lane c looks at the
-// maximum and sum of the c-th part, the values are added in the order of the shares, eight parts requested together.
-template <int HD, int DT, int R, int STEP>
-__global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnParams p, int n_cta) {
+// Joins the partial results of segments that several CTAs shared: 32 rows of a (block of rows, head) a CTA, a warp a row.  Lane c looks at
+// the maximum and sum of the c-th part, the values are added in the order of the shares, eight parts requested together.
+template <int HD, int DT, class S>
+__global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnParams p, int n_max) {
     constexpr int VPL = HD / 32;                     // channels of a lane
     __shared__ long long sm_plan[2 * kRowsWarps];
     after_launch_ahead();
-    const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto first = [&](int b) { return (int)((long long)rows_from(p.r, b) * p.group / R) + b; };
-    const int b = last_from(p.r.B, (int)blockIdx.x, first);
-    const PagedSeq seq = paged_seq<R, STEP>(p.kv, p.r, p.group, b);
-    const int rb = (int)blockIdx.x - first(b);
-    if (rb < 0 || rb >= seq.blocks) return;
-    // steps of the sequences before b, and of all
+    const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x;
+    auto sequence = [&](int i) { return last_from(p.r.B, i, [&](int b) { return first_block<S>(p.r, p.group, b); }); };
+    const RowBlock x = row_block<S>(p.kv, p.r, p.group, i, sequence(i));
+    if (x.n_rows <= (int)blockIdx.z * 32) return;
+    // units of the blocks before this one, and of all
     long long before = 0, total = 0;
-    for (int i = threadIdx.x; i < p.r.B; i += kRowsThreads) {
-        const PagedSeq s = paged_seq<R, STEP>(p.kv, p.r, p.group, i);
-        const long long w = (long long)s.blocks * p.kv.n_kv * s.steps;
+    const int blocks = block_count<S>(p.r.N, p.r.B, p.group);
+    for (int k = threadIdx.x; k < blocks; k += kRowsThreads) {
+        const long long w = block_units<S>(p.kv, row_block<S>(p.kv, p.r, p.group, k, sequence(k)));
         total += w;
-        if (i < b) before += w;
+        if (k < i) before += w;
     }
     block_sum2(before, total, sm_plan);
-    const long long u0 = before + ((long long)rb * p.kv.n_kv + h) * seq.steps, u1 = u0 + seq.steps - 1;
+    const int n_cta = share_ctas<S>(total, n_max);
+    const long long u0 = before + (long long)h * (x.steps + S::EXTRA) + S::EXTRA, u1 = u0 + x.steps - 1;
     const int c0 = share_of(total, u0, n_cta), c1 = share_of(total, u1, n_cta);
     if (c0 == c1) return;
-    const int r0 = rb * R, n_rows = min(seq.own.y * p.group - r0, R);
-    auto part_of = [&](int c) { return p.partial + (size_t)(2 * c + (c == c0)) * kPartial<R, HD>; };
-    for (int r = warp; r < n_rows; r += kRowsWarps) {
+    constexpr int R = S::R;
+    const int r0 = x.r0, n_rows = min(x.n_rows, (int)blockIdx.z * 32 + 32);
+    auto part_of = [&](int c) { return partial_of<S, HD>(p.partial, c, c == c0); };
+    for (int r = blockIdx.z * 32 + warp; r < n_rows; r += kRowsWarps) {
         float mx = -1e30f, sum = 0.f, acc[VPL];
 #pragma unroll
         for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
@@ -633,11 +593,11 @@ __global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnPara
             const int c = base + lane;
             const bool live = c <= c1 && share_begin(total, c, n_cta) < share_begin(total, c + 1, n_cta);
             const float2 ml = live ? *reinterpret_cast<const float2*>(part_of(c) + R * HD + 2 * r) : make_float2(-1e30f, 0.f);
-            float x = fmaxf(ml.x, mx);
+            float top = fmaxf(ml.x, mx);
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-            const float f = exp2_fast(mx - x), w = exp2_fast(ml.x - x);
-            mx = x;
+            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float f = exp2_fast(mx - top), w = exp2_fast(ml.x - top);
+            mx = top;
             sum = sum * f + warp_sum(ml.y * w);
 #pragma unroll
             for (int i = 0; i < VPL; ++i) acc[i] *= f;
@@ -659,8 +619,8 @@ __global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnPara
                 }
             }
         }
-        const float inv = sum > 0.f ? kCodeUnit<DT> / sum : (sum == 0.f ? 0.f : sum);
-        __half* dst = p.out + (long long)(seq.own.x + (r0 + r) / p.group) * p.ldo + (h * p.group + (r0 + r) % p.group) * HD + lane * VPL;
+        const float inv = result_factor(sum, kCodeUnit<DT>);
+        __half* dst = p.out + (long long)(x.own.x + (r0 + r) / p.group) * p.ldo + (h * p.group + (r0 + r) % p.group) * HD + lane * VPL;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) dst[i] = __float2half_rn(acc[i] * inv);
     }
@@ -754,9 +714,13 @@ extern "C" int glq_paged_read(const glq_paged_kv_t* kv, const glq_paged_rows_t* 
     });
 }
 
-// How a call runs, from what the host knows.
+// How a call runs, from what the host knows.  More than 16 rows a key/value head: 256 of them at once on the 5th-generation tensor cores, head sizes
+// 64 and 128.
+enum class AttnKernel { rows8, rows16, prompt };
 struct AttnPlan {
-    int nb, grid;          // blocks of 8 rows in a row block; CTAs
+    AttnKernel kernel;
+    int grid;
+    size_t partial;        // floats of a partial result
 };
 int sm_count() {
     int dev = 0, n = 148;
@@ -764,24 +728,24 @@ int sm_count() {
     return n;
 }
 AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
-    const long long most = rows->q_start ? std::min(rows->max_new, rows->rows) : rows->rows / rows->B;
-    AttnPlan a;
-    a.nb = most * (n_heads / kv->n_kv) <= 8 ? 1 : 2;
-    a.grid = sm_count() * (kv->head_dim == 256 || a.nb == 2 ? 1 : 2);
-    return a;
+    const long long most = (rows->q_start ? std::min(rows->max_new, rows->rows) : rows->rows / rows->B) * (long long)(n_heads / kv->n_kv);
+    const int D = kv->head_dim;
+    if (most > 16 && (D == 64 || D == 128)) return {AttnKernel::prompt, sm_count(), (size_t)PromptShare::R * (D + 2)};
+    if (most > 8) return {AttnKernel::rows16, sm_count(), (size_t)16 * (D + 2)};
+    return {AttnKernel::rows8, sm_count() * (D == 256 ? 1 : 2), (size_t)8 * (D + 2)};
 }
 int check_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
     const int bad = check_cache(kv, rows);
     if (bad != GLQ_OK) return bad;
     if (n_heads <= 0 || n_heads % kv->n_kv != 0 || (rows->q_start && rows->max_new < 0)) return GLQ_ERR_ARG;
-    if ((long long)rows->rows * n_heads > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
+    if ((long long)rows->rows * n_heads + rows->B > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
     return GLQ_OK;
 }
 
 extern "C" size_t glq_paged_attention_workspace_bytes(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
     if (check_attention(kv, rows, n_heads) != GLQ_OK || rows->rows == 0 || rows->B == 0) return 0;
     const AttnPlan a = plan_attention(kv, rows, n_heads);
-    return (size_t)a.grid * 2 * (8 * a.nb) * (kv->head_dim + 2) * sizeof(float);
+    return (size_t)a.grid * 2 * a.partial * sizeof(float);
 }
 
 extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, void* out,
@@ -800,18 +764,23 @@ extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_row
         const int group = n_heads / kv->n_kv;
         const AttnParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<__half*>(out), ldq, ldo, n_heads,
                            group, scale * 1.4426950408889634f * kCodeUnit<DT>, static_cast<float*>(workspace)};
+        auto join = [&](auto share) {
+            using S = decltype(share);
+            const dim3 grid((unsigned)block_count<S>(rows->rows, rows->B, group), (unsigned)kv->n_kv, (S::R + 31) / 32);
+            return launch_kernel(true, paged_join_kernel<HD, DT, S>, grid, dim3(kRowsThreads), 0, st, p, plan.grid) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
+        };
         auto run = [&](auto nb) {
-            constexpr int NB = decltype(nb)::value, R = 8 * NB;
-            constexpr size_t smem = RowsCfg<HD, NB>::SMEM;
+            constexpr int NB = decltype(nb)::value;
             static SmemLimit limit;
             auto* kern = paged_attention_rows_kernel<HD, DT, NB>;
-            const long long blocks = (long long)rows->rows * group / R + rows->B;
-            if (blocks > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
-            if (reserve_smem(reinterpret_cast<const void*>(kern), limit, smem) != cudaSuccess) return GLQ_ERR_CUDA;
-            if (launch_kernel(true, kern, dim3((unsigned)plan.grid), dim3(kRowsThreads), smem, st, p) != cudaSuccess) return GLQ_ERR_CUDA;
-            return launch_kernel(true, paged_join_kernel<HD, DT, R, kRowsStep>, dim3((unsigned)blocks, (unsigned)kv->n_kv), dim3(kRowsThreads), 0, st,
-                                 p, plan.grid) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
+            if (reserve_smem(reinterpret_cast<const void*>(kern), limit, RowsCfg<HD, NB>::SMEM) != cudaSuccess ||
+                launch_kernel(true, kern, dim3((unsigned)plan.grid), dim3(kRowsThreads), RowsCfg<HD, NB>::SMEM, st, p) != cudaSuccess)
+                return GLQ_ERR_CUDA;
+            return join(RowsShare<NB>{});
         };
-        return plan.nb == 1 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
+        if constexpr (HD == 64 || HD == 128)
+            if (plan.kernel == AttnKernel::prompt)
+                return launch_paged_prompt(HD, DT, p, plan.grid, st) == cudaSuccess ? join(PromptShare{}) : GLQ_ERR_CUDA;
+        return plan.kernel == AttnKernel::rows8 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
     });
 }

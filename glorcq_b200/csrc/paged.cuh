@@ -67,40 +67,70 @@ __device__ __forceinline__ void after_launch_ahead() {
 }
 
 // ---- sharing out the work of an attention call -----------------------------------------------------------------------
-// A segment is a block of rows of one (sequence, key/value head); its work are steps of STEP tokens.  The steps of all segments, counted in
-// order (sequence, block of rows, head), are cut into equal shares, one for each CTA, whatever the lengths: the lengths are on the device, and
-// a batch of 64 sequences of 800 to 8192 tokens takes as long as its sum, not as its longest.  A segment that a share's end cuts leaves
-// partial results, at most two of them per CTA, which paged_join_kernel joins.
-__host__ __device__ __forceinline__ long long share_begin(long long total, int cta, int n_cta) { return total * cta / n_cta; }
-// the CTA in whose share step u lies
-__device__ __forceinline__ int share_of(long long total, long long u, int n_cta) { return (int)(((u + 1) * n_cta + total - 1) / total) - 1; }
-
-struct PagedSeq {
-    int2 own;               // first row, rows
-    int start, steps, blocks;      // tokens before the call; steps and blocks of rows of a head
+// A segment is a block of R rows (token of the call, head of the group) of one (sequence, key/value head); its work are steps of STEP
+// tokens, up to the last key that a row of it sees, and EXTRA steps' worth of beginning and end.  The units of all segments, counted in order
+// (sequence, block of rows, head), are cut into equal shares, one for each CTA, whatever the lengths: these are on the device, and a batch of
+// 64 sequences of 800 to 8192 tokens takes as long as its sum, not as its longest.  A cut that falls into a segment's EXTRA units parts nothing;
+// another leaves partial results, at most two of them per CTA, which paged_join_kernel joins.
+// Blocks of rows are numbered so that nobody has to count those of the sequences before: sequence b's are rows * group / R + b and on.
+template <int R_, int STEP_, int EXTRA_, int LEAST_> struct ShareOf {
+    static constexpr int R = R_, STEP = STEP_, EXTRA = EXTRA_;
+    static constexpr int LEAST = LEAST_;      // units of a share, so long as there are fewer shares than CTAs
 };
-template <int R, int STEP> __device__ __forceinline__ PagedSeq paged_seq(const PagedKv& kv, const PagedRows& r, int group, int b) {
-    PagedSeq s;
-    s.own = rows_of(r, b);
-    s.start = start_of(r, b, kv.capacity);
-    s.blocks = (s.own.y * group + R - 1) / R;
-    s.steps = s.own.y > 0 ? (min(s.start + s.own.y, kv.capacity) + STEP - 1) / STEP : 0;
-    return s;
+__host__ __device__ __forceinline__ long long share_begin(long long total, int cta, int n_cta) { return total * cta / n_cta; }
+// the CTA in whose share unit u lies
+__device__ __forceinline__ int share_of(long long total, long long u, int n_cta) { return (int)(((u + 1) * n_cta + total - 1) / total) - 1; }
+template <class S> __device__ __forceinline__ int share_ctas(long long total, int n_cta) {
+    return (int)min((long long)n_cta, max(1ll, total / S::LEAST));
 }
-// All threads of the block; `sm`: THREADS / 32 + 3 long longs.  Returns the total; b0, off0: the sequence, and the step of it, where
-// the share of `cta` begins (nothing, where that is empty).
-template <int THREADS, int R, int STEP>
-__device__ __forceinline__ long long paged_plan(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, long long* sm, int& b0, long long& off0) {
+
+struct RowBlock {
+    int b, r0, n_rows;      // sequence; first row of the block, counted from the sequence's; 0 rows: there is no such block
+    int2 own;               // the sequence's first row in the batch, its number of rows
+    int start, steps;
+};
+template <class S> __device__ __forceinline__ int first_block(const PagedRows& r, int group, int b) {
+    return (int)((long long)rows_from(r, b) * group / S::R) + b;
+}
+// block i, in sequence b (first_block(b) <= i, and b the last such)
+template <class S> __device__ __forceinline__ RowBlock row_block(const PagedKv& kv, const PagedRows& r, int group, int i, int b) {
+    RowBlock x;
+    x.b = b;
+    x.own = rows_of(r, b);
+    x.r0 = (i - first_block<S>(r, group, b)) * S::R;
+    x.n_rows = x.r0 < 0 ? 0 : max(0, min(x.own.y * group - x.r0, S::R));
+    x.start = start_of(r, b, kv.capacity);
+    x.steps = x.n_rows > 0 ? min(x.start + (x.r0 + x.n_rows - 1) / group, kv.capacity - 1) / S::STEP + 1 : 0;
+    return x;
+}
+template <class S> __device__ __forceinline__ long long block_units(const PagedKv& kv, const RowBlock& x) {
+    return x.n_rows > 0 ? (long long)kv.n_kv * (x.steps + S::EXTRA) : 0;
+}
+template <class S> __host__ __device__ __forceinline__ int block_count(int rows, int B, int group) {
+    return (int)((long long)rows * group / S::R) + B;
+}
+
+// All threads of the block; `sm`: THREADS / 32 + 3 long longs.  Returns the units of all; i0, off0: the block, and the unit of it, where the
+// share of `cta` begins (nothing, where that is empty).
+template <class S, int THREADS>
+__device__ __forceinline__ long long paged_plan(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, long long* sm, int& i0, long long& off0) {
     constexpr int W = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (r.B + THREADS - 1) / THREADS;
-    auto weight = [&](int b) {
-        const PagedSeq s = paged_seq<R, STEP>(kv, r, group, b);
-        return (long long)s.blocks * kv.n_kv * s.steps;
+    const int blocks = block_count<S>(r.N, r.B, group), per = (blocks + THREADS - 1) / THREADS;
+    const int from = tid * per, to = min(from + per, blocks);
+    auto each = [&](auto&& f) {       // f(block, units) until it says that it is enough
+        if (from >= to) return;
+        int b = last_from(r.B, from, [&](int b) { return first_block<S>(r, group, b); });
+        for (int i = from; i < to; ++i) {
+            while (b + 1 < r.B && first_block<S>(r, group, b + 1) <= i) ++b;
+            if (f(i, block_units<S>(kv, row_block<S>(kv, r, group, i, b)))) return;
+        }
     };
     long long mine = 0;
-    for (int i = 0; i < per; ++i)
-        if (tid * per + i < r.B) mine += weight(tid * per + i);
+    each([&](int, long long w) {
+        mine += w;
+        return false;
+    });
     long long incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -115,24 +145,96 @@ __device__ __forceinline__ long long paged_plan(const PagedKv& kv, const PagedRo
         if (w < warp) before += sm[w];
         total += sm[w];
     }
-    const long long u0 = share_begin(total, cta, n_cta);
+    const int n = share_ctas<S>(total, n_cta);
+    const long long u0 = cta < n ? share_begin(total, cta, n) : total;
     long long at = before + incl - mine;
-    if (mine > 0 && u0 >= at && u0 < at + mine) {
-        for (int i = 0;; ++i) {
-            const long long w = weight(tid * per + i);
+    if (u0 >= at && u0 < at + mine)
+        each([&](int i, long long w) {
             if (u0 < at + w) {
-                sm[W + 1] = tid * per + i;
+                sm[W + 1] = i;
                 sm[W + 2] = u0 - at;
-                break;
+                return true;
             }
             at += w;
-        }
-    }
+            return false;
+        });
     __syncthreads();
-    b0 = (int)sm[W + 1];
+    i0 = (int)sm[W + 1];
     off0 = sm[W + 2];
     return total;
 }
+
+// A CTA's pieces of segments, one after another.
+template <class S> struct Pieces {
+    long long left, off;
+    int i, b;
+    // piece: steps step0 .. step1 of head h of block x
+    RowBlock x;
+    int h, step0, step1;
+    template <int THREADS> __device__ __forceinline__ void begin(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, long long* sm) {
+        const long long total = paged_plan<S, THREADS>(kv, r, group, cta, n_cta, sm, i, off);
+        const int n = share_ctas<S>(total, n_cta);
+        left = cta < n ? share_begin(total, cta + 1, n) - share_begin(total, cta, n) : 0;
+        if (left > 0) b = last_from(r.B, i, [&](int b) { return first_block<S>(r, group, b); });
+    }
+    __device__ __forceinline__ bool next(const PagedKv& kv, const PagedRows& r, int group) {
+        while (left > 0) {
+            x = row_block<S>(kv, r, group, i, b);
+            if (off >= block_units<S>(kv, x)) {
+                ++i;
+                off = 0;
+                while (b + 1 < r.B && first_block<S>(r, group, b + 1) <= i) ++b;
+                continue;
+            }
+            const int units = x.steps + S::EXTRA, v0 = (int)(off % units), v1 = (int)min((long long)units, v0 + left);
+            h = (int)(off / units);
+            off += v1 - v0;
+            left -= v1 - v0;
+            step0 = max(v0 - S::EXTRA, 0);
+            step1 = max(v1 - S::EXTRA, 0);
+            if (step1 > step0) return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ bool whole() const { return step0 == 0 && step1 == x.steps; }
+};
+// where CTA `cta` leaves its partial results of a piece: R rows of HD values, then (maximum, sum) of each row
+template <class S, int HD> constexpr int kPartial = S::R * (HD + 2);
+template <class S, int HD> __device__ __forceinline__ float* partial_of(float* partial, int cta, bool from_first_step) {
+    return partial + (size_t)(2 * cta + from_first_step) * kPartial<S, HD>;
+}
+
+struct AttnParams {
+    PagedKv kv;
+    PagedRows r;
+    const __half* q;
+    __half* out;
+    long long ldq, ldo;
+    int n_heads, group;
+    float scale2;           // softmax scale * log2(e) * kCodeUnit
+    float* partial;         // two partial results for each CTA
+};
+__device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; -inf -> 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Blocks of rows of paged_prompt_kernel (paged_prompt.cu): head sizes 64 and 128, many rows a head.
+using PromptShare = ShareOf<256, 128, 1, 1>;
+cudaError_t launch_paged_prompt(int head_dim, int dtype, const AttnParams& p, int grid, cudaStream_t st);
+
+// what weighted values are multiplied by; a row that saw nothing is zero, not-a-number stays
+__device__ __forceinline__ float result_factor(float sum, float unit) { return sum > 0.f ? unit / sum : (sum == 0.f ? 0.f : sum); }
 
 // ---- codes --------------------------------------------------------------------------------------------------------
 constexpr int kI8 = GLQ_KV_I8, kE4M3 = GLQ_KV_E4M3;

@@ -43,6 +43,8 @@ def check_attention(got, cache, start, new, q, rows=None, scale=None):
         err = (got[r:r + n].cpu().double() - ref).abs()
         assert (err <= tol).all(), f"sequence {b}: {(err / tol.clamp(min=1e-30)).max()} of the bound"
         at += n
+    from glorcq_b200 import tiled
+    assert tiled.debug_error() is None          # no wait ran out
 
 
 # ---- attention -----------------------------------------------------------------------------------------------------------
