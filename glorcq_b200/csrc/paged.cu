@@ -753,7 +753,7 @@ extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_row
     const int bad = check_attention(kv, rows, n_heads);
     if (bad != GLQ_OK) return bad;
     if (rows->rows == 0 || rows->B == 0) return GLQ_OK;
-    if (!q || !out || ldq < (int64_t)n_heads * kv->head_dim || ldo < (int64_t)n_heads * kv->head_dim) return GLQ_ERR_ARG;
+    if (!q || !out || !(scale >= 0.f) || ldq < (int64_t)n_heads * kv->head_dim || ldo < (int64_t)n_heads * kv->head_dim) return GLQ_ERR_ARG;
     if (ldq % 8 || ldo % 8 || !aligned16(q) || !aligned16(out)) return GLQ_ERR_ALIGN;
     if (!workspace || workspace_bytes < glq_paged_attention_workspace_bytes(kv, rows, n_heads)) return GLQ_ERR_WORKSPACE;
     if (!aligned16(workspace)) return GLQ_ERR_ALIGN;

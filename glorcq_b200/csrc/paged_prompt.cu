@@ -5,13 +5,17 @@
 // lies, tokens by channels, which is the MN-major form of the operand).  Tensor memory: S of both tiles, O of both tiles.
 //
 // Warps, which keep their roles over all segments of a CTA:
-//   0..3, 4..7  softmax of tile 0 and 1: a thread has a row; reads S twice (maximum; exponentials), writes P as fp16; brings the row's Q to
-//               shared memory, multiplies O where the maximum has grown, writes the result
-//   8..15       codes to fp16 operands in shared memory, 16 tokens of a step each, so that one page, one pair of scales, is a warp's
-//   16          issues the MMAs: P V of one tile, then the next S of it (whose columns P held until then), then the other tile's, so that
+//   0..3, 4..7  softmax of tile 0 and 1: a thread has a row; writes P as fp16, brings the row's Q to shared memory, multiplies O where m has grown,
+//               writes the result
+//   8..11       codes to fp16 operands in shared memory, two times 16 tokens of a step each, so that one page, one pair of scales, is a
+//               warp's at a time
+//   12          issues the MMAs: P V of one tile, then the next S of it (whose columns P held until then), then the other tile's, so that
 //               one tile's products run while the other's softmax does
-// Scales and maximum as in paged_attention_rows_kernel: w = 2^(ks s + log2 vs - m) in fp16, the sum of w / vs in fp32, m raised only when a
-// score exceeds it by 2^8.
+// Scales and m as in paged_attention_rows_kernel: w = 2^(ks s + log2 vs - m) in fp16, the sum of w / vs in fp32, m raised only when a score exceeds it
+// by 2^8.  Keys that a row does not see get a score of -3e38 in tensor memory, in the steps that have such keys, and the common path has no masks.
+//
+// The loops are rolled where they can be: every warp of a scheduler runs another role's code, and what the instruction cache does not hold costs the
+// one warp that issues the MMAs more than the MMAs (134 cycles an MMA with unrolled loops everywhere).
 //
 // Every wait is bounded (tc_wait); a wait that runs out marks the CTA dead, all roles leave their loops and the kernel ends.
 #include "paged.cuh"
@@ -30,8 +34,11 @@ int glq_paged_error_words(unsigned long long* out4, int clear) {
 namespace glq {
 namespace {
 
-constexpr int kPromptSoftmax = 8, kPromptProducers = 8, kPromptMma = kPromptSoftmax + kPromptProducers;
-constexpr int kPromptThreads = (kPromptMma + 1) * 32;
+constexpr int kPromptSoftmax = 8, kPromptProducers = 4, kPromptMma = kPromptSoftmax + kPromptProducers;
+constexpr int kPromptThreads = (kPromptMma + 4) * 32;        // (three warps of the last warpgroup have no role)
+// Registers of a thread: 128 at launch.
+constexpr int kRegsSoftmax = 152, kRegsProducer = 120, kRegsMma = 88;
+static_assert((kPromptSoftmax * kRegsSoftmax + kPromptProducers * kRegsProducer + 4 * kRegsMma) * 32 <= kPromptThreads * 128, "registers");
 constexpr int kStepTokens = PromptShare::STEP, kGroups = kStepTokens / 16;
 
 template <int HD> struct PromptCfg {
@@ -106,6 +113,27 @@ template <int N> __device__ __forceinline__ void tmem_st(uint32_t taddr, const u
                  "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
+__device__ __forceinline__ unsigned long long pack2(float a, float b) {
+    unsigned long long d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void unpack2(unsigned long long v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // What a role needs of a piece: per tile its rows, the last key that one of them sees, and the steps that it takes part in.
@@ -125,7 +153,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     using C = PromptCfg<HD>;
     extern __shared__ unsigned char prompt_smem[];
     __shared__ __align__(8) unsigned long long bars[2 * 9];
-    __shared__ float s_scale[2][3][kGroups];           // of a stage: ks, log2 vs, 1 / vs of its groups of 16 tokens
+    __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs
     __shared__ long long sm_plan[kPromptThreads / 32 + 3];
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
@@ -163,6 +191,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     bool ok = true;
 
     if (warp < kPromptSoftmax) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         // ================= softmax: a row a thread =================
         const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -178,7 +207,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             if (view.steps > 0) {
                 const __half* src = p.q + (long long)(piece.x.own.x + token) * p.ldq + head * HD;
                 const uint32_t dst = q_smem + tile * C::TILE + row * 128;
-#pragma unroll
+#pragma unroll 8
                 for (int c = 0; c < HD / 8; ++c) {
                     const uint4 v = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
                     sts128(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4), v.x, v.y, v.z, v.w);
@@ -192,37 +221,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 ok = wait_warp(s_full + 8 * tile, done & 1, dead, 120) && wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121);
                 if (!ok) break;
                 tc_fence_after();
-                const float* scale = s_scale[g & 1][0];
+                const float4* scale = s_scale[g & 1];
                 const int first = (piece.step0 + j) * kStepTokens;
-                const bool masked = first + kStepTokens - 1 > limit_low;
-                const int see = limit - first;                    // columns up to here are this row's
-                float top = -INFINITY;
+                if (first + kStepTokens - 1 > limit_low) {
+#pragma unroll 1
+                    for (int c = max(0, (limit_low - first) / 16); c < kGroups; ++c) {
+                        uint32_t v[16];
+                        tc_ld16(s_tm + 16 * c, v);
+                        tc_ld_wait();
 #pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (first + 16 * c + i > limit) v[i] = __float_as_uint(-3e38f);
+                        tmem_st<16>(s_tm + 16 * c, v);
+                    }
+                    tmem_st_wait();
+                }
+                float top = -INFINITY;
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t v[32];
                     tmem_ld32(s_tm + 32 * c, v);
+                    const float4 s0 = scale[2 * c], s1 = scale[2 * c + 1];
                     tc_ld_wait();
+                    float x[2];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const int grp = 2 * c + half;
-                        float x = -INFINITY;
-                        if (masked) {
+                        const uint32_t* u = v + 16 * half;
+                        x[half] = max3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) x = fmaxf(x, 16 * grp + i <= see ? __uint_as_float(v[16 * half + i]) : -INFINITY);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) x = fmaxf(x, __uint_as_float(v[16 * half + i]));
-                        }
-                        // (nothing to see: not 0 times infinity)
-                        top = fmaxf(top, x == -INFINITY ? -INFINITY : x * (scale[grp] * p.scale2) + scale[kGroups + grp]);
+                        for (int i = 3; i < 15; i += 2) x[half] = max3(x[half], __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+                        x[half] = fmaxf(x[half], __uint_as_float(u[15]));
                     }
+                    top = max3(top, fmaf(x[0], s0.x, s0.y), fmaf(x[1], s1.x, s1.y));
                 }
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float up = fmaxf(m, top), f = exp2_fast(m - up);
                     m = up;
                     l *= f;
-                    if (j > 0) {          // (the product before this step's scores has been added)
-#pragma unroll
+                    if (j > 0)            // (the product before this step's scores has been added)
+#pragma unroll 1
                         for (int c = 0; c < HD / 16; ++c) {
                             uint32_t v[16];
                             tc_ld16(o_tm + 16 * c, v);
@@ -231,29 +268,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                             for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
                             tmem_st<16>(o_tm + 16 * c, v);
                         }
-                    }
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     uint32_t v[32], w[16];
                     tmem_ld32(s_tm + 32 * c, v);
+                    const float4 s0 = scale[2 * c], s1 = scale[2 * c + 1];
                     tc_ld_wait();
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const int grp = 2 * c + half;
-                        const float cs = scale[grp] * p.scale2, off = scale[kGroups + grp] - m, iv = scale[2 * kGroups + grp];
-                        float sum = 0.f;
+                        const float cs = half ? s1.x : s0.x, off = (half ? s1.y : s0.y) - m;
+                        const unsigned long long cs2 = pack2(cs, cs), off2 = pack2(off, off);
+                        unsigned long long sum2 = 0ull;
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            float a = exp2_fast(__uint_as_float(v[16 * half + i]) * cs + off), b = exp2_fast(__uint_as_float(v[16 * half + i + 1]) * cs + off);
-                            if (masked) {
-                                a = 16 * grp + i <= see ? a : 0.f;
-                                b = 16 * grp + i + 1 <= see ? b : 0.f;
-                            }
-                            sum += a + b;
+                            float a, b;
+                            unpack2(fma2(pack2(__uint_as_float(v[16 * half + i]), __uint_as_float(v[16 * half + i + 1])), cs2, off2), a, b);
+                            a = exp2_fast(a);
+                            b = exp2_fast(b);
+                            sum2 = add2(sum2, pack2(a, b));
                             w[8 * half + i / 2] = pack_half2(a, b);
                         }
-                        l += sum * iv;
+                        float a, b;
+                        unpack2(sum2, a, b);
+                        l += (a + b) * (half ? s1.z : s0.z);
                     }
                     tmem_st<16>(s_tm + 16 * c, w);
                 }
@@ -271,7 +309,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 __half* out = p.out + (long long)(piece.x.own.x + token) * p.ldo + head * HD;
                 float* part = partial_of<PromptShare, HD>(p.partial, blockIdx.x, piece.step0 == 0);
                 float* mine = part + (128 * tile + row) * HD;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
                     uint32_t v[16];
                     if (view.steps > 0) {
@@ -299,141 +337,139 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             gs += steps;
         }
     } else if (warp < kPromptMma) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsProducer));
         // ================= codes to operands =================
-        constexpr int U = HD / 32, PIECES = HD / 16;        // 16-byte pieces: of a lane, of a row
-        const int group16 = warp - kPromptSoftmax;
-        // Piece u of lane: row of the group, piece of the row; its two 16-byte halves go to pieces 2 c and 2 c + 1 of their block.  With two blocks the
-        // lanes of the second store the odd one first, so that eight lanes meet 32 banks.
-        int row[U], off[U][2];
-        bool odd_first[U];
+        constexpr int U = HD / 32, BLOCKS = HD / 64;        // 16-byte pieces of a lane, 64-channel blocks
+        const int group0 = 2 * (warp - kPromptSoftmax);
+        // Piece u of lane: row lane / 4 + 8 (u / BLOCKS) of a group, piece lane % 4 of block u % BLOCKS; its halves become pieces 2c and 2c + 1 of 8 in the
+        // operand's row.  Eight lanes then meet 32 banks: two rows, one even and one odd.
+        const int r0 = lane >> 2, c0 = lane & 3;
+        const uint32_t even = (16 * group0 + r0) * 128 + (((2 * c0) ^ (r0 & 7)) << 4), odd = (16 * group0 + r0) * 128 + (((2 * c0 + 1) ^ (r0 & 7)) << 4);
+        uint4 kc[2][U], vc[2][U];
+        float ks[2], vs[2];
+        int phys[2], phys1[2], phys2[2];
+        auto request = [&](const unsigned char* pages, const float* scales, int step, const int (&phys)[2], uint4 (&c)[2][U], float (&s)[2]) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = u * 32 + lane, c = i % PIECES;
-            row[u] = i / PIECES;
-            const int r = 16 * group16 + row[u], cc = (c & 3) * 2;
-            odd_first[u] = c >= 4;
-            off[u][0] = (c >> 2) * 16384 + r * 128 + ((cc ^ (r & 7)) << 4);
-            off[u][1] = (c >> 2) * 16384 + r * 128 + (((cc + 1) ^ (r & 7)) << 4);
-        }
-        uint4 kc[U], vc[U];
-        float ks = 0.f, vs = 0.f;
-        auto request = [&](const unsigned char* pages, const float* scales, int step, int phys, uint4 (&c)[U], float& s) {
-            s = 0.f;
-            if (phys >= 0) {
-                const size_t block = (size_t)phys * p.kv.n_kv + piece.h;
-                s = scales[block];
-                const unsigned char* src = pages + ((block << p.kv.page_shift) + ((step * kStepTokens + 16 * group16) & (p.kv.page - 1))) * HD + lane * 16;
+            for (int k = 0; k < 2; ++k) {
+                s[k] = 0.f;
 #pragma unroll
-                for (int u = 0; u < U; ++u) c[u] = *reinterpret_cast<const uint4*>(src + u * 512);
+                for (int u = 0; u < U; ++u) c[k][u] = make_uint4(0u, 0u, 0u, 0u);       // (a page that is not there: zeros)
+                if (phys[k] >= 0) {
+                    const size_t block = (size_t)phys[k] * p.kv.n_kv + piece.h;
+                    s[k] = scales[block];
+                    const unsigned char* src = pages + ((block << p.kv.page_shift) + ((step * kStepTokens + 16 * (group0 + k)) & (p.kv.page - 1))) * HD + r0 * HD + c0 * 16;
+#pragma unroll
+                    for (int u = 0; u < U; ++u) c[k][u] = *reinterpret_cast<const uint4*>(src + (u / BLOCKS) * 8 * HD + (u % BLOCKS) * 64);
+                }
             }
         };
-        auto store = [&](uint32_t tile, const uint4 (&c)[U], bool there) {
+        auto store = [&](uint32_t tile, const uint4 (&c)[2][U]) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                uint32_t h[8];
-                if (there) {
-                    codes_to_half<DT>(c[u].x, h[0], h[1]);
-                    codes_to_half<DT>(c[u].y, h[2], h[3]);
-                    codes_to_half<DT>(c[u].z, h[4], h[5]);
-                    codes_to_half<DT>(c[u].w, h[6], h[7]);
-                } else {
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) h[i] = 0u;
+                for (int u = 0; u < U; ++u) {
+                    uint32_t h[8];
+                    codes_to_half<DT>(c[k][u].x, h[0], h[1]);
+                    codes_to_half<DT>(c[k][u].y, h[2], h[3]);
+                    codes_to_half<DT>(c[k][u].z, h[4], h[5]);
+                    codes_to_half<DT>(c[k][u].w, h[6], h[7]);
+                    const uint32_t at = tile + 2048 * k + (u / BLOCKS) * 1024 + (u % BLOCKS) * 16384;
+                    sts128(at + even, h[0], h[1], h[2], h[3]);
+                    sts128(at + odd, h[4], h[5], h[6], h[7]);
                 }
-                if (odd_first[u]) {
-                    sts128(tile + off[u][1], h[4], h[5], h[6], h[7]);
-                    sts128(tile + off[u][0], h[0], h[1], h[2], h[3]);
-                } else {
-                    sts128(tile + off[u][0], h[0], h[1], h[2], h[3]);
-                    sts128(tile + off[u][1], h[4], h[5], h[6], h[7]);
-                }
-            }
         };
         while (ok && piece.next(p.kv, p.r, p.group)) {
             const int steps = max(tile_view(piece, p, 0).steps, tile_view(piece, p, 1).steps);
-            auto lookup = [&](int j) { return j < steps ? page_of(p.kv, piece.x.b, ((piece.step0 + j) * kStepTokens + 16 * group16) >> p.kv.page_shift) : -1; };
-            int phys = lookup(0), phys1 = lookup(1);
+            auto lookup = [&](int j, int (&to)[2]) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    to[k] = j < steps ? page_of(p.kv, piece.x.b, ((piece.step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
+            };
+            lookup(0, phys);
+            lookup(1, phys1);
             request(p.kv.k, p.kv.k_scale, piece.step0, phys, kc, ks);
             request(p.kv.v, p.kv.v_scale, piece.step0, phys, vc, vs);
             for (int j = 0; j < steps; ++j) {
                 const uint32_t g = gs + j, stage = g & 1, parity = ((g >> 1) & 1) ^ 1;
-                const int phys2 = lookup(j + 2);
+                lookup(j + 2, phys2);
                 if (!(ok = wait_warp(k_empty + 8 * stage, parity, dead, 123))) break;
-                store(k_smem + stage * C::TILE, kc, phys >= 0);
+                store(k_smem + stage * C::TILE, kc);
                 fence_async_smem();
                 arrive_warp(k_full + 8 * stage, lane);
-                const float ks0 = ks, vs0 = vs;
+                const float ks0[2] = {ks[0], ks[1]};
                 request(p.kv.k, p.kv.k_scale, piece.step0 + j + 1, phys1, kc, ks);
                 if (!(ok = wait_warp(v_empty + 8 * stage, parity, dead, 124))) break;
-                store(v_smem + stage * C::TILE, vc, phys >= 0 && vs0 > 0.f);
-                if (lane == 0) {
-                    s_scale[stage][0][group16] = ks0;
-                    s_scale[stage][1][group16] = phys < 0 ? -INFINITY : vs0 > 0.f ? log2_fast(vs0) : 0.f;
-                    s_scale[stage][2][group16] = vs0 > 0.f ? rcp_fast(vs0) : 1.f;
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    if (!(vs[k] > 0.f))           // a block without a scale: its values are zero whatever its codes
+#pragma unroll
+                        for (int u = 0; u < U; ++u) vc[k][u] = make_uint4(0u, 0u, 0u, 0u);
+                store(v_smem + stage * C::TILE, vc);
+                if (lane < 2) {
+                    const float k1 = lane ? ks0[1] : ks0[0], v1 = lane ? vs[1] : vs[0];
+                    const bool there = (lane ? phys[1] : phys[0]) >= 0;
+                    // (a factor above zero: -3e38 times it hides a key)
+                    s_scale[stage][group0 + lane] = make_float4(fmaxf(k1 * p.scale2, 1e-30f), !there ? -INFINITY : v1 > 0.f ? log2_fast(v1) : 0.f,
+                                                                v1 > 0.f ? rcp_fast(v1) : 1.f, 0.f);
                 }
                 fence_async_smem();
                 arrive_warp(v_full + 8 * stage, lane);
                 request(p.kv.v, p.kv.v_scale, piece.step0 + j + 1, phys1, vc, vs);
-                phys = phys1;
-                phys1 = phys2;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    phys[k] = phys1[k];
+                    phys1[k] = phys2[k];
+                }
             }
             gs += steps;
         }
     } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
+        if (warp == kPromptMma) {
         // ================= MMA issue =================
         constexpr uint32_t s_desc = tc_idesc(128), o_desc = tc_idesc(HD) | (1u << 16);       // V: MN-major
-        uint32_t done[2] = {0, 0}, pieces[2] = {0, 0};       // of each tile: steps, pieces that it had steps in
+        uint32_t done = 0, pieces = 0;        // bit t: parity of tile t's steps, of the pieces that it had steps in
         while (ok && piece.next(p.kv, p.r, p.group)) {
-            const int n[2] = {tile_view(piece, p, 0).steps, tile_view(piece, p, 1).steps}, steps = max(n[0], n[1]);
-            auto scores = [&](int tile, uint32_t stage) {
-                const uint32_t a = q_smem + tile * C::TILE, b = k_smem + stage * C::TILE;
-#pragma unroll
-                for (int blk = 0; blk < HD / 64; ++blk)
-                    mma4_ss(tmem + C::S_COL + tile * 128, tc_smem_desc(a + blk * 16384), tc_smem_desc(b + blk * 16384), s_desc, blk > 0);
-                commit_warp(s_full + 8 * tile);
-            };
-            auto values = [&](int tile, uint32_t stage, bool first) {
-                const uint32_t b = v_smem + stage * C::TILE;
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-                    mma4_ts(tmem + C::O_COL + tile * HD, tmem + C::S_COL + tile * 128 + 32 * half, value_desc(b + half * 8192), o_desc, !first || half > 0);
-                commit_warp(pv_done + 8 * tile);
-            };
-            if (steps == 0) continue;
-            ok = wait_warp(k_full + 8 * (gs & 1), (gs >> 1) & 1, dead, 126);
-#pragma unroll
-            for (int tile = 0; tile < 2; ++tile) {
-                if (!ok || n[tile] == 0 || !(ok = wait_warp(q_ready + 8 * tile, pieces[tile] & 1, dead, 125))) continue;
-                tc_fence_after();
-                scores(tile, gs & 1);
-            }
-            if (!ok) break;
-            commit_warp(k_empty + 8 * (gs & 1));
-            for (int j = 0; j < steps && ok; ++j) {
-                const uint32_t g = gs + j, stage = g & 1;
-                ok = wait_warp(v_full + 8 * stage, (g >> 1) & 1, dead, 121) &&
-                     (j + 1 == steps || wait_warp(k_full + 8 * (stage ^ 1), ((g + 1) >> 1) & 1, dead, 126));
-#pragma unroll
-                for (int tile = 0; tile < 2; ++tile) {
-                    if (!ok || j >= n[tile]) continue;
-                    ok = wait_warp(p_ready + 8 * tile, done[tile] & 1, dead, 127) &&
-                         (j > 0 || wait_warp(o_free + 8 * tile, (pieces[tile] & 1) ^ 1, dead, 128));
-                    if (!ok) continue;
-                    tc_fence_after();
-                    values(tile, stage, j == 0);
-                    const bool last = tile == 1 || j >= n[1];
-                    if (last) commit_warp(v_empty + 8 * stage);
-                    if (j + 1 < n[tile]) {
-                        ok = wait_warp(pv_done + 8 * tile, done[tile] & 1, dead, 122);       // P is where the scores go
-                        if (!ok) continue;
-                        scores(tile, stage ^ 1);
+            const int n0 = tile_view(piece, p, 0).steps, n1 = tile_view(piece, p, 1).steps, steps = max(n0, n1);
+            // Round j: P V of step j, then the scores of step j + 1, for the tiles in turn; round -1 has scores alone.
+#pragma unroll 1
+            for (int j = -1; j < steps && ok; ++j) {
+                const uint32_t g = gs + j, stage = g & 1, next = stage ^ 1;
+                if (j >= 0) ok = wait_warp(v_full + 8 * stage, (g >> 1) & 1, dead, 121);
+                if (j + 1 < steps) ok = ok && wait_warp(k_full + 8 * next, ((g + 1) >> 1) & 1, dead, 126);
+#pragma unroll 1
+                for (int tile = 0; tile < 2 && ok; ++tile) {
+                    const int n = tile ? n1 : n0;
+                    const uint32_t s_at = tmem + C::S_COL + tile * 128, o_at = tmem + C::O_COL + tile * HD, bar = 8 * tile;
+                    if (j >= n) continue;
+                    if (j >= 0) {
+                        ok = wait_warp(p_ready + bar, (done >> tile) & 1, dead, 127) &&
+                             (j > 0 || wait_warp(o_free + bar, ((pieces >> tile) & 1) ^ 1, dead, 128));
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t b = v_smem + stage * C::TILE;
+                        mma4_ts(o_at, s_at, value_desc(b), o_desc, j > 0);
+                        mma4_ts(o_at, s_at + 32, value_desc(b + 8192), o_desc, 1);
+                        commit_warp(pv_done + bar);
+                        if (tile == 1 || j >= n1) commit_warp(v_empty + 8 * stage);
                     }
-                    ++done[tile];
+                    if (j + 1 < n) {
+                        ok = j >= 0 ? wait_warp(pv_done + bar, (done >> tile) & 1, dead, 122)              // P is where the scores go
+                                    : wait_warp(q_ready + bar, (pieces >> tile) & 1, dead, 125);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t a = q_smem + tile * C::TILE, b = k_smem + next * C::TILE;
+                        mma4_ss(s_at, tc_smem_desc(a), tc_smem_desc(b), s_desc, 0);
+                        if (HD == 128) mma4_ss(s_at, tc_smem_desc(a + 16384), tc_smem_desc(b + 16384), s_desc, 1);
+                        commit_warp(s_full + bar);
+                    }
+                    if (j >= 0) done ^= 1u << tile;
                 }
-                if (ok && j + 1 < steps) commit_warp(k_empty + 8 * (stage ^ 1));
+                if (ok && j + 1 < steps) commit_warp(k_empty + 8 * next);
             }
             gs += steps;
-            for (int tile = 0; tile < 2; ++tile) pieces[tile] += n[tile] > 0;
+            pieces ^= (n0 > 0) | (n1 > 0) << 1;
+        }
         }
     }
     __syncthreads();

@@ -476,7 +476,7 @@ int glq_paged_append(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, con
 
 /* Causal attention of the call's rows over the cache, the call's own tokens (glq_paged_append before it) among it:
  * out = softmax(scale * q . K^T) V over the keys at positions 0 .. the row's own, head h of n_heads on key/value head
- * h / (n_heads / n_kv).  q, out fp16 (rows, n_heads, head_dim); a row that sees no key is zero.  Scores, softmax and sums in fp32, the
+ * h / (n_heads / n_kv).  q, out fp16 (rows, n_heads, head_dim); a row that sees no key is zero.  scale >= 0.  Scores, softmax and sums in fp32, the
  * probabilities rounded to fp16 as the second product's operand.  Workspace contents irrelevant. */
 size_t glq_paged_attention_workspace_bytes(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads);
 int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, void* out, int64_t ldo,
