@@ -5,12 +5,14 @@
 // lies, tokens by channels, which is the MN-major form of the operand).  Tensor memory: S of both tiles, O of both tiles.
 //
 // Warps, which keep their roles over all segments of a CTA:
-//   0..3, 4..7  softmax of tile 0 and 1: a thread has a row; writes P as fp16, brings the row's Q to shared memory, multiplies O where m has grown,
-//               writes the result
+//   0..3, 4..7  softmax of tile 0 and 1: a thread has a row; writes P as fp16, multiplies O where m has grown, writes the result
 //   8..11       codes to fp16 operands in shared memory, two times 16 tokens of a step each, so that one page, one pair of scales, is a
 //               warp's at a time
-//   12          issues the MMAs: P V of one tile, then the next S of it (whose columns P held until then), then the other tile's, so that
-//               one tile's products run while the other's softmax does
+//   12, 13      issue the MMAs of tile 0 and 1 (one warp for both needed longer for it than the MMAs themselves)
+//   14          brings the rows of the tiles to shared memory, the next segment's while this one's last step is under way
+//   15          works out the CTA's pieces of segments and hands them to the others through a small queue
+// P takes half of the columns of the scores that it is made of, so the next scores of a tile wait for its P V; the other tile's products run
+// meanwhile, and while this one's softmax does.
 // Scales and m as in paged_attention_rows_kernel: w = 2^(ks s + log2 vs - m) in fp16, the sum of w / vs in fp32, m raised only when a score exceeds it
 // by 2^8.  Keys that a row does not see get a score of -3e38 in tensor memory, in the steps that have such keys, and the common path has no masks.
 //
@@ -35,9 +37,9 @@ namespace glq {
 namespace {
 
 constexpr int kPromptSoftmax = 8, kPromptProducers = 4, kPromptMma = kPromptSoftmax + kPromptProducers;
-constexpr int kPromptThreads = (kPromptMma + 4) * 32;        // (three warps of the last warpgroup have no role)
+constexpr int kPromptThreads = (kPromptMma + 4) * 32;
 // Registers of a thread: 128 at launch.
-constexpr int kRegsSoftmax = 152, kRegsProducer = 120, kRegsMma = 88;
+constexpr int kRegsSoftmax = 168, kRegsProducer = 104, kRegsMma = 72;
 static_assert((kPromptSoftmax * kRegsSoftmax + kPromptProducers * kRegsProducer + 4 * kRegsMma) * 32 <= kPromptThreads * 128, "registers");
 constexpr int kStepTokens = PromptShare::STEP, kGroups = kStepTokens / 16;
 
@@ -49,6 +51,10 @@ template <int HD> struct PromptCfg {
 
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* dead, int code) {
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || tc_wait(bar, parity, dead, code));
+}
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, bool live) {       // not live: zeros, nothing is read
+    const int bytes = live ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void arrive_warp(uint32_t bar, int lane) {
     __syncwarp();
@@ -106,6 +112,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
+// tcgen05.wait::ld for values that are used behind it: they are its operands, so that no use is moved in front of it
+__device__ __forceinline__ void tmem_arrived(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]) :: "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
+}
 template <int N> __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* v) {
     static_assert(N == 16, "");
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -136,23 +149,21 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// What a role needs of a piece: per tile its rows, the last key that one of them sees, and the steps that it takes part in.
-struct TileView {
-    int rows, steps;
+// A piece as it is handed out.
+struct PromptPiece {
+    int b, h, row, r0, rows, start;      // sequence, head; the sequence's first row in the batch, the block's first and number of rows; tokens before the call
+    int step0;
+    int steps[2], most;                  // steps that a tile takes part in, the larger of them; most < 0 ends the list
+    int whole;                           // the segment is this CTA's alone
 };
-__device__ __forceinline__ TileView tile_view(const Pieces<PromptShare>& piece, const AttnParams& p, int tile) {
-    TileView v;
-    v.rows = max(0, min(piece.x.n_rows - 128 * tile, 128));
-    const int last = min(piece.x.start + (piece.x.r0 + 128 * tile + v.rows - 1) / p.group, p.kv.capacity - 1);
-    v.steps = v.rows > 0 ? max(0, min(piece.step1, last / kStepTokens + 1) - piece.step0) : 0;
-    return v;
-}
+constexpr int kPieceQueue = 4, kPieceReaders = kPromptSoftmax + kPromptProducers + 3;
 
 template <int HD, int DT>
 __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const AttnParams p) {
     using C = PromptCfg<HD>;
     extern __shared__ unsigned char prompt_smem[];
-    __shared__ __align__(8) unsigned long long bars[2 * 9];
+    __shared__ __align__(8) unsigned long long bars[2 * 10 + 2 * kPieceQueue];
+    __shared__ PromptPiece s_piece[kPieceQueue];
     __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs
     __shared__ long long sm_plan[kPromptThreads / 32 + 3];
     __shared__ uint32_t s_tmem;
@@ -162,19 +173,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     const uint32_t q_smem = base, k_smem = base + 2 * C::TILE, v_smem = base + 4 * C::TILE;
     // [0], [1] of each: stages or tiles
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48, s_full = k_full + 64,
-                   p_ready = k_full + 80, pv_done = k_full + 96, q_ready = k_full + 112, o_free = k_full + 128;
+                   p_ready = k_full + 80, pv_done = k_full + 96, q_ready = k_full + 112, o_free = k_full + 128, q_free = k_full + 144,
+                   piece_full = k_full + 160, piece_empty = piece_full + 8 * kPieceQueue;
     volatile int* dead = &s_dead;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + 8 * i, kPromptProducers);
             mbar_init(v_full + 8 * i, kPromptProducers);
-            mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_empty + 8 * i, 1);
+            mbar_init(k_empty + 8 * i, 2);
+            mbar_init(v_empty + 8 * i, 2);
             mbar_init(s_full + 8 * i, 1);
             mbar_init(pv_done + 8 * i, 1);
             mbar_init(p_ready + 8 * i, 4);
-            mbar_init(q_ready + 8 * i, 4);
+            mbar_init(q_ready + 8 * i, 1);
+            mbar_init(q_free + 8 * i, 1);
             mbar_init(o_free + 8 * i, 4);
+        }
+        for (int i = 0; i < kPieceQueue; ++i) {
+            mbar_init(piece_full + 8 * i, 1);
+            mbar_init(piece_empty + 8 * i, kPieceReaders);
         }
         s_dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -182,13 +199,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     if (warp == kPromptMma) tc_alloc(smem_u32(&s_tmem), 512);
     tc_fence_before();
     after_launch_ahead();
-    Pieces<PromptShare> piece;
-    piece.template begin<kPromptThreads>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan);
+    Pieces<PromptShare> pieces;
+    pieces.template begin<kPromptThreads>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     uint32_t gs = 0;                     // steps of the pieces before, over all roles alike
     bool ok = true;
+    // The pieces in order, for one role's loop: next_piece() waits for one (false: no more), done_piece() gives its place back.
+    uint32_t n_piece = 0;
+    const PromptPiece* piece = s_piece;
+    auto next_piece = [&]() {
+        piece = s_piece + n_piece % kPieceQueue;
+        ok = wait_warp(piece_full + 8 * (n_piece % kPieceQueue), (n_piece / kPieceQueue) & 1, dead, 131);
+        return ok && piece->most >= 0;
+    };
+    auto done_piece = [&]() {
+        arrive_warp(piece_empty + 8 * (n_piece % kPieceQueue), lane);
+        ++n_piece;
+    };
 
     if (warp < kPromptSoftmax) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
@@ -197,38 +226,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_tm = trow + C::S_COL + tile * 128, o_tm = trow + C::O_COL + tile * HD;
         uint32_t done = 0;               // this tile's steps of the pieces before
-        while (ok && piece.next(p.kv, p.r, p.group)) {
-            const TileView view = tile_view(piece, p, tile);
-            const int steps = max(view.steps, tile_view(piece, p, tile ^ 1).steps);
-            const bool live = row < view.rows;
-            const int r = piece.x.r0 + 128 * tile + row, token = live ? r / p.group : 0, head = piece.h * p.group + (live ? r - token * p.group : 0);
-            const int limit = live ? min(piece.x.start + token, p.kv.capacity - 1) : -1;
-            const int limit_low = min(piece.x.start + (piece.x.r0 + 128 * tile) / p.group, p.kv.capacity - 1);       // every live row sees keys up to here
-            if (view.steps > 0) {
-                const __half* src = p.q + (long long)(piece.x.own.x + token) * p.ldq + head * HD;
-                const uint32_t dst = q_smem + tile * C::TILE + row * 128;
-#pragma unroll 8
-                for (int c = 0; c < HD / 8; ++c) {
-                    const uint4 v = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);
-                    sts128(dst + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4), v.x, v.y, v.z, v.w);
-                }
-                fence_async_smem();
-                arrive_warp(q_ready + 8 * tile, lane);
-            }
+        while (next_piece()) {
+            const int steps = piece->steps[tile], first_row = piece->r0 + 128 * tile;
+            const bool live = row < piece->rows - 128 * tile;
+            const int limit = live ? min(piece->start + (first_row + row) / p.group, p.kv.capacity - 1) : -1;      // the last key that the row sees
+            const int limit_low = min(piece->start + first_row / p.group, p.kv.capacity - 1);                      // that every row of the tile sees
+            int first = piece->step0 * kStepTokens;
             float m = -1e30f, l = 0.f;
-            for (int j = 0; j < view.steps && ok; ++j) {
+            for (int j = 0; j < steps && ok; ++j, first += kStepTokens) {
                 const uint32_t g = gs + j;
                 ok = wait_warp(s_full + 8 * tile, done & 1, dead, 120) && wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121);
                 if (!ok) break;
                 tc_fence_after();
                 const float4* scale = s_scale[g & 1];
-                const int first = (piece.step0 + j) * kStepTokens;
                 if (first + kStepTokens - 1 > limit_low) {
 #pragma unroll 1
                     for (int c = max(0, (limit_low - first) / 16); c < kGroups; ++c) {
                         uint32_t v[16];
                         tc_ld16(s_tm + 16 * c, v);
-                        tc_ld_wait();
+                        tmem_arrived(v);
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             if (first + 16 * c + i > limit) v[i] = __float_as_uint(-3e38f);
@@ -236,23 +252,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                     }
                     tmem_st_wait();
                 }
+                // 32 columns at a time, the next ones on their way
+                uint32_t v[2][32];
+                tmem_ld32(s_tm, v[0]);
                 float top = -INFINITY;
-#pragma unroll 1
+#pragma unroll 2
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(s_tm + 32 * c, v);
-                    const float4 s0 = scale[2 * c], s1 = scale[2 * c + 1];
-                    tc_ld_wait();
-                    float x[2];
+                    tmem_arrived(v[c & 1]);
+                    tmem_ld32(s_tm + 32 * ((c + 1) & 3), v[(c + 1) & 1]);         // (and the first ones again)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const uint32_t* u = v + 16 * half;
-                        x[half] = max3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
+                        const uint32_t* u = v[c & 1] + 16 * half;
+                        const float4 sc = scale[2 * c + half];
+                        float x = max3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
 #pragma unroll
-                        for (int i = 3; i < 15; i += 2) x[half] = max3(x[half], __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
-                        x[half] = fmaxf(x[half], __uint_as_float(u[15]));
+                        for (int i = 3; i < 15; i += 2) x = max3(x, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+                        top = fmaxf(top, fmaf(fmaxf(x, __uint_as_float(u[15])), sc.x, sc.y));
                     }
-                    top = max3(top, fmaf(x[0], s0.x, s0.y), fmaf(x[1], s1.x, s1.y));
                 }
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float up = fmaxf(m, top), f = exp2_fast(m - up);
@@ -261,29 +277,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                     if (j > 0)            // (the product before this step's scores has been added)
 #pragma unroll 1
                         for (int c = 0; c < HD / 16; ++c) {
-                            uint32_t v[16];
-                            tc_ld16(o_tm + 16 * c, v);
-                            tc_ld_wait();
+                            uint32_t x[16];
+                            tc_ld16(o_tm + 16 * c, x);
+                            tmem_arrived(x);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                            tmem_st<16>(o_tm + 16 * c, v);
+                            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+                            tmem_st<16>(o_tm + 16 * c, x);
                         }
                 }
-#pragma unroll 1
+#pragma unroll 2
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t v[32], w[16];
-                    tmem_ld32(s_tm + 32 * c, v);
-                    const float4 s0 = scale[2 * c], s1 = scale[2 * c + 1];
-                    tc_ld_wait();
+                    uint32_t w[16];
+                    tmem_arrived(v[c & 1]);
+                    tmem_ld32(s_tm + 32 * (c < 3 ? c + 1 : 3), v[(c + 1) & 1]);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float cs = half ? s1.x : s0.x, off = (half ? s1.y : s0.y) - m;
-                        const unsigned long long cs2 = pack2(cs, cs), off2 = pack2(off, off);
+                        const uint32_t* u = v[c & 1] + 16 * half;
+                        const float4 sc = scale[2 * c + half];
+                        const float off = sc.y - m;
+                        const unsigned long long cs2 = pack2(sc.x, sc.x), off2 = pack2(off, off);
                         unsigned long long sum2 = 0ull;
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
                             float a, b;
-                            unpack2(fma2(pack2(__uint_as_float(v[16 * half + i]), __uint_as_float(v[16 * half + i + 1])), cs2, off2), a, b);
+                            unpack2(fma2(pack2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), cs2, off2), a, b);
                             a = exp2_fast(a);
                             b = exp2_fast(b);
                             sum2 = add2(sum2, pack2(a, b));
@@ -291,7 +308,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                         }
                         float a, b;
                         unpack2(sum2, a, b);
-                        l += (a + b) * (half ? s1.z : s0.z);
+                        l += (a + b) * sc.z;
                     }
                     tmem_st<16>(s_tm + 16 * c, w);
                 }
@@ -300,21 +317,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 arrive_warp(p_ready + 8 * tile, lane);
                 ++done;
             }
-            if (ok && view.steps > 0) ok = wait_warp(pv_done + 8 * tile, (done - 1) & 1, dead, 122);
+            if (ok && steps > 0) ok = wait_warp(pv_done + 8 * tile, (done - 1) & 1, dead, 122);
             if (!ok) break;
             tc_fence_after();
-            if (view.rows > 0) {
-                const bool whole = piece.whole();
+            if (piece->rows > 128 * tile) {
+                const bool whole = piece->whole;
                 const float f = result_factor(l, kCodeUnit<DT>);
-                __half* out = p.out + (long long)(piece.x.own.x + token) * p.ldo + head * HD;
-                float* part = partial_of<PromptShare, HD>(p.partial, blockIdx.x, piece.step0 == 0);
+                const int r = first_row + (live ? row : 0), token = r / p.group;
+                __half* out = p.out + (long long)(piece->row + token) * p.ldo + (piece->h * p.group + r - token * p.group) * HD;
+                float* part = partial_of<PromptShare, HD>(p.partial, blockIdx.x, piece->step0 == 0);
                 float* mine = part + (128 * tile + row) * HD;
 #pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
                     uint32_t v[16];
-                    if (view.steps > 0) {
+                    if (steps > 0) {
                         tc_ld16(o_tm + 16 * c, v);
-                        tc_ld_wait();
+                        tmem_arrived(v);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0u;
@@ -333,8 +351,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 if (live && !whole) *reinterpret_cast<float2*>(part + PromptShare::R * HD + 2 * (128 * tile + row)) = make_float2(m, l);
             }
             tc_fence_before();
-            if (view.steps > 0) arrive_warp(o_free + 8 * tile, lane);
-            gs += steps;
+            if (steps > 0) arrive_warp(o_free + 8 * tile, lane);
+            gs += piece->most;
+            done_piece();
         }
     } else if (warp < kPromptMma) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsProducer));
@@ -347,15 +366,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         const uint32_t even = (16 * group0 + r0) * 128 + (((2 * c0) ^ (r0 & 7)) << 4), odd = (16 * group0 + r0) * 128 + (((2 * c0 + 1) ^ (r0 & 7)) << 4);
         uint4 kc[2][U], vc[2][U];
         float ks[2], vs[2];
-        int phys[2], phys1[2], phys2[2];
+        int phys[2], phys1[2], phys2[2], h = 0;
         auto request = [&](const unsigned char* pages, const float* scales, int step, const int (&phys)[2], uint4 (&c)[2][U], float (&s)[2]) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 s[k] = 0.f;
+                if (phys[k] < 0) {           // a page that is not there: zeros
 #pragma unroll
-                for (int u = 0; u < U; ++u) c[k][u] = make_uint4(0u, 0u, 0u, 0u);       // (a page that is not there: zeros)
-                if (phys[k] >= 0) {
-                    const size_t block = (size_t)phys[k] * p.kv.n_kv + piece.h;
+                    for (int u = 0; u < U; ++u) c[k][u] = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    const size_t block = (size_t)phys[k] * p.kv.n_kv + h;
                     s[k] = scales[block];
                     const unsigned char* src = pages + ((block << p.kv.page_shift) + ((step * kStepTokens + 16 * (group0 + k)) & (p.kv.page - 1))) * HD + r0 * HD + c0 * 16;
 #pragma unroll
@@ -378,17 +398,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                     sts128(at + odd, h[4], h[5], h[6], h[7]);
                 }
         };
-        while (ok && piece.next(p.kv, p.r, p.group)) {
-            const int steps = max(tile_view(piece, p, 0).steps, tile_view(piece, p, 1).steps);
+        while (next_piece()) {
+            const int steps = piece->most, step0 = piece->step0, b = piece->b;
+            h = piece->h;
             auto lookup = [&](int j, int (&to)[2]) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    to[k] = j < steps ? page_of(p.kv, piece.x.b, ((piece.step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
+                for (int k = 0; k < 2; ++k) to[k] = j < steps ? page_of(p.kv, b, ((step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
             };
             lookup(0, phys);
             lookup(1, phys1);
-            request(p.kv.k, p.kv.k_scale, piece.step0, phys, kc, ks);
-            request(p.kv.v, p.kv.v_scale, piece.step0, phys, vc, vs);
+            request(p.kv.k, p.kv.k_scale, step0, phys, kc, ks);
+            request(p.kv.v, p.kv.v_scale, step0, phys, vc, vs);
             for (int j = 0; j < steps; ++j) {
                 const uint32_t g = gs + j, stage = g & 1, parity = ((g >> 1) & 1) ^ 1;
                 lookup(j + 2, phys2);
@@ -397,7 +417,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 fence_async_smem();
                 arrive_warp(k_full + 8 * stage, lane);
                 const float ks0[2] = {ks[0], ks[1]};
-                request(p.kv.k, p.kv.k_scale, piece.step0 + j + 1, phys1, kc, ks);
+                request(p.kv.k, p.kv.k_scale, step0 + j + 1, phys1, kc, ks);
                 if (!(ok = wait_warp(v_empty + 8 * stage, parity, dead, 124))) break;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -414,7 +434,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 }
                 fence_async_smem();
                 arrive_warp(v_full + 8 * stage, lane);
-                request(p.kv.v, p.kv.v_scale, piece.step0 + j + 1, phys1, vc, vs);
+                request(p.kv.v, p.kv.v_scale, step0 + j + 1, phys1, vc, vs);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     phys[k] = phys1[k];
@@ -422,54 +442,126 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 }
             }
             gs += steps;
+            if (!ok) break;
+            done_piece();
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
-        if (warp == kPromptMma) {
-        // ================= MMA issue =================
-        constexpr uint32_t s_desc = tc_idesc(128), o_desc = tc_idesc(HD) | (1u << 16);       // V: MN-major
-        uint32_t done = 0, pieces = 0;        // bit t: parity of tile t's steps, of the pieces that it had steps in
-        while (ok && piece.next(p.kv, p.r, p.group)) {
-            const int n0 = tile_view(piece, p, 0).steps, n1 = tile_view(piece, p, 1).steps, steps = max(n0, n1);
-            // Round j: P V of step j, then the scores of step j + 1, for the tiles in turn; round -1 has scores alone.
-#pragma unroll 1
-            for (int j = -1; j < steps && ok; ++j) {
-                const uint32_t g = gs + j, stage = g & 1, next = stage ^ 1;
-                if (j >= 0) ok = wait_warp(v_full + 8 * stage, (g >> 1) & 1, dead, 121);
-                if (j + 1 < steps) ok = ok && wait_warp(k_full + 8 * next, ((g + 1) >> 1) & 1, dead, 126);
-#pragma unroll 1
-                for (int tile = 0; tile < 2 && ok; ++tile) {
-                    const int n = tile ? n1 : n0;
-                    const uint32_t s_at = tmem + C::S_COL + tile * 128, o_at = tmem + C::O_COL + tile * HD, bar = 8 * tile;
-                    if (j >= n) continue;
-                    if (j >= 0) {
-                        ok = wait_warp(p_ready + bar, (done >> tile) & 1, dead, 127) &&
-                             (j > 0 || wait_warp(o_free + bar, ((pieces >> tile) & 1) ^ 1, dead, 128));
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t b = v_smem + stage * C::TILE;
-                        mma4_ts(o_at, s_at, value_desc(b), o_desc, j > 0);
-                        mma4_ts(o_at, s_at + 32, value_desc(b + 8192), o_desc, 1);
-                        commit_warp(pv_done + bar);
-                        if (tile == 1 || j >= n1) commit_warp(v_empty + 8 * stage);
-                    }
-                    if (j + 1 < n) {
-                        ok = j >= 0 ? wait_warp(pv_done + bar, (done >> tile) & 1, dead, 122)              // P is where the scores go
-                                    : wait_warp(q_ready + bar, (pieces >> tile) & 1, dead, 125);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t a = q_smem + tile * C::TILE, b = k_smem + next * C::TILE;
-                        mma4_ss(s_at, tc_smem_desc(a), tc_smem_desc(b), s_desc, 0);
-                        if (HD == 128) mma4_ss(s_at, tc_smem_desc(a + 16384), tc_smem_desc(b + 16384), s_desc, 1);
-                        commit_warp(s_full + bar);
-                    }
-                    if (j >= 0) done ^= 1u << tile;
+        if (warp < kPromptMma + 2) {
+            // ================= MMA issue =================
+            constexpr uint32_t s_desc = tc_idesc(128), o_desc = tc_idesc(HD) | (1u << 16);       // V: MN-major
+            const int tile = warp - kPromptMma;
+            const uint32_t s_at = tmem + C::S_COL + tile * 128, o_at = tmem + C::O_COL + tile * HD, bar = 8 * tile;
+            const uint64_t q_at = tc_smem_desc(q_smem + tile * C::TILE), k_at = tc_smem_desc(k_smem), v_at = value_desc(v_smem);
+            auto scores = [&](uint32_t stage) {
+                const uint64_t k = k_at + stage * (C::TILE >> 4);
+                mma4_ss(s_at, q_at, k, s_desc, 0);
+                if (HD == 128) mma4_ss(s_at, q_at + (16384 >> 4), k + (16384 >> 4), s_desc, 1);
+                commit_warp(s_full + bar);
+            };
+            uint32_t done = 0, had = 0;           // steps, pieces that the tile had steps in
+            while (next_piece()) {
+                const int n = piece->steps[tile], steps = piece->most;
+                if (n > 0) {
+                    ok = wait_warp(q_ready + bar, had & 1, dead, 125) && wait_warp(k_full + 8 * (gs & 1), (gs >> 1) & 1, dead, 126);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(gs & 1);
                 }
-                if (ok && j + 1 < steps) commit_warp(k_empty + 8 * next);
+                for (int j = 0; j < n; ++j, ++done) {
+                    const uint32_t g = gs + j, stage = g & 1;
+                    ok = wait_warp(p_ready + bar, done & 1, dead, 127) && wait_warp(v_full + 8 * stage, (g >> 1) & 1, dead, 121) &&
+                         (j > 0 || wait_warp(o_free + bar, (had & 1) ^ 1, dead, 128));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t v = v_at + stage * (C::TILE >> 4);
+                    mma4_ts(o_at, s_at, v, o_desc, j > 0);
+                    mma4_ts(o_at, s_at + 32, v + (8192 >> 4), o_desc, 1);
+                    commit_warp(pv_done + bar);
+                    if (lane == 0) {
+                        mbar_arrive(k_empty + 8 * stage);
+                        if (j + 1 == n) mbar_arrive(q_free + bar);
+                    }
+                    ok = (j + 1 == n || wait_warp(k_full + 8 * (stage ^ 1), ((g + 1) >> 1) & 1, dead, 126)) && wait_warp(pv_done + bar, done & 1, dead, 122);
+                    if (!ok) break;
+                    if (j + 1 < n) {
+                        tc_fence_after();
+                        scores(stage ^ 1);
+                    }
+                    if (lane == 0) mbar_arrive(v_empty + 8 * stage);
+                }
+                // steps that only the other tile takes part in
+                for (int j = n; j < steps && ok; ++j) {
+                    const uint32_t g = gs + j, stage = 8 * (g & 1);
+                    ok = wait_warp(k_full + stage, (g >> 1) & 1, dead, 126) && wait_warp(v_full + stage, (g >> 1) & 1, dead, 121);
+                    if (ok && lane == 0) {
+                        mbar_arrive(k_empty + stage);
+                        mbar_arrive(v_empty + stage);
+                    }
+                }
+                if (!ok) break;
+                gs += steps;
+                had += n > 0;
+                done_piece();
             }
-            gs += steps;
-            pieces ^= (n0 > 0) | (n1 > 0) << 1;
-        }
+        } else if (warp == kPromptMma + 2) {
+            // ================= rows to operands =================
+            constexpr int LPR = HD / 8, RPP = 32 / LPR;          // lanes of a row, rows of a pass
+            const int c = lane % LPR;
+            uint32_t had[2] = {0, 0};
+            for (; next_piece() && ok; done_piece()) {
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile) {
+                    if (!ok || piece->steps[tile] == 0 || !(ok = wait_warp(q_free + 8 * tile, (had[tile] & 1) ^ 1, dead, 130))) continue;
+                    ++had[tile];
+                    const int rows = piece->rows - 128 * tile;
+                    const int first = piece->r0 + 128 * tile + lane / LPR;
+                    int token = first / p.group, head = first - token * p.group;
+                    const int more_tokens = RPP / p.group, more_heads = RPP - more_tokens * p.group;
+                    const __half* from = p.q + (long long)piece->row * p.ldq + piece->h * p.group * HD + 8 * c;
+#pragma unroll 4
+                    for (int row = lane / LPR; row < 128; row += RPP) {
+                        const bool live = row < rows;
+                        copy_async_16(q_smem + tile * C::TILE + row * 128 + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4),
+                                      from + (live ? (long long)token * p.ldq + head * HD : 0ll), live);
+                        token += more_tokens;
+                        head += more_heads;
+                        if (head >= p.group) {
+                            head -= p.group;
+                            ++token;
+                        }
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_smem();
+                    arrive_warp(q_ready + 8 * tile, lane);
+                }
+            }
+        } else {
+            // ================= pieces =================
+            for (bool more = true; more && ok; ++n_piece) {
+                ok = wait_warp(piece_empty + 8 * (n_piece % kPieceQueue), ((n_piece / kPieceQueue) & 1) ^ 1, dead, 132);
+                more = ok && pieces.next(p.kv, p.r, p.group);
+                PromptPiece x{};
+                x.most = -1;
+                if (more) {
+                    x.b = pieces.x.b;
+                    x.h = pieces.h;
+                    x.row = pieces.x.own.x;
+                    x.r0 = pieces.x.r0;
+                    x.rows = pieces.x.n_rows;
+                    x.start = pieces.x.start;
+                    x.step0 = pieces.step0;
+                    x.whole = pieces.whole();
+                    for (int tile = 0; tile < 2; ++tile) {
+                        const int rows = min(x.rows - 128 * tile, 128);
+                        const int last = min(x.start + (x.r0 + 128 * tile + rows - 1) / p.group, p.kv.capacity - 1);
+                        x.steps[tile] = rows > 0 ? max(0, min(pieces.step1, last / kStepTokens + 1) - x.step0) : 0;
+                    }
+                    x.most = max(x.steps[0], x.steps[1]);
+                }
+                if (lane == 0 && ok) s_piece[n_piece % kPieceQueue] = x;
+                arrive_warp(piece_full + 8 * (n_piece % kPieceQueue), lane);
+            }
         }
     }
     __syncthreads();
