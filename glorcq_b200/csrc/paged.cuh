@@ -230,7 +230,7 @@ __device__ __forceinline__ float rcp_fast(float x) {
     return y;
 }
 // Blocks of rows of paged_prompt_kernel (paged_prompt.cu): head sizes 64 and 128, many rows a head.
-using PromptShare = ShareOf<256, 128, 1, 1>;
+using PromptShare = ShareOf<256, 128, 2, 1>;
 cudaError_t launch_paged_prompt(int head_dim, int dtype, const AttnParams& p, int grid, cudaStream_t st);
 
 // what weighted values are multiplied by; a row that saw nothing is zero, not-a-number stays

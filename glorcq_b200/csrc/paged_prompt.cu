@@ -7,9 +7,8 @@
 // Warps, which keep their roles over all segments of a CTA:
 //   0..3, 4..7  softmax of tile 0 and 1: a thread has a row; writes P as fp16, multiplies O where m has grown, writes the result
 //   8..11       codes to fp16 operands in shared memory, two times 16 tokens of a step each, so that one page, one pair of scales, is a
-//               warp's at a time
+//               warp's at a time; a segment's rows
 //   12, 13      issue the MMAs of tile 0 and 1 (one warp for both needed longer for it than the MMAs themselves)
-//   14          brings the rows of the tiles to shared memory, the next segment's while this one's last step is under way
 //   15          works out the CTA's pieces of segments and hands them to the others through a small queue
 // P takes half of the columns of the scores that it is made of, so the next scores of a tile wait for its P V; the other tile's products run
 // meanwhile, and while this one's softmax does.
@@ -41,6 +40,8 @@ constexpr int kPromptThreads = (kPromptMma + 4) * 32;
 // Registers of a thread: 128 at launch.
 constexpr int kRegsSoftmax = 168, kRegsProducer = 104, kRegsMma = 72;
 static_assert((kPromptSoftmax * kRegsSoftmax + kPromptProducers * kRegsProducer + 4 * kRegsMma) * 32 <= kPromptThreads * 128, "registers");
+// every so many pairs of exponentials one is taken by exp2_poly
+constexpr int kPolyEvery = 4;
 constexpr int kStepTokens = PromptShare::STEP, kGroups = kStepTokens / 16;
 
 template <int HD> struct PromptCfg {
@@ -142,6 +143,24 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+// 2^x of two values on the multiply-add pipe, the special-function unit being what the exponentials are bound by: a whole number and a rest in
+// [-1/2, 1/2], whose power is a polynomial (minimax by relative error, 2.6e-6), the whole number added to the exponent.  Below -126: about 2^-126,
+// which fp16 has as zero.
+__device__ __forceinline__ void exp2_poly(unsigned long long x, float& a, float& b) {
+    unpack2(x, a, b);
+    const unsigned long long y = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f)), big = pack2(12582912.f, 12582912.f);
+    const unsigned long long t = add2(y, big), f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), y);
+    unsigned long long r = pack2(0.0095701f, 0.0095701f);
+    r = fma2(r, f, pack2(0.05591786f, 0.05591786f));
+    r = fma2(r, f, pack2(0.24024745f, 0.24024745f));
+    r = fma2(r, f, pack2(0.69312181f, 0.69312181f));
+    r = fma2(r, f, pack2(0.99999926f, 0.99999926f));
+    float ta, tb;
+    unpack2(t, ta, tb);
+    unpack2(r, a, b);
+    a = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
+    b = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -156,13 +175,13 @@ struct PromptPiece {
     int steps[2], most;                  // steps that a tile takes part in, the larger of them; most < 0 ends the list
     int whole;                           // the segment is this CTA's alone
 };
-constexpr int kPieceQueue = 4, kPieceReaders = kPromptSoftmax + kPromptProducers + 3;
+constexpr int kPieceQueue = 4, kPieceReaders = kPromptSoftmax + kPromptProducers + 2;
 
 template <int HD, int DT>
 __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const AttnParams p) {
     using C = PromptCfg<HD>;
     extern __shared__ unsigned char prompt_smem[];
-    __shared__ __align__(8) unsigned long long bars[2 * 10 + 2 * kPieceQueue];
+    __shared__ __align__(8) unsigned long long bars[2 * 11 + 2 * kPieceQueue];
     __shared__ PromptPiece s_piece[kPieceQueue];
     __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs
     __shared__ long long sm_plan[kPromptThreads / 32 + 3];
@@ -174,7 +193,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     // [0], [1] of each: stages or tiles
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48, s_full = k_full + 64,
                    p_ready = k_full + 80, pv_done = k_full + 96, q_ready = k_full + 112, o_free = k_full + 128, q_free = k_full + 144,
-                   piece_full = k_full + 160, piece_empty = piece_full + 8 * kPieceQueue;
+                   p_half = k_full + 160, piece_full = k_full + 176, piece_empty = piece_full + 8 * kPieceQueue;
     volatile int* dead = &s_dead;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -185,7 +204,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             mbar_init(s_full + 8 * i, 1);
             mbar_init(pv_done + 8 * i, 1);
             mbar_init(p_ready + 8 * i, 4);
-            mbar_init(q_ready + 8 * i, 1);
+            mbar_init(p_half + 8 * i, 4);
+            mbar_init(q_ready + 8 * i, kPromptProducers);
             mbar_init(q_free + 8 * i, 1);
             mbar_init(o_free + 8 * i, 4);
         }
@@ -235,7 +255,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             float m = -1e30f, l = 0.f;
             for (int j = 0; j < steps && ok; ++j, first += kStepTokens) {
                 const uint32_t g = gs + j;
-                ok = wait_warp(s_full + 8 * tile, done & 1, dead, 120) && wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121);
+                ok = wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121) && wait_warp(s_full + 8 * tile, done & 1, dead, 120);
                 if (!ok) break;
                 tc_fence_after();
                 const float4* scale = s_scale[g & 1];
@@ -285,32 +305,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                             tmem_st<16>(o_tm + 16 * c, x);
                         }
                 }
-#pragma unroll 2
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[16];
-                    tmem_arrived(v[c & 1]);
-                    tmem_ld32(s_tm + 32 * (c < 3 ? c + 1 : 3), v[(c + 1) & 1]);
+#pragma unroll 1
+                for (int c2 = 0; c2 < 4; c2 += 2) {
+                    uint32_t w[32];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t* u = v[c & 1] + 16 * half;
-                        const float4 sc = scale[2 * c + half];
-                        const float off = sc.y - m;
-                        const unsigned long long cs2 = pack2(sc.x, sc.x), off2 = pack2(off, off);
-                        unsigned long long sum2 = 0ull;
+                    for (int c = 0; c < 2; ++c) {
+                        tmem_arrived(v[c]);
+                        if (c2 + c < 3) tmem_ld32(s_tm + 32 * (c2 + c + 1), v[c ^ 1]);
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
+                        for (int half = 0; half < 2; ++half) {
+                            const uint32_t* u = v[c] + 16 * half;
+                            const float4 sc = scale[2 * (c2 + c) + half];
+                            const float off = sc.y - m;
+                            const unsigned long long cs2 = pack2(sc.x, sc.x), off2 = pack2(off, off);
+                            unsigned long long sum2 = 0ull;
+#pragma unroll
+                            for (int i = 0; i < 16; i += 2) {
+                                const unsigned long long x = fma2(pack2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), cs2, off2);
+                                float a, b;
+                                if (i / 2 % kPolyEvery == kPolyEvery - 1) {
+                                    exp2_poly(x, a, b);
+                                } else {
+                                    unpack2(x, a, b);
+                                    a = exp2_fast(a);
+                                    b = exp2_fast(b);
+                                }
+                                sum2 = add2(sum2, pack2(a, b));
+                                w[16 * c + 8 * half + i / 2] = pack_half2(a, b);
+                            }
                             float a, b;
-                            unpack2(fma2(pack2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), cs2, off2), a, b);
-                            a = exp2_fast(a);
-                            b = exp2_fast(b);
-                            sum2 = add2(sum2, pack2(a, b));
-                            w[8 * half + i / 2] = pack_half2(a, b);
+                            unpack2(sum2, a, b);
+                            l += (a + b) * sc.z;
                         }
-                        float a, b;
-                        unpack2(sum2, a, b);
-                        l += (a + b) * sc.z;
                     }
-                    tmem_st<16>(s_tm + 16 * c, w);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) tmem_st<16>(s_tm + 16 * (c2 + c), w + 16 * c);
+                    if (c2 == 0) {          // P V of the first 64 tokens may begin
+                        tmem_st_wait();
+                        tc_fence_before();
+                        arrive_warp(p_half + 8 * tile, lane);
+                    }
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -320,6 +354,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             if (ok && steps > 0) ok = wait_warp(pv_done + 8 * tile, (done - 1) & 1, dead, 122);
             if (!ok) break;
             tc_fence_after();
+            if (m <= -1e30f) l = 0.f;         // nothing seen: the sum is of exp2_poly's smallest numbers
             if (piece->rows > 128 * tile) {
                 const bool whole = piece->whole;
                 const float f = result_factor(l, kCodeUnit<DT>);
@@ -367,6 +402,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         uint4 kc[2][U], vc[2][U];
         float ks[2], vs[2];
         int phys[2], phys1[2], phys2[2], h = 0;
+        uint32_t had = 0;                 // bit t: parity of the pieces that tile t had steps in
         auto request = [&](const unsigned char* pages, const float* scales, int step, const int (&phys)[2], uint4 (&c)[2][U], float (&s)[2]) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -418,6 +454,35 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 arrive_warp(k_full + 8 * stage, lane);
                 const float ks0[2] = {ks[0], ks[1]};
                 request(p.kv.k, p.kv.k_scale, step0 + j + 1, phys1, kc, ks);
+                if (j == 0) {           // the tiles' rows, a quarter a warp
+                    constexpr int LPR = HD / 8, RPP = 32 / LPR;          // lanes of a row, rows of a pass
+                    const int c = lane % LPR, row0 = (warp - kPromptSoftmax) * 32 + lane / LPR;
+                    const int more_tokens = RPP / p.group, more_heads = RPP - more_tokens * p.group;
+                    const __half* from = p.q + (long long)piece->row * p.ldq + h * p.group * HD + 8 * c;
+#pragma unroll 1
+                    for (int tile = 0; tile < 2; ++tile) {
+                        if (!ok || piece->steps[tile] == 0 || !(ok = wait_warp(q_free + 8 * tile, ((had >> tile) & 1) ^ 1, dead, 130))) continue;
+                        had ^= 1u << tile;
+                        int token = (piece->r0 + 128 * tile + row0) / p.group, head = piece->r0 + 128 * tile + row0 - token * p.group;
+                        const int rows = piece->rows - 128 * tile;
+#pragma unroll 2
+                        for (int i = 0; i < 32 / RPP; ++i) {
+                            const int row = row0 + i * RPP;
+                            copy_async_16(q_smem + tile * C::TILE + row * 128 + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4),
+                                          from + (row < rows ? (long long)token * p.ldq + head * HD : 0ll), row < rows);
+                            token += more_tokens;
+                            head += more_heads;
+                            if (head >= p.group) {
+                                head -= p.group;
+                                ++token;
+                            }
+                        }
+                        asm volatile("cp.async.wait_all;" ::: "memory");
+                        fence_async_smem();
+                        arrive_warp(q_ready + 8 * tile, lane);
+                    }
+                    if (!ok) break;
+                }
                 if (!(ok = wait_warp(v_empty + 8 * stage, parity, dead, 124))) break;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -470,20 +535,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 }
                 for (int j = 0; j < n; ++j, ++done) {
                     const uint32_t g = gs + j, stage = g & 1;
-                    ok = wait_warp(p_ready + bar, done & 1, dead, 127) && wait_warp(v_full + 8 * stage, (g >> 1) & 1, dead, 121) &&
-                         (j > 0 || wait_warp(o_free + bar, (had & 1) ^ 1, dead, 128));
+                    // (who has written P has waited for V; the next K is usually there long before P)
+                    ok = (j > 0 || wait_warp(o_free + bar, (had & 1) ^ 1, dead, 128)) &&
+                         (j + 1 == n || wait_warp(k_full + 8 * (stage ^ 1), ((g + 1) >> 1) & 1, dead, 126)) && wait_warp(p_half + bar, done & 1, dead, 127);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t v = v_at + stage * (C::TILE >> 4);
                     mma4_ts(o_at, s_at, v, o_desc, j > 0);
+                    if (!(ok = wait_warp(p_ready + bar, done & 1, dead, 129))) break;
+                    tc_fence_after();
                     mma4_ts(o_at, s_at + 32, v + (8192 >> 4), o_desc, 1);
                     commit_warp(pv_done + bar);
                     if (lane == 0) {
                         mbar_arrive(k_empty + 8 * stage);
                         if (j + 1 == n) mbar_arrive(q_free + bar);
                     }
-                    ok = (j + 1 == n || wait_warp(k_full + 8 * (stage ^ 1), ((g + 1) >> 1) & 1, dead, 126)) && wait_warp(pv_done + bar, done & 1, dead, 122);
-                    if (!ok) break;
+                    if (!(ok = wait_warp(pv_done + bar, done & 1, dead, 122))) break;
                     if (j + 1 < n) {
                         tc_fence_after();
                         scores(stage ^ 1);
@@ -504,39 +571,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 had += n > 0;
                 done_piece();
             }
-        } else if (warp == kPromptMma + 2) {
-            // ================= rows to operands =================
-            constexpr int LPR = HD / 8, RPP = 32 / LPR;          // lanes of a row, rows of a pass
-            const int c = lane % LPR;
-            uint32_t had[2] = {0, 0};
-            for (; next_piece() && ok; done_piece()) {
-#pragma unroll
-                for (int tile = 0; tile < 2; ++tile) {
-                    if (!ok || piece->steps[tile] == 0 || !(ok = wait_warp(q_free + 8 * tile, (had[tile] & 1) ^ 1, dead, 130))) continue;
-                    ++had[tile];
-                    const int rows = piece->rows - 128 * tile;
-                    const int first = piece->r0 + 128 * tile + lane / LPR;
-                    int token = first / p.group, head = first - token * p.group;
-                    const int more_tokens = RPP / p.group, more_heads = RPP - more_tokens * p.group;
-                    const __half* from = p.q + (long long)piece->row * p.ldq + piece->h * p.group * HD + 8 * c;
-#pragma unroll 4
-                    for (int row = lane / LPR; row < 128; row += RPP) {
-                        const bool live = row < rows;
-                        copy_async_16(q_smem + tile * C::TILE + row * 128 + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4),
-                                      from + (live ? (long long)token * p.ldq + head * HD : 0ll), live);
-                        token += more_tokens;
-                        head += more_heads;
-                        if (head >= p.group) {
-                            head -= p.group;
-                            ++token;
-                        }
-                    }
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    fence_async_smem();
-                    arrive_warp(q_ready + 8 * tile, lane);
-                }
-            }
-        } else {
+        } else if (warp == kPromptMma + 3) {
             // ================= pieces =================
             for (bool more = true; more && ok; ++n_piece) {
                 ok = wait_warp(piece_empty + 8 * (n_piece % kPieceQueue), ((n_piece / kPieceQueue) & 1) ^ 1, dead, 132);
