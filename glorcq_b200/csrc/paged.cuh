@@ -60,6 +60,10 @@ __device__ __forceinline__ int page_of(const PagedKv& kv, int b, int j) {
     return p >= 0 && p < kv.n_pages ? p : -1;
 }
 
+// the same in two parts, for who looks ahead: the table's entry (-1 behind its end), and whether that is a page
+__device__ __forceinline__ int page_entry(const PagedKv& kv, int b, int j) { return j < kv.max_pages ? kv.table[b * kv.table_stride + j] : -1; }
+__device__ __forceinline__ bool page_there(const PagedKv& kv, int entry) { return (unsigned)entry < (unsigned)kv.n_pages; }
+
 // what all kernels here do first
 __device__ __forceinline__ void after_launch_ahead() {
     asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -401,13 +401,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         const uint32_t even = (16 * group0 + r0) * 128 + (((2 * c0) ^ (r0 & 7)) << 4), odd = (16 * group0 + r0) * 128 + (((2 * c0 + 1) ^ (r0 & 7)) << 4);
         uint4 kc[2][U], vc[2][U];
         float ks[2], vs[2];
-        int phys[2], phys1[2], phys2[2], h = 0;
+        int phys[2], phys1[2], phys2[2], h = 0;       // entries of the page table: of this step, the next and the one behind that (looked at when used)
         uint32_t had = 0;                 // bit t: parity of the pieces that tile t had steps in
         auto request = [&](const unsigned char* pages, const float* scales, int step, const int (&phys)[2], uint4 (&c)[2][U], float (&s)[2]) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 s[k] = 0.f;
-                if (phys[k] < 0) {           // a page that is not there: zeros
+                if (!page_there(p.kv, phys[k])) {           // zeros
 #pragma unroll
                     for (int u = 0; u < U; ++u) c[k][u] = make_uint4(0u, 0u, 0u, 0u);
                 } else {
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             h = piece->h;
             auto lookup = [&](int j, int (&to)[2]) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) to[k] = j < steps ? page_of(p.kv, b, ((step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
+                for (int k = 0; k < 2; ++k) to[k] = j < steps ? page_entry(p.kv, b, ((step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
             };
             lookup(0, phys);
             lookup(1, phys1);
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 store(v_smem + stage * C::TILE, vc);
                 if (lane < 2) {
                     const float k1 = lane ? ks0[1] : ks0[0], v1 = lane ? vs[1] : vs[0];
-                    const bool there = (lane ? phys[1] : phys[0]) >= 0;
+                    const bool there = page_there(p.kv, lane ? phys[1] : phys[0]);
                     // (a factor above zero: -3e38 times it hides a key)
                     s_scale[stage][group0 + lane] = make_float4(fmaxf(k1 * p.scale2, 1e-30f), !there ? -INFINITY : v1 > 0.f ? log2_fast(v1) : 0.f,
                                                                 v1 > 0.f ? rcp_fast(v1) : 1.f, 0.f);
