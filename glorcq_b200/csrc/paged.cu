@@ -275,25 +275,6 @@ __device__ __forceinline__ void store_result(__half* dst, const float4& acc, flo
     __half2 o[2] = {__floats2half2_rn(acc.x * inv, acc.y * inv), __floats2half2_rn(acc.z * inv, acc.w * inv)};
     *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
 }
-__device__ __forceinline__ void block_sum2(long long& x, long long& y, long long* sm) {      // kRowsThreads threads, 2 kRowsWarps words
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        x += __shfl_xor_sync(0xffffffffu, x, d);
-        y += __shfl_xor_sync(0xffffffffu, y, d);
-    }
-    if ((threadIdx.x & 31) == 0) {
-        sm[threadIdx.x >> 5] = x;
-        sm[kRowsWarps + (threadIdx.x >> 5)] = y;
-    }
-    __syncthreads();
-    x = y = 0;
-#pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) {
-        x += sm[w];
-        y += sm[kRowsWarps + w];
-    }
-}
-
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
@@ -347,6 +328,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
     after_launch_ahead();
     Pieces<Share> piece;
     piece.template begin<kRowsThreads>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan);
+    if (threadIdx.x == 0) p.join[blockIdx.x] = piece.join_item(p.kv, p.r, p.group, blockIdx.x);
 
     while (piece.next(p.kv, p.r, p.group)) {
         const int b = piece.x.b, r0 = piece.x.r0, n_rows = piece.x.n_rows, start = piece.x.start, h = piece.h, step0 = piece.step0, step1 = piece.step1;
@@ -558,40 +540,25 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
     }
 }
 
-// Joins the partial results of segments that several CTAs shared: 32 rows of a (block of rows, head) a CTA, a warp a row.  Lane c looks at
-// the maximum and sum of the c-th part, the values are added in the order of the shares, eight parts requested together.
+// Joins the partial results of segments that several CTAs shared: 32 rows of one a CTA, a warp a row.  Lane c looks at the maximum and sum of
+// the c-th part, the values are added in the order of the shares, eight parts requested together.
 template <int HD, int DT, class S>
-__global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnParams p, int n_max) {
+__global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnParams p) {
     constexpr int VPL = HD / 32;                     // channels of a lane
-    __shared__ long long sm_plan[2 * kRowsWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     after_launch_ahead();
-    const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x;
-    auto sequence = [&](int i) { return last_from(p.r.B, i, [&](int b) { return first_block<S>(p.r, p.group, b); }); };
-    const RowBlock x = row_block<S>(p.kv, p.r, p.group, i, sequence(i));
-    if (x.n_rows <= (int)blockIdx.z * 32) return;
-    // units of the blocks before this one, and of all
-    long long before = 0, total = 0;
-    const int blocks = block_count<S>(p.r.N, p.r.B, p.group);
-    for (int k = threadIdx.x; k < blocks; k += kRowsThreads) {
-        const long long w = block_units<S>(p.kv, row_block<S>(p.kv, p.r, p.group, k, sequence(k)));
-        total += w;
-        if (k < i) before += w;
-    }
-    block_sum2(before, total, sm_plan);
-    const int n_cta = share_ctas<S>(total, n_max);
-    const long long u0 = before + (long long)h * (x.steps + S::EXTRA) + S::EXTRA, u1 = u0 + x.steps - 1;
-    const int c0 = share_of(total, u0, n_cta), c1 = share_of(total, u1, n_cta);
-    if (c0 == c1) return;
+    const JoinItem x = p.join[blockIdx.x];
+    const int r0 = x.r0, n_rows = min(x.n_rows, (int)blockIdx.y * 32 + 32), c0 = x.first_cta, c1 = c0 + x.parts - 1, h = x.h;
+    if (x.parts == 0) return;
     constexpr int R = S::R;
-    const int r0 = x.r0, n_rows = min(x.n_rows, (int)blockIdx.z * 32 + 32);
     auto part_of = [&](int c) { return partial_of<S, HD>(p.partial, c, c == c0); };
-    for (int r = blockIdx.z * 32 + warp; r < n_rows; r += kRowsWarps) {
+    for (int r = blockIdx.y * 32 + warp; r < n_rows; r += kRowsWarps) {
         float mx = -1e30f, sum = 0.f, acc[VPL];
 #pragma unroll
         for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
         for (int base = c0; base <= c1; base += 32) {
             const int c = base + lane;
-            const bool live = c <= c1 && share_begin(total, c, n_cta) < share_begin(total, c + 1, n_cta);
+            const bool live = c <= c1;
             const float2 ml = live ? *reinterpret_cast<const float2*>(part_of(c) + R * HD + 2 * r) : make_float2(-1e30f, 0.f);
             float top = fmaxf(ml.x, mx);
 #pragma unroll
@@ -620,7 +587,7 @@ __global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnPara
             }
         }
         const float inv = result_factor(sum, kCodeUnit<DT>);
-        __half* dst = p.out + (long long)(x.own.x + (r0 + r) / p.group) * p.ldo + (h * p.group + (r0 + r) % p.group) * HD + lane * VPL;
+        __half* dst = p.out + (long long)(x.row + (r0 + r) / p.group) * p.ldo + (h * p.group + (r0 + r) % p.group) * HD + lane * VPL;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) dst[i] = __float2half_rn(acc[i] * inv);
     }
@@ -745,7 +712,7 @@ int check_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int 
 extern "C" size_t glq_paged_attention_workspace_bytes(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
     if (check_attention(kv, rows, n_heads) != GLQ_OK || rows->rows == 0 || rows->B == 0) return 0;
     const AttnPlan a = plan_attention(kv, rows, n_heads);
-    return (size_t)a.grid * 2 * a.partial * sizeof(float);
+    return (size_t)a.grid * (sizeof(JoinItem) + 2 * a.partial * sizeof(float));
 }
 
 extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, const void* q, int64_t ldq, void* out,
@@ -763,11 +730,12 @@ extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_row
         constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
         const int group = n_heads / kv->n_kv;
         const AttnParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<__half*>(out), ldq, ldo, n_heads,
-                           group, scale * 1.4426950408889634f * kCodeUnit<DT>, static_cast<float*>(workspace)};
+                           group, scale * 1.4426950408889634f * kCodeUnit<DT>, static_cast<JoinItem*>(workspace),
+                           reinterpret_cast<float*>(static_cast<JoinItem*>(workspace) + plan.grid)};
         auto join = [&](auto share) {
             using S = decltype(share);
-            const dim3 grid((unsigned)block_count<S>(rows->rows, rows->B, group), (unsigned)kv->n_kv, (S::R + 31) / 32);
-            return launch_kernel(true, paged_join_kernel<HD, DT, S>, grid, dim3(kRowsThreads), 0, st, p, plan.grid) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
+            const dim3 grid((unsigned)plan.grid, (S::R + 31) / 32);
+            return launch_kernel(true, paged_join_kernel<HD, DT, S>, grid, dim3(kRowsThreads), 0, st, p) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
         };
         auto run = [&](auto nb) {
             constexpr int NB = decltype(nb)::value;

@@ -168,17 +168,24 @@ __device__ __forceinline__ long long paged_plan(const PagedKv& kv, const PagedRo
     return total;
 }
 
+// A segment that several CTAs share: written by the second of them, for paged_join_kernel.
+struct JoinItem {
+    int parts, first_cta;        // CTAs first_cta .. first_cta + parts - 1 (0 parts: nothing to join)
+    int row, r0, n_rows, h;      // as in RowBlock
+    int unused[2];
+};
+
 // A CTA's pieces of segments, one after another.
 template <class S> struct Pieces {
-    long long left, off;
-    int i, b;
+    long long left, off, total;
+    int i, b, n_cta;
     // piece: steps step0 .. step1 of head h of block x
     RowBlock x;
     int h, step0, step1;
     template <int THREADS> __device__ __forceinline__ void begin(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, long long* sm) {
-        const long long total = paged_plan<S, THREADS>(kv, r, group, cta, n_cta, sm, i, off);
-        const int n = share_ctas<S>(total, n_cta);
-        left = cta < n ? share_begin(total, cta + 1, n) - share_begin(total, cta, n) : 0;
+        total = paged_plan<S, THREADS>(kv, r, group, cta, n_cta, sm, i, off);
+        this->n_cta = share_ctas<S>(total, n_cta);
+        left = cta < this->n_cta ? share_begin(total, cta + 1, this->n_cta) - share_begin(total, cta, this->n_cta) : 0;
         if (left > 0) b = last_from(r.B, i, [&](int b) { return first_block<S>(r, group, b); });
     }
     __device__ __forceinline__ bool next(const PagedKv& kv, const PagedRows& r, int group) {
@@ -201,6 +208,24 @@ template <class S> struct Pieces {
         return false;
     }
     __device__ __forceinline__ bool whole() const { return step0 == 0 && step1 == x.steps; }
+    // What CTA `cta` has to say to paged_join_kernel, asked before the first next().
+    __device__ __forceinline__ JoinItem join_item(const PagedKv& kv, const PagedRows& r, int group, int cta) const {
+        JoinItem j{};
+        if (left <= 0) return j;
+        const RowBlock x = row_block<S>(kv, r, group, i, b);
+        const int units = x.steps + S::EXTRA, v0 = (int)(off % units);
+        if (v0 <= S::EXTRA) return j;
+        const long long u0 = share_begin(total, cta, n_cta) - v0;
+        const int c0 = share_of(total, u0 + S::EXTRA, n_cta);
+        if (c0 + 1 != cta) return j;
+        j.parts = share_of(total, u0 + units - 1, n_cta) - c0 + 1;
+        j.first_cta = c0;
+        j.row = x.own.x;
+        j.r0 = x.r0;
+        j.n_rows = x.n_rows;
+        j.h = (int)(off / units);
+        return j;
+    }
 };
 // where CTA `cta` leaves its partial results of a piece: R rows of HD values, then (maximum, sum) of each row
 template <class S, int HD> constexpr int kPartial = S::R * (HD + 2);
@@ -216,7 +241,8 @@ struct AttnParams {
     long long ldq, ldo;
     int n_heads, group;
     float scale2;           // softmax scale * log2(e) * kCodeUnit
-    float* partial;         // two partial results for each CTA
+    JoinItem* join;         // an item for each CTA, then
+    float* partial;         // two partial results for each
 };
 __device__ __forceinline__ float exp2_fast(float x) {      // 2 ulp; -inf -> 0
     float y;

@@ -573,6 +573,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             }
         } else if (warp == kPromptMma + 3) {
             // ================= pieces =================
+            if (lane == 0) p.join[blockIdx.x] = pieces.join_item(p.kv, p.r, p.group, blockIdx.x);
             for (bool more = true; more && ok; ++n_piece) {
                 ok = wait_warp(piece_empty + 8 * (n_piece % kPieceQueue), ((n_piece / kPieceQueue) & 1) ^ 1, dead, 132);
                 more = ok && pieces.next(p.kv, p.r, p.group);
