@@ -322,13 +322,12 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
     float* sm_o = sm_rows;                                         // [warp][R][HD]
     float* sm_m = sm_o + kRowsWarps * R * HD;                      // [warp][R]
     float* sm_l = sm_m + kRowsWarps * R;                           // [warp][R]
-    __shared__ long long sm_plan[kRowsWarps + 3];
+    __shared__ ShareStart sm_plan;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_addr(sm_rows) + warp * C::RING, scales = smem_addr(sm_rows) + (uint32_t)C::SMEM - (kRowsWarps - warp) * S * 8;
     after_launch_ahead();
     Pieces<Share> piece;
     piece.template begin<kRowsThreads>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan);
-    if (threadIdx.x == 0) p.join[blockIdx.x] = piece.join_item(p.kv, p.r, p.group, blockIdx.x);
 
     while (piece.next(p.kv, p.r, p.group)) {
         const int b = piece.x.b, r0 = piece.x.r0, n_rows = piece.x.n_rows, start = piece.x.start, h = piece.h, step0 = piece.step0, step1 = piece.step1;
@@ -538,6 +537,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
         }
         __syncthreads();
     }
+    if (threadIdx.x == 0) p.join[blockIdx.x] = join_item<Share>(piece.total, gridDim.x, blockIdx.x, sm_plan);
 }
 
 // Joins the partial results of segments that several CTAs shared: 32 rows of one a CTA, a warp a row.  Lane c looks at the maximum and sum of
@@ -688,6 +688,7 @@ struct AttnPlan {
     AttnKernel kernel;
     int grid;
     size_t partial;        // floats of a partial result
+    bool fits;
 };
 int sm_count() {
     int dev = 0, n = 148;
@@ -697,9 +698,13 @@ int sm_count() {
 AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
     const long long most = (rows->q_start ? std::min(rows->max_new, rows->rows) : rows->rows / rows->B) * (long long)(n_heads / kv->n_kv);
     const int D = kv->head_dim;
-    if (most > 16 && (D == 64 || D == 128)) return {AttnKernel::prompt, sm_count(), (size_t)PromptShare::R * (D + 2)};
-    if (most > 8) return {AttnKernel::rows16, sm_count(), (size_t)16 * (D + 2)};
-    return {AttnKernel::rows8, sm_count() * (D == 256 ? 1 : 2), (size_t)8 * (D + 2)};
+    auto make = [&](AttnKernel kernel, int ctas, auto share) -> AttnPlan {
+        using S = decltype(share);
+        return {kernel, sm_count() * ctas, (size_t)S::R * (D + 2), units_fit<S>(rows->rows, rows->B, n_heads / kv->n_kv, kv->n_kv, kv->max_pages * kv->page)};
+    };
+    if (most > 16 && (D == 64 || D == 128)) return make(AttnKernel::prompt, 1, PromptShare{});
+    if (most > 8) return make(AttnKernel::rows16, 1, RowsShare<2>{});
+    return make(AttnKernel::rows8, D == 256 ? 1 : 2, RowsShare<1>{});
 }
 int check_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
     const int bad = check_cache(kv, rows);
@@ -725,6 +730,7 @@ extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_row
     if (!workspace || workspace_bytes < glq_paged_attention_workspace_bytes(kv, rows, n_heads)) return GLQ_ERR_WORKSPACE;
     if (!aligned16(workspace)) return GLQ_ERR_ALIGN;
     const AttnPlan plan = plan_attention(kv, rows, n_heads);
+    if (!plan.fits) return GLQ_ERR_UNSUPPORTED;
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     return by_type(kv, [&](auto hd, auto dt) {
         constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;

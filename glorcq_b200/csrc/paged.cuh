@@ -81,12 +81,16 @@ template <int R_, int STEP_, int EXTRA_, int LEAST_> struct ShareOf {
     static constexpr int R = R_, STEP = STEP_, EXTRA = EXTRA_;
     static constexpr int LEAST = LEAST_;      // units of a share, so long as there are fewer shares than CTAs
 };
-__host__ __device__ __forceinline__ long long share_begin(long long total, int cta, int n_cta) { return total * cta / n_cta; }
+// Units are counted in 32 bits (the host refuses what might not fit: 64-bit divisions took longer than the rest of a small call's planning).
+__device__ __forceinline__ int share_begin(int total, int cta, int n_cta) { return total / n_cta * cta + total % n_cta * cta / n_cta; }
 // the CTA in whose share unit u lies
-__device__ __forceinline__ int share_of(long long total, long long u, int n_cta) { return (int)(((u + 1) * n_cta + total - 1) / total) - 1; }
-template <class S> __device__ __forceinline__ int share_ctas(long long total, int n_cta) {
-    return (int)min((long long)n_cta, max(1ll, total / S::LEAST));
+__device__ __forceinline__ int share_of(int total, int u, int n_cta) {
+    int c = min((int)((float)u / (float)total * (float)n_cta), n_cta - 1);
+    while (share_begin(total, c, n_cta) > u) --c;
+    while (share_begin(total, c + 1, n_cta) <= u) ++c;
+    return c;
 }
+template <class S> __device__ __forceinline__ int share_ctas(int total, int n_cta) { return min(n_cta, max(1, total / S::LEAST)); }
 
 struct RowBlock {
     int b, r0, n_rows;      // sequence; first row of the block, counted from the sequence's; 0 rows: there is no such block
@@ -107,64 +111,81 @@ template <class S> __device__ __forceinline__ RowBlock row_block(const PagedKv& 
     x.steps = x.n_rows > 0 ? min(x.start + (x.r0 + x.n_rows - 1) / group, kv.capacity - 1) / S::STEP + 1 : 0;
     return x;
 }
-template <class S> __device__ __forceinline__ long long block_units(const PagedKv& kv, const RowBlock& x) {
-    return x.n_rows > 0 ? (long long)kv.n_kv * (x.steps + S::EXTRA) : 0;
+template <class S> __device__ __forceinline__ int block_units(const PagedKv& kv, const RowBlock& x) {
+    return x.n_rows > 0 ? kv.n_kv * (x.steps + S::EXTRA) : 0;
+}
+template <class S> inline bool units_fit(int rows, int B, int group, int n_kv, int capacity) {
+    return ((double)rows * group / S::R + B) * n_kv * ((double)capacity / S::STEP + 1 + S::EXTRA) < 2147483647.0;
 }
 template <class S> __host__ __device__ __forceinline__ int block_count(int rows, int B, int group) {
     return (int)((long long)rows * group / S::R) + B;
 }
 
-// All threads of the block; `sm`: THREADS / 32 + 3 long longs.  Returns the units of all; i0, off0: the block, and the unit of it, where the
-// share of `cta` begins (nothing, where that is empty).
+// Where a CTA's share begins: in block i, x, off units of which belong to shares before; the units of all.
+struct ShareStart {
+    RowBlock x;
+    int i, off;
+    int sums[32];
+};
+// All threads of the block; `sm` in shared memory.  Returns the units of all; what it says of the beginning holds where `cta` has a share.
 template <class S, int THREADS>
-__device__ __forceinline__ long long paged_plan(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, long long* sm, int& i0, long long& off0) {
+__device__ __forceinline__ int paged_plan(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, ShareStart& sm) {
     constexpr int W = THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int blocks = block_count<S>(r.N, r.B, group), per = (blocks + THREADS - 1) / THREADS;
     const int from = tid * per, to = min(from + per, blocks);
-    auto each = [&](auto&& f) {       // f(block, units) until it says that it is enough
+    auto each = [&](auto&& f) {       // f(block, what it is) until it says that it is enough
         if (from >= to) return;
         int b = last_from(r.B, from, [&](int b) { return first_block<S>(r, group, b); });
         for (int i = from; i < to; ++i) {
             while (b + 1 < r.B && first_block<S>(r, group, b + 1) <= i) ++b;
-            if (f(i, block_units<S>(kv, row_block<S>(kv, r, group, i, b)))) return;
+            if (f(i, row_block<S>(kv, r, group, i, b))) return;
         }
     };
-    long long mine = 0;
-    each([&](int, long long w) {
-        mine += w;
+    int mine = 0;
+    RowBlock x{};
+    each([&](int, const RowBlock& y) {
+        x = y;
+        mine += block_units<S>(kv, y);
         return false;
     });
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+        const int o = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += o;
     }
-    if (lane == 31) sm[warp] = incl;
+    if (lane == 31) sm.sums[warp] = incl;
     __syncthreads();
-    long long before = 0, total = 0;
+    int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-        if (w < warp) before += sm[w];
-        total += sm[w];
+        if (w < warp) before += sm.sums[w];
+        total += sm.sums[w];
     }
     const int n = share_ctas<S>(total, n_cta);
-    const long long u0 = cta < n ? share_begin(total, cta, n) : total;
-    long long at = before + incl - mine;
-    if (u0 >= at && u0 < at + mine)
-        each([&](int i, long long w) {
-            if (u0 < at + w) {
-                sm[W + 1] = i;
-                sm[W + 2] = u0 - at;
-                return true;
-            }
-            at += w;
-            return false;
-        });
+    const int u0 = cta < n ? share_begin(total, cta, n) : total;
+    int at = before + incl - mine;
+    if (u0 >= at && u0 < at + mine) {
+        if (per == 1) {
+            sm.x = x;
+            sm.i = from;
+            sm.off = u0 - at;
+        } else {
+            each([&](int i, const RowBlock& y) {
+                const int w = block_units<S>(kv, y);
+                if (u0 < at + w) {
+                    sm.x = y;
+                    sm.i = i;
+                    sm.off = u0 - at;
+                    return true;
+                }
+                at += w;
+                return false;
+            });
+        }
+    }
     __syncthreads();
-    i0 = (int)sm[W + 1];
-    off0 = sm[W + 2];
     return total;
 }
 
@@ -177,28 +198,31 @@ struct JoinItem {
 
 // A CTA's pieces of segments, one after another.
 template <class S> struct Pieces {
-    long long left, off, total;
-    int i, b, n_cta;
-    // piece: steps step0 .. step1 of head h of block x
-    RowBlock x;
-    int h, step0, step1;
-    template <int THREADS> __device__ __forceinline__ void begin(const PagedKv& kv, const PagedRows& r, int group, int cta, int n_cta, long long* sm) {
-        total = paged_plan<S, THREADS>(kv, r, group, cta, n_cta, sm, i, off);
-        this->n_cta = share_ctas<S>(total, n_cta);
-        left = cta < this->n_cta ? share_begin(total, cta + 1, this->n_cta) - share_begin(total, cta, this->n_cta) : 0;
-        if (left > 0) b = last_from(r.B, i, [&](int b) { return first_block<S>(r, group, b); });
+    int left, off, i;
+    RowBlock x;                  // block i
+    int h, step0, step1;         // the piece: steps step0 .. step1 of head h of it
+    int total, n_cta;
+    template <int THREADS> __device__ __forceinline__ void begin(const PagedKv& kv, const PagedRows& r, int group, int cta, int most_ctas, ShareStart& sm) {
+        total = paged_plan<S, THREADS>(kv, r, group, cta, most_ctas, sm);
+        n_cta = share_ctas<S>(total, most_ctas);
+        left = cta < n_cta ? share_begin(total, cta + 1, n_cta) - share_begin(total, cta, n_cta) : 0;
+        i = sm.i;
+        off = sm.off;
+        x = sm.x;
     }
     __device__ __forceinline__ bool next(const PagedKv& kv, const PagedRows& r, int group) {
         while (left > 0) {
-            x = row_block<S>(kv, r, group, i, b);
             if (off >= block_units<S>(kv, x)) {
                 ++i;
                 off = 0;
+                int b = x.b;
                 while (b + 1 < r.B && first_block<S>(r, group, b + 1) <= i) ++b;
+                x = row_block<S>(kv, r, group, i, b);
                 continue;
             }
-            const int units = x.steps + S::EXTRA, v0 = (int)(off % units), v1 = (int)min((long long)units, v0 + left);
-            h = (int)(off / units);
+            const int units = x.steps + S::EXTRA;
+            h = off / units;
+            const int v0 = off - h * units, v1 = min(units, v0 + left);
             off += v1 - v0;
             left -= v1 - v0;
             step0 = max(v0 - S::EXTRA, 0);
@@ -208,25 +232,24 @@ template <class S> struct Pieces {
         return false;
     }
     __device__ __forceinline__ bool whole() const { return step0 == 0 && step1 == x.steps; }
-    // What CTA `cta` has to say to paged_join_kernel, asked before the first next().
-    __device__ __forceinline__ JoinItem join_item(const PagedKv& kv, const PagedRows& r, int group, int cta) const {
-        JoinItem j{};
-        if (left <= 0) return j;
-        const RowBlock x = row_block<S>(kv, r, group, i, b);
-        const int units = x.steps + S::EXTRA, v0 = (int)(off % units);
-        if (v0 <= S::EXTRA) return j;
-        const long long u0 = share_begin(total, cta, n_cta) - v0;
-        const int c0 = share_of(total, u0 + S::EXTRA, n_cta);
-        if (c0 + 1 != cta) return j;
-        j.parts = share_of(total, u0 + units - 1, n_cta) - c0 + 1;
-        j.first_cta = c0;
-        j.row = x.own.x;
-        j.r0 = x.r0;
-        j.n_rows = x.n_rows;
-        j.h = (int)(off / units);
-        return j;
-    }
 };
+// What CTA `cta` has to say to paged_join_kernel.
+template <class S> __device__ __forceinline__ JoinItem join_item(int total, int most_ctas, int cta, const ShareStart& sm) {
+    JoinItem j{};
+    const int n = share_ctas<S>(total, most_ctas);
+    if (cta >= n || share_begin(total, cta, n) == share_begin(total, cta + 1, n)) return j;
+    const int units = sm.x.steps + S::EXTRA, h = sm.off / units, v0 = sm.off - h * units;
+    if (v0 <= S::EXTRA) return j;
+    const int u0 = share_begin(total, cta, n) - v0, c0 = share_of(total, u0 + S::EXTRA, n);
+    if (c0 + 1 != cta) return j;
+    j.parts = share_of(total, u0 + units - 1, n) - c0 + 1;
+    j.first_cta = c0;
+    j.row = sm.x.own.x;
+    j.r0 = sm.x.r0;
+    j.n_rows = sm.x.n_rows;
+    j.h = h;
+    return j;
+}
 // where CTA `cta` leaves its partial results of a piece: R rows of HD values, then (maximum, sum) of each row
 template <class S, int HD> constexpr int kPartial = S::R * (HD + 2);
 template <class S, int HD> __device__ __forceinline__ float* partial_of(float* partial, int cta, bool from_first_step) {

@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     __shared__ __align__(8) unsigned long long bars[2 * 11 + 2 * kPieceQueue];
     __shared__ PromptPiece s_piece[kPieceQueue];
     __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs
-    __shared__ long long sm_plan[kPromptThreads / 32 + 3];
+    __shared__ ShareStart sm_plan;
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -573,7 +573,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             }
         } else if (warp == kPromptMma + 3) {
             // ================= pieces =================
-            if (lane == 0) p.join[blockIdx.x] = pieces.join_item(p.kv, p.r, p.group, blockIdx.x);
             for (bool more = true; more && ok; ++n_piece) {
                 ok = wait_warp(piece_empty + 8 * (n_piece % kPieceQueue), ((n_piece / kPieceQueue) & 1) ^ 1, dead, 132);
                 more = ok && pieces.next(p.kv, p.r, p.group);
@@ -598,6 +597,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 if (lane == 0 && ok) s_piece[n_piece % kPieceQueue] = x;
                 arrive_warp(piece_full + 8 * (n_piece % kPieceQueue), lane);
             }
+            if (lane == 0) p.join[blockIdx.x] = join_item<PromptShare>(pieces.total, gridDim.x, blockIdx.x, sm_plan);
         }
     }
     __syncthreads();
