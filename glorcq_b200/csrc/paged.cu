@@ -1,6 +1,7 @@
 // Paged key/value cache in 8 bits: writing new tokens (glq_paged_append), attention (glq_paged_attention) and reading rows
 // back (glq_paged_read).  include/glorcq_b200.h has the definitions, paged.cuh what the kernels share.
 #include <algorithm>
+#include <utility>
 
 #include "paged.cuh"
 
@@ -281,20 +282,24 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return d;
 }
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// (with the constant parts of the addresses in the instructions: added up in registers they were a fifth of the kernel's whole-number operations)
+template <int DST, int SRC> __device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1+%3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
 }
 __device__ __forceinline__ void copy_async_4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
+template <int WORDS, int OFF> __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
     if (WORDS == 4)
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a), "n"(OFF) : "memory");
     else if (WORDS == 2)
-        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(w[0]), "=r"(w[1]) : "r"(a), "n"(OFF) : "memory");
     else
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
+        asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(w[0]) : "r"(a), "n"(OFF) : "memory");
 }
+template <int... I, class F> __device__ __forceinline__ void unrolled(std::integer_sequence<int, I...>, F&& f) { (f(std::integral_constant<int, I>{}), ...); }
+// f(0), f(1), .. f(N - 1), the number a constant
+template <int N, class F> __device__ __forceinline__ void unrolled(F&& f) { unrolled(std::make_integer_sequence<int, N>{}, f); }
 
 // Shared memory of paged_attention_rows_kernel.  A warp has a ring of its own: S stages of 16 tokens, keys, then values, then the two scales.  A
 // row's 16-byte pieces are stored at piece ^ swizzle(row), so that the fragments' loads (8 lanes together: two rows and four pieces of the keys, four
@@ -367,19 +372,22 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
         // The warp's tiles are i = 0, 1, ..: tokens 16 (8 (step0 + i) + warp) and 15 more.  Lane k has the page of the tile i + k of the
         // current 32, asked for together; -1 ends the list or is a page that is not there.
         const int tile0 = step0 * kRowsWarps + warp, count = tile0 < n_tiles ? (n_tiles - tile0 + kRowsWarps - 1) / kRowsWarps : 0;
-        auto pages_from = [&](int i) { return i + lane < count ? page_of(p.kv, b, (tile0 + (i + lane) * kRowsWarps) * 16 >> p.kv.page_shift) : -1; };
+        auto pages_from = [&](int i) { return i + lane < count ? page_entry(p.kv, b, (tile0 + (i + lane) * kRowsWarps) * 16 >> p.kv.page_shift) : -1; };
         int pages = pages_from(0), pages_next = pages_from(32);
         auto request = [&](int i, int stage, int phys) {
-            if (phys >= 0) {
+            if (page_there(p.kv, phys)) {
                 const size_t block = (size_t)phys * p.kv.n_kv + h;
                 const size_t from = ((block << p.kv.page_shift) + (((tile0 + i * kRowsWarps) * 16) & (p.kv.page - 1))) * HD + lane * 16;
-                const uint32_t at = ring + stage * C::STAGE;
-#pragma unroll
-                for (int u = 0; u < (HD + 31) / 32; ++u) {
-                    const int piece = u * 32 + lane, row = piece / C::PIECES, c = piece % C::PIECES;
-                    copy_async_16(at + row * HD + ((c ^ C::key_swizzle(row)) << 4), p.kv.k + from + u * 512);
-                    copy_async_16(at + 16 * HD + row * HD + ((c ^ C::value_swizzle(row)) << 4), p.kv.v + from + u * 512);
-                }
+                // Pass u of the warp: rows 32 / PIECES u + lane / PIECES.  What the swizzles take from u is a constant too.
+                constexpr int RPP = 32 / C::PIECES;
+                const int row = lane / C::PIECES, c = lane % C::PIECES;
+                const uint32_t at = ring + stage * C::STAGE, k_at = at + row * HD + ((c ^ C::key_swizzle(row)) << 4);
+                const uint32_t v_off = row * HD + ((c ^ C::value_swizzle(row)) << 4);
+                unrolled<(HD + 31) / 32>([&](auto u_) {
+                    constexpr int u = decltype(u_)::value;
+                    copy_async_16<u * 512, u * 512>(k_at ^ (C::key_swizzle(u * RPP) << 4), p.kv.k + from);
+                    copy_async_16<16 * HD + u * 512, u * 512>(at + (v_off ^ (C::value_swizzle(u * RPP) << 4)), p.kv.v + from);
+                });
                 if (lane < 2) copy_async_4(scales + stage * 8 + lane * 4, (lane ? p.kv.v_scale : p.kv.k_scale) + block);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -400,23 +408,22 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
             float ks, vscale;
             asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vscale) : "r"(scales + stage * 8) : "memory");
             uint32_t kw[2][KW], vw[4][VW];
-#pragma unroll
-            for (int c = 0; c < KW / KC; ++c)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int row = g + 8 * u;
-                    const uint32_t a = KC == 4 ? ((t + 4 * c) ^ C::key_swizzle(row)) << 4 : t * 8;
-                    lds_words<KC>(at + row * HD + a, &kw[u][KC * c]);
-                }
-#pragma unroll
-            for (int c = 0; c < VW / VC; ++c)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int row = 2 * t + (u & 1) + 8 * (u >> 1);
-                    const uint32_t a = VC == 4 ? ((g + 8 * c) ^ C::value_swizzle(row)) << 4
-                                     : VC == 2 ? (((g >> 1) ^ C::value_swizzle(row)) << 4) + (g & 1) * 8 : g * 4;
-                    lds_words<VC>(at + 16 * HD + row * HD + a, &vw[u][VC * c]);
-                }
+            unrolled<KW / KC>([&](auto c_) {
+                constexpr int c = decltype(c_)::value;
+                const uint32_t a = at + (KC == 4 ? g * HD + (((t + 4 * (c & 1)) ^ C::key_swizzle(g)) << 4) : g * HD + t * 8);
+                lds_words<KC, 64 * (c & ~1)>(a, &kw[0][KC * c]);
+                lds_words<KC, 8 * HD + 64 * (c & ~1)>(a, &kw[1][KC * c]);          // (row g + 8 has row g's swizzle)
+            });
+            unrolled<VW / VC>([&](auto c_) {
+                constexpr int c = decltype(c_)::value;
+                // (so have 2t and 2t + 1, and 8 more)
+                const uint32_t a = at + 2 * t * HD + (VC == 4 ? (g ^ C::value_swizzle(2 * t)) << 4
+                                                    : VC == 2 ? (((g >> 1) ^ C::value_swizzle(2 * t)) << 4) + (g & 1) * 8 : g * 4);
+                unrolled<4>([&](auto u_) {
+                    constexpr int u = decltype(u_)::value;
+                    lds_words<VC, 16 * HD + ((u & 1) + 8 * (u >> 1)) * HD + 128 * c>(a, &vw[u][VC * c]);
+                });
+            });
             float s[NB][4];
 #pragma unroll
             for (int n = 0; n < NB; ++n)
@@ -433,14 +440,14 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
             const float c = ks * p.scale2, lv = vscale > 0.f ? log2_fast(vscale) : 0.f, iv = vscale > 0.f ? rcp_fast(vscale) : 1.f;
             // w of token g (+ 8) and rows 2t, 2t + 1 of each block of rows
             uint32_t pf[NB][2];
-            const bool masked = tile * 16 + 15 > limit_low || phys < 0;
+            const bool there = page_there(p.kv, phys), masked = tile * 16 + 15 > limit_low || !there;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 const int tok = tile * 16 + g;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[n][e] = s[n][e] * c + lv;
-                    if (masked && (phys < 0 || tok + 8 * (e >> 1) > limit[n][e & 1])) s[n][e] = -INFINITY;
+                    if (masked && (!there || tok + 8 * (e >> 1) > limit[n][e & 1])) s[n][e] = -INFINITY;
                 }
                 const float hi0 = fmaxf(s[n][0], s[n][2]), hi1 = fmaxf(s[n][1], s[n][3]);
                 if (__any_sync(0xffffffffu, hi0 > m[n][0] + 8.f || hi1 > m[n][1] + 8.f)) {
