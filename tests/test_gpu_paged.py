@@ -64,6 +64,18 @@ def test_attention_of_a_decoded_token(dev, dtype, heads, kv, D, P, held):
     got = paged_attention(q, *cache, i64(held, dev))
     check_attention(got, cache, held, [1] * len(held), q)
     assert torch.equal(got, paged_attention(q, *cache, i64(held, dev)))
+    # a table with room for long sequences: the work is shared out evenly instead of a cluster taking a sequence and head
+    long = wide(cache, 40000)
+    got = paged_attention(q, *long, i64(held, dev))
+    check_attention(got, cache, held, [1] * len(held), q)
+    assert torch.equal(got, paged_attention(q, *long, i64(held, dev)))
+
+
+def wide(cache, tokens):
+    """The cache with a table of that many tokens a sequence, the new places empty."""
+    table = torch.full((cache[4].shape[0], tokens // cache[0].shape[2] + 1), -1, dtype=torch.int32, device=cache[4].device)
+    table[:, : cache[4].shape[1]] = cache[4]
+    return [*cache[:4], table]
 
 
 CHUNKS = [  # dtype, heads, kv heads, D, page, held, new
@@ -83,6 +95,7 @@ def test_attention_of_several_tokens(dev, dtype, heads, kv, D, P, held, new):
     assert torch.equal(got, paged_attention(q, *cache, i64(held, dev), q_starts(new, dev), max_new=max(new)))
     # the most rows of a sequence not told: perhaps another kernel
     check_attention(paged_attention(q, *cache, i64(held, dev), q_starts(new, dev)), cache, held, new, q)
+    check_attention(paged_attention(q, *wide(cache, 40000), i64(held, dev), q_starts(new, dev), max_new=max(new)), cache, held, new, q)
     if len(set(new)) == 1:
         assert torch.equal(got, paged_attention(q, *cache, i64(held, dev)))
 
