@@ -10,11 +10,12 @@ using namespace glq;
 namespace {
 
 // ---------------------------------------------------------------------------------------------
-// Append.  A block of a page and head is one CTA's: its scale needs the largest value of all new tokens before a code can be written.  The values
-// are computed twice (second time from the first-level cache) unless one pass of the CTA covers them.  Two halves of a row that the
-// rotation mixes belong to one lane: lane c of HD / 16 has channels 8c .. 8c+7 and HD/2 + 8c .. .  Bound by memory.
+// Append.  A block of a page and head is one CTA's: its scale needs the largest value of all new tokens before a code can be written.  Up to four rows a
+// lane stay in registers in between; of larger blocks the values are computed twice (the second time from the caches).  Two halves of a row that the
+// rotation mixes belong to one lane: lane c of HD / 16 has channels 8c .. 8c+7 and HD/2 + 8c .. .  Queries: a CTA a row, whose lanes use a
+// position's angles for all their heads.  Bound by memory: what counts is that a lane's loads are all requested before the first is used.
 // ---------------------------------------------------------------------------------------------
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 128, kAppendCtas = 4;       // CTAs an SM: with five, registers spill
 
 struct AppendParams {
     PagedKv kv;
@@ -23,154 +24,207 @@ struct AppendParams {
     __half* q_out;
     const float *cos, *sin;
     long long ldq, ldk, ldv, ldqo;
-    int n_heads, page_items, cos_rows;
+    int n_heads, page_items, cos_rows, query_rows, stride;       // (rows of queries that a CTA takes at once; every so many CTAs one has a block)
     float eps;
 };
+constexpr int kAppendHeld = 4;
 
-struct RowHalves {
+struct __align__(16) RowHalves {
     float a[8], b[8];      // first half's channels, second half's
 };
-__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
-    __align__(16) __half h[8];
-    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void widen8(const uint4& w, float (&f)[8]) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __half2float(h[i]);
-}
-__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
-    __align__(16) __half h[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = __float2half_rn(f[i]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
-}
-// Norm and rotation of one row by its HD / 16 lanes, in fp32; products and sums rounded one by one, so that they do not depend on
-// what the compiler contracts.  pos < 0: no rotation.
-template <int HD>
-__device__ __forceinline__ void norm_rotate(RowHalves& x, const __half* norm, float eps, const float* cos, const float* sin, int pos, int c) {
-    constexpr int LPR = HD / 16;
-    if (norm) {
-        float ss = 0.f, wa[8], wb[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
-#pragma unroll
-        for (int d = LPR / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        const float r = rsqrtf(ss / HD + eps);
-        load8(norm + 8 * c, wa);
-        load8(norm + HD / 2 + 8 * c, wb);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x.a[i] = x.a[i] * r * wa[i];
-            x.b[i] = x.b[i] * r * wb[i];
-        }
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&in[i]));
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
     }
-    if (cos && pos >= 0) {
-        __align__(16) float cs[8], sn[8];
-        const float4* cp = reinterpret_cast<const float4*>(cos + (size_t)pos * (HD / 2) + 8 * c);
-        const float4* sp = reinterpret_cast<const float4*>(sin + (size_t)pos * (HD / 2) + 8 * c);
-        reinterpret_cast<float4*>(cs)[0] = cp[0];
-        reinterpret_cast<float4*>(cs)[1] = cp[1];
-        reinterpret_cast<float4*>(sn)[0] = sp[0];
-        reinterpret_cast<float4*>(sn)[1] = sp[1];
+}
+__device__ __forceinline__ uint4 narrow8(const float (&f)[8]) {
+    return make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+}
+// RMS norm of one row by its HD / 16 lanes, in fp32.
+template <int HD> __device__ __forceinline__ void norm_row(RowHalves& x, const RowHalves& w, float eps) {
+    float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float a = __fsub_rn(__fmul_rn(x.a[i], cs[i]), __fmul_rn(x.b[i], sn[i]));
-            x.b[i] = __fadd_rn(__fmul_rn(x.b[i], cs[i]), __fmul_rn(x.a[i], sn[i]));
-            x.a[i] = a;
-        }
+    for (int i = 0; i < 8; ++i) ss += x.a[i] * x.a[i] + x.b[i] * x.b[i];
+#pragma unroll
+    for (int d = HD / 32; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    const float r = rsqrtf(ss / HD + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x.a[i] = x.a[i] * r * w.a[i];
+        x.b[i] = x.b[i] * r * w.b[i];
+    }
+}
+// A lane's cosines (a) and sines (b) of a position.
+template <int HD> __device__ __forceinline__ void load_angles(RowHalves& cs, const float* cos, const float* sin, int pos, int c) {
+    const float4* cp = reinterpret_cast<const float4*>(cos + (size_t)pos * (HD / 2) + 8 * c);
+    const float4* sp = reinterpret_cast<const float4*>(sin + (size_t)pos * (HD / 2) + 8 * c);
+    reinterpret_cast<float4*>(cs.a)[0] = cp[0];
+    reinterpret_cast<float4*>(cs.a)[1] = cp[1];
+    reinterpret_cast<float4*>(cs.b)[0] = sp[0];
+    reinterpret_cast<float4*>(cs.b)[1] = sp[1];
+}
+// Products and sums rounded one by one, so that they do not depend on what the compiler contracts.
+__device__ __forceinline__ void rotate(RowHalves& x, const RowHalves& cs) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float a = __fsub_rn(__fmul_rn(x.a[i], cs.a[i]), __fmul_rn(x.b[i], cs.b[i]));
+        x.b[i] = __fadd_rn(__fmul_rn(x.b[i], cs.a[i]), __fmul_rn(x.a[i], cs.b[i]));
+        x.a[i] = a;
     }
 }
 
 template <int DT> __device__ __forceinline__ uint2 codes8(const float (&f)[8], float inv) {
-    uint2 w = make_uint2(0u, 0u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w.x |= to_code<DT>(__fmul_rn(f[i], inv)) << (8 * i);
-        w.y |= to_code<DT>(__fmul_rn(f[i + 4], inv)) << (8 * i);
-    }
-    return w;
+    return make_uint2(to_codes<DT>(__fmul_rn(f[0], inv), __fmul_rn(f[1], inv), __fmul_rn(f[2], inv), __fmul_rn(f[3], inv)),
+                      to_codes<DT>(__fmul_rn(f[4], inv), __fmul_rn(f[5], inv), __fmul_rn(f[6], inv), __fmul_rn(f[7], inv)));
 }
 
 template <int HD, int DT>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kernel(const AppendParams p) {
     constexpr int LPR = HD / 16, RPP = kAppendThreads / LPR;       // lanes of a row, rows of a pass
     const int tid = threadIdx.x, c = tid % LPR, slot = tid / LPR;
     after_launch_ahead();
-    const int block_items = p.page_items * 2 * p.kv.n_kv;
-    if ((int)blockIdx.x >= block_items) {                          // queries: 2 RPP (row, head) pairs
-        const long long total = (long long)p.r.N * p.n_heads;
-#pragma unroll 1
-        for (int u = 0; u < 2; ++u) {
-            const long long i = ((long long)((int)blockIdx.x - block_items) * 2 + u) * RPP + slot;
-            const bool live = i < total;
-            const int row = live ? (int)(i / p.n_heads) : 0, h = live ? (int)(i - (long long)row * p.n_heads) : 0;
-            // rows in front of the first sequence or behind the last are not touched
-            const int b = last_from(p.r.B, row, [&](int b) { return rows_from(p.r, b); });
-            const int2 own = rows_of(p.r, b);
-            const bool mine = live && row >= own.x && row - own.x < own.y;
-            RowHalves x = {};
-            if (mine) {
+    const PagedRows& rows = p.r;
+    // Blocks, whose scale waits for their last load, and queries, which stream, in turn.
+    const int block_items = p.page_items * 2 * p.kv.n_kv, turn = (int)blockIdx.x / p.stride;
+    const bool is_block = turn < block_items && turn * p.stride == (int)blockIdx.x;
+    const int work = is_block ? turn : (int)blockIdx.x - min(turn + 1, block_items);
+    RowHalves weight = {};
+    auto load_weight = [&](const __half* w) {
+        widen8(*reinterpret_cast<const uint4*>(w + 8 * c), weight.a);
+        widen8(*reinterpret_cast<const uint4*>(w + HD / 2 + 8 * c), weight.b);
+    };
+    if (!is_block) {                                    // queries
+        // one row, the heads of which go round the slots, or as many whole rows as there are slots for
+        const int row = work * p.query_rows + (p.query_rows > 1 ? slot / p.n_heads : 0);
+        const int first = p.query_rows > 1 ? slot % p.n_heads : slot;
+        const bool there = row < p.r.N && (p.query_rows == 1 || slot < p.query_rows * p.n_heads);
+        // row b is usually sequence b's where a sequence has one token
+        int b = min(there ? row : 0, rows.B - 1);
+        int2 own = rows_of(rows, b);
+        if (row < own.x || row - own.x >= own.y) {
+            b = last_from(rows.B, there ? row : 0, [&](int b) { return rows_from(rows, b); });
+            own = rows_of(rows, b);
+        }
+        // rows in front of the first sequence or behind the last are not touched
+        const bool mine = there && row >= own.x && row - own.x < own.y;
+        RowHalves cs = {};
+        if (mine && p.cos) {
+            const long long at = (long long)start_of(rows, b, p.kv.capacity) + (row - own.x);
+            load_angles<HD>(cs, p.cos, p.sin, (int)min(at, (long long)p.cos_rows - 1), c);
+        }
+        if (p.q_norm) load_weight(p.q_norm);
+        const int rounds = p.query_rows > 1 ? 1 : (p.n_heads + RPP - 1) / RPP;       // (alike for all threads, who stay together for the norm's shuffles)
+        for (int k = 0; k < rounds; k += 2) {
+            uint4 raw[2][2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int h = first + (k + u) * RPP;
+                const bool live = mine && k + u < rounds && h < p.n_heads;
                 const __half* src = p.q + row * p.ldq + h * HD + 8 * c;
-                load8(src, x.a);
-                load8(src + HD / 2, x.b);
+                raw[u][0] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+                raw[u][1] = live ? *reinterpret_cast<const uint4*>(src + HD / 2) : make_uint4(0u, 0u, 0u, 0u);
             }
-            const long long at = mine ? (long long)start_of(p.r, b, p.kv.capacity) + (row - own.x) : 0;
-            norm_rotate<HD>(x, p.q_norm, p.eps, p.cos, p.sin, (int)min(at, (long long)p.cos_rows - 1), c);
-            if (mine) {
-                __half* dst = p.q_out + row * p.ldqo + h * HD + 8 * c;
-                store8(dst, x.a);
-                store8(dst + HD / 2, x.b);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int h = first + (k + u) * RPP;
+                RowHalves x;
+                widen8(raw[u][0], x.a);
+                widen8(raw[u][1], x.b);
+                if (p.q_norm) norm_row<HD>(x, weight, p.eps);
+                if (p.cos) rotate(x, cs);
+                if (mine && k + u < rounds && h < p.n_heads) {
+                    __half* dst = p.q_out + row * p.ldqo + h * HD + 8 * c;
+                    *reinterpret_cast<uint4*>(dst) = narrow8(x.a);
+                    *reinterpret_cast<uint4*>(dst + HD / 2) = narrow8(x.b);
+                }
             }
         }
         return;
     }
-    const int hz = blockIdx.x % (2 * p.kv.n_kv), item = blockIdx.x / (2 * p.kv.n_kv);
+    const int hz = work % (2 * p.kv.n_kv), item = work / (2 * p.kv.n_kv);
     const int h = hz >> 1;
     const bool is_k = (hz & 1) == 0;
-    // sequence b's blocks are items rows / page + 2 b ..: n rows lie in at most (n - 2) / page + 2 pages
-    auto first = [&](int b) { return (rows_from(p.r, b) >> p.kv.page_shift) + 2 * b; };
-    const int b = last_from(p.r.B, item, first);
-    if (item < first(b)) return;       // (rows in front of the first sequence)
-    const int2 own = rows_of(p.r, b);
-    const int start = start_of(p.r, b, p.kv.capacity);
-    const int j = item - first(b) + (start >> p.kv.page_shift);
+    // Item b is the first page of sequence b's rows; n rows lie in at most n / page + 1 more, items B + rows / page + b and on.  (Decoded tokens have
+    // none of these: they come last, and nobody looks for the sequence of the others.)
+    auto more = [&](int b) { return rows.B + (rows_from(rows, b) >> p.kv.page_shift) + b; };
+    const int b = item < rows.B ? item : last_from(rows.B, item, more);
+    const int2 own = rows_of(rows, b);
+    const int start = start_of(rows, b, p.kv.capacity);
+    if (item >= rows.B && item < more(b)) return;       // (rows in front of the first sequence)
+    const int j = (item < rows.B ? 0 : item - more(b) + 1) + (start >> p.kv.page_shift);
     const int at = j << p.kv.page_shift;
     if (own.y == 0 || (long long)at >= (long long)start + own.y) return;
-    const int phys = page_of(p.kv, b, j);
-    if (phys < 0) return;
     const int s0 = max(start - at, 0), s1 = (int)min((long long)start + own.y - at, (long long)p.kv.page);
-    const size_t block = (size_t)phys * p.kv.n_kv + h;
-    unsigned char* codes = (is_k ? p.kv.k : p.kv.v) + block * ((size_t)HD << p.kv.page_shift);
-    float* scale_at = (is_k ? p.kv.k_scale : p.kv.v_scale) + block;
     const __half* src = (is_k ? p.k : p.v) + (long long)(own.x + at - start) * (is_k ? p.ldk : p.ldv) + h * HD + 8 * c;
     const long long ld = is_k ? p.ldk : p.ldv;
-    const float old = *scale_at;
+    const __half* norm = is_k ? p.k_norm : nullptr;
+    const int entry = page_entry(p.kv, b, j);          // (looked at when the rows have been requested too)
+    if (norm) load_weight(norm);
 
-    RowHalves x;
-    auto row_values = [&](int s) {
-        x = RowHalves{};
-        if (s < s1) {
-            load8(src + s * ld, x.a);
-            load8(src + s * ld + HD / 2, x.b);
+    // up to four rows of a lane: s + slot + u RPP.  They are held as they are; norm and rotation are done twice.
+    uint4 raw[kAppendHeld][2];
+    auto load_rows = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < kAppendHeld; ++u) {
+            const int r = s + slot + u * RPP;
+            raw[u][0] = r < s1 ? *reinterpret_cast<const uint4*>(src + r * ld) : make_uint4(0u, 0u, 0u, 0u);
+            raw[u][1] = r < s1 ? *reinterpret_cast<const uint4*>(src + r * ld + HD / 2) : make_uint4(0u, 0u, 0u, 0u);
         }
-        if (is_k) norm_rotate<HD>(x, p.k_norm, p.eps, p.cos, p.sin, s < s1 ? at + s : -1, c);
     };
-    float big = 0.f;
-    for (int s = s0; s < s1; s += RPP) {       // (whole warps stay together for the norm's shuffles)
-        row_values(s + slot);
-        if (s + slot < s1)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float u = fabsf(x.a[i]), w = fabsf(x.b[i]);
-                big = fmaxf(big, u <= FLT_MAX ? u : 0.f);
-                big = fmaxf(big, w <= FLT_MAX ? w : 0.f);
-            }
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+    RowHalves turned = {};                             // the first row's angles
+    auto values = [&](int s, int u) {
+        RowHalves x;
+        widen8(raw[u][0], x.a);
+        widen8(raw[u][1], x.b);
+        if (norm) norm_row<HD>(x, weight, p.eps);        // (whole warps: a row's lanes shuffle)
+        if (is_k && p.cos && s + slot + u * RPP < s1) {
+            RowHalves cs = turned;
+            if (u > 0 || s != s0) load_angles<HD>(cs, p.cos, p.sin, min(at + s + slot + u * RPP, p.cos_rows - 1), c);
+            rotate(x, cs);
+        }
+        return x;
+    };
+    load_rows(s0);
+    if (is_k && p.cos && s0 + slot < s1) load_angles<HD>(turned, p.cos, p.sin, min(at + s0 + slot, p.cos_rows - 1), c);
+    if (!page_there(p.kv, entry)) return;
+    const size_t block = (size_t)entry * p.kv.n_kv + h;
+    unsigned char* codes = (is_k ? p.kv.k : p.kv.v) + block * ((size_t)HD << p.kv.page_shift);
+    float* scale_at = (is_k ? p.kv.k_scale : p.kv.v_scale) + block;
+    const float old = *scale_at;
+    const bool held = s1 - s0 <= kAppendHeld * RPP;
     __shared__ float red[kAppendThreads / 32];
-    if ((tid & 31) == 0) red[tid >> 5] = big;
-    __syncthreads();
+    // largest magnitude of the new values; `finite`: of those that are (not-a-numbers never count)
+    auto largest = [&](bool finite) {
+        float big = 0.f;
+        for (int s = s0; s < s1; s += kAppendHeld * RPP) {
+            if (s > s0 || (finite && !held)) load_rows(s);
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) big = fmaxf(big, red[w]);
+            for (int u = 0; u < kAppendHeld; ++u) {
+                if (s + u * RPP >= s1) break;
+                const RowHalves x = values(s, u);            // (rows that are not there are zero)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = fabsf(x.a[i]), w = fabsf(x.b[i]);
+                    big = fmaxf(big, finite && v > FLT_MAX ? 0.f : v);
+                    big = fmaxf(big, finite && w > FLT_MAX ? 0.f : w);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+        __syncthreads();
+        if ((tid & 31) == 0) red[tid >> 5] = big;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kAppendThreads / 32; ++w) big = fmaxf(big, red[w]);
+        return big;
+    };
+    float big = largest(false);
+    if (big > FLT_MAX) big = largest(true);
     const float need = big / kCodeMax<DT>;
     float scale = need;
     if (s0 > 0 && old > 0.f) {
@@ -182,22 +236,25 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
             scale = ldexpf(old, n);
             const float down = ldexpf(1.f, -n);
             for (int w = tid; w < s0 * (HD / 4); w += kAppendThreads) {
-                uint32_t v = reinterpret_cast<uint32_t*>(codes)[w], o = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o |= to_code<DT>(code_value<DT>((v >> (8 * i)) & 0xffu) * down) << (8 * i);
-                reinterpret_cast<uint32_t*>(codes)[w] = o;
+                const uint32_t v = reinterpret_cast<uint32_t*>(codes)[w];
+                reinterpret_cast<uint32_t*>(codes)[w] = to_codes<DT>(code_value<DT>(v & 0xffu) * down, code_value<DT>(v >> 8 & 0xffu) * down,
+                                                                     code_value<DT>(v >> 16 & 0xffu) * down, code_value<DT>(v >> 24) * down);
             }
         }
     }
     if (tid == 0 && scale != old) *scale_at = scale;
     const float inv = scale > 0.f ? 1.f / scale : 0.f;
-    const bool again = s1 - s0 > RPP;
-    for (int s = s0; s < s1; s += RPP) {
-        if (again) row_values(s + slot);
-        if (s + slot < s1) {
-            unsigned char* dst = codes + (size_t)(s + slot) * HD + 8 * c;
-            *reinterpret_cast<uint2*>(dst) = codes8<DT>(x.a, inv);
-            *reinterpret_cast<uint2*>(dst + HD / 2) = codes8<DT>(x.b, inv);
+    for (int s = s0; s < s1; s += kAppendHeld * RPP) {
+        if (!held) load_rows(s);
+#pragma unroll
+        for (int u = 0; u < kAppendHeld; ++u) {
+            if (s + u * RPP >= s1) break;
+            const RowHalves x = values(s, u);
+            if (s + slot + u * RPP < s1) {
+                unsigned char* dst = codes + (size_t)(s + slot + u * RPP) * HD + 8 * c;
+                *reinterpret_cast<uint2*>(dst) = codes8<DT>(x.a, inv);
+                *reinterpret_cast<uint2*>(dst + HD / 2) = codes8<DT>(x.b, inv);
+            }
         }
     }
 }
@@ -217,11 +274,13 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const ReadPara
     constexpr int LPR = HD / 16, RPP = kReadThreads / LPR;
     const int c = threadIdx.x % LPR;
     const long long i = (long long)blockIdx.x * RPP + threadIdx.x / LPR;
+    __shared__ SharedRows sm_q;
     after_launch_ahead();
+    const PagedRows rows = rows_in_shared(p.r, sm_q);
     if (i >= (long long)p.r.N * p.kv.n_kv) return;
     const int row = (int)(i / p.kv.n_kv), h = (int)(i - (long long)row * p.kv.n_kv);
-    const int b = last_from(p.r.B, row, [&](int b) { return rows_from(p.r, b); });
-    const int2 own = rows_of(p.r, b);
+    const int b = last_from(p.r.B, row, [&](int b) { return rows_from(rows, b); });
+    const int2 own = rows_of(rows, b);
     if (row < own.x || row - own.x >= own.y) return;
     const long long at = (long long)start_of(p.r, b, p.kv.capacity) + (row - own.x);
     const int phys = at < p.kv.capacity ? page_of(p.kv, b, (int)(at >> p.kv.page_shift)) : -1;
@@ -352,18 +411,20 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
     __shared__ ShareStart sm_plan;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const uint32_t ring = smem_addr(sm_rows) + warp * C::RING, scales = smem_addr(sm_rows) + (uint32_t)C::RINGS + warp * S * 8;
+    __shared__ SharedRows sm_q;
     after_launch_ahead();
+    const PagedRows rows = rows_in_shared(p.r, sm_q);
     Pieces<Share> piece;
     if (CLUSTER) {
         const int i = blockIdx.z;
-        piece.x = row_block<Share>(p.kv, p.r, p.group, i, last_from(p.r.B, i, [&](int b) { return first_block<Share>(p.r, p.group, b); }));
+        piece.x = row_block<Share>(p.kv, rows, p.group, i, last_from(p.r.B, i, [&](int b) { return first_block<Share>(rows, p.group, b); }));
         if (piece.x.n_rows == 0) return;        // (all of the cluster)
         piece.h = blockIdx.y;
     } else {
-        piece.template begin<kRowsThreads>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan);
+        piece.template begin<kRowsThreads>(p.kv, rows, p.group, blockIdx.x, gridDim.x, sm_plan);
     }
 
-    for (bool more = true; more && (CLUSTER || piece.next(p.kv, p.r, p.group)); more = !CLUSTER) {
+    for (bool more = true; more && (CLUSTER || piece.next(p.kv, rows, p.group)); more = !CLUSTER) {
         const int b = piece.x.b, r0 = piece.x.r0, n_rows = piece.x.n_rows, start = piece.x.start, h = piece.h, step0 = piece.step0, step1 = piece.step1;
         const int2 own = piece.x.own;
         const int limit_all = min(start + (r0 + n_rows - 1) / p.group, p.kv.capacity - 1);       // the last key that a row sees
@@ -660,6 +721,11 @@ __global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnPara
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
+int sm_count() {
+    int dev = 0, n = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    return n;
+}
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check_cache(const glq_paged_kv_t* kv, const glq_paged_rows_t* r) {
@@ -719,11 +785,13 @@ extern "C" int glq_paged_append(const glq_paged_kv_t* kv, const glq_paged_rows_t
         constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
         AppendParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<const __half*>(k),
                        static_cast<const __half*>(v), static_cast<const __half*>(q_norm), static_cast<const __half*>(k_norm),
-                       static_cast<__half*>(q_out), cos, sin, ldq, ldk, ldv, ldqo, n_heads, 0, cos_rows, eps};
-        const long long items = (long long)rows->rows / kv->page + 2ll * rows->B, per = 2 * (kAppendThreads / (HD / 16));
-        const long long grid = items * 2 * kv->n_kv + (q ? ((long long)rows->rows * n_heads + per - 1) / per : 0);
+                       static_cast<__half*>(q_out), cos, sin, ldq, ldk, ldv, ldqo, n_heads, 0, cos_rows, 1, 1, eps};
+        if (q) p.query_rows = std::max(1, kAppendThreads / (HD / 16) / n_heads);
+        const long long items = (long long)rows->rows / kv->page + 2ll * rows->B;
+        const long long grid = items * 2 * kv->n_kv + (q ? (rows->rows + p.query_rows - 1) / p.query_rows : 0);
         if (items * 2 * kv->n_kv > 0x3fffffffll || grid > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
         p.page_items = (int)items;
+        p.stride = (int)std::max<long long>(1, grid / (items * 2 * kv->n_kv));
         return launch_kernel(true, paged_append_kernel<HD, DT>, dim3((unsigned)grid), dim3(kAppendThreads), 0,
                              reinterpret_cast<cudaStream_t>(stream), p) == cudaSuccess ? GLQ_OK : GLQ_ERR_CUDA;
     });
@@ -771,11 +839,6 @@ template <typename K, typename A> cudaError_t launch_cluster(K* kern, dim3 grid,
     cfg.attrs = attr;
     cfg.numAttrs = pdl_disabled() ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, kern, arg);
-}
-int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
 }
 AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, int n_heads) {
     const long long most = (rows->q_start ? std::min(rows->max_new, rows->rows) : rows->rows / rows->B) * (long long)(n_heads / kv->n_kv);

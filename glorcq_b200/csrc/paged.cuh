@@ -53,6 +53,28 @@ template <class F> __device__ __forceinline__ int last_from(int B, int i, F firs
     }
     return lo;
 }
+// The rows with q_start and start in shared memory, loaded together: last_from's steps take a tenth of the time that they take in global memory.  All
+// threads of the block.
+constexpr int kRowsShared = 512;
+struct SharedRows {
+    long long start[kRowsShared];
+    int q_start[kRowsShared + 1];
+};
+__device__ __forceinline__ PagedRows rows_in_shared(const PagedRows& r, SharedRows& sm) {
+    if (!r.q_start || r.B < 3 || r.B > kRowsShared) return r;
+    for (int i = threadIdx.x; i <= r.B; i += blockDim.x) {
+        const int q = r.q_start[i];
+        const long long s = r.start[(long long)min(i, r.B - 1) * r.start_stride];
+        sm.q_start[i] = q;
+        if (i < r.B) sm.start[i] = s;
+    }
+    __syncthreads();
+    PagedRows x = r;
+    x.q_start = sm.q_start;
+    x.start = sm.start;
+    x.start_stride = 1;
+    return x;
+}
 // physical page of sequence b's logical page j, or -1
 __device__ __forceinline__ int page_of(const PagedKv& kv, int b, int j) {
     if (j >= kv.max_pages) return -1;
@@ -283,7 +305,7 @@ __device__ __forceinline__ float rcp_fast(float x) {
     return y;
 }
 // Blocks of rows of paged_prompt_kernel (paged_prompt.cu): head sizes 64 and 128, many rows a head.
-using PromptShare = ShareOf<256, 128, 2, 1>;
+using PromptShare = ShareOf<256, 128, 4, 8>;
 cudaError_t launch_paged_prompt(int head_dim, int dtype, const AttnParams& p, int grid, cudaStream_t st);
 
 // what weighted values are multiplied by; a row that saw nothing is zero, not-a-number stays
@@ -314,6 +336,22 @@ template <int DT> __device__ __forceinline__ uint32_t to_code(float y) {
     y = y != y ? 0.f : fminf(fmaxf(y, -kCodeMax<DT>), kCodeMax<DT>);
     if (DT == kI8) return (uint32_t)__float2int_rn(y) & 0xffu;
     return (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+}
+// The same for four values.  The conversions have to_code's ends and zeros but for two things: whole numbers end at -128, which the byte-wise maximum
+// mends, and e4m3 keeps not-a-number (0x7f), which is rare.
+template <int DT> __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d) {
+    uint32_t w;
+    if (DT == kI8) {
+        asm("{\n .reg .b32 t;\n cvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n cvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n}\n"
+            : "=r"(w)
+            : "r"(__float2int_rn(a)), "r"(__float2int_rn(b)), "r"(__float2int_rn(c)), "r"(__float2int_rn(d)));
+        return __vmaxs4(w, 0x81818181u);
+    }
+    asm("{\n .reg .b16 l, h;\n cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n mov.b32 %0, {l, h};\n}\n"
+        : "=r"(w)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    if (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) return to_code<DT>(a) | to_code<DT>(b) << 8 | to_code<DT>(c) << 16 | to_code<DT>(d) << 24;
+    return w;
 }
 template <int DT> __device__ __forceinline__ float code_value(uint32_t byte) {
     if (DT == kI8) return (float)(int)(signed char)(unsigned char)byte;

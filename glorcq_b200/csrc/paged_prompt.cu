@@ -218,9 +218,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     }
     if (warp == kPromptMma) tc_alloc(smem_u32(&s_tmem), 512);
     tc_fence_before();
+    __shared__ SharedRows sm_q;
     after_launch_ahead();
+    const PagedRows rows_q = rows_in_shared(p.r, sm_q);
     Pieces<PromptShare> pieces;
-    pieces.template begin<kPromptThreads>(p.kv, p.r, p.group, blockIdx.x, gridDim.x, sm_plan);
+    pieces.template begin<kPromptThreads>(p.kv, rows_q, p.group, blockIdx.x, gridDim.x, sm_plan);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
@@ -575,7 +577,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             // ================= pieces =================
             for (bool more = true; more && ok; ++n_piece) {
                 ok = wait_warp(piece_empty + 8 * (n_piece % kPieceQueue), ((n_piece / kPieceQueue) & 1) ^ 1, dead, 132);
-                more = ok && pieces.next(p.kv, p.r, p.group);
+                more = ok && pieces.next(p.kv, rows_q, p.group);
                 PromptPiece x{};
                 x.most = -1;
                 if (more) {
