@@ -813,8 +813,8 @@ extern "C" int glq_paged_read(const glq_paged_kv_t* kv, const glq_paged_rows_t* 
     });
 }
 
-// How a call runs, from what the host knows.  More than 16 rows a key/value head: 256 of them at once on the 5th-generation tensor cores, head sizes
-// 64 and 128.
+// How a call runs, from what the host knows.  More than 16 rows a key/value head: 256 (128) of them at once on the 5th-generation tensor cores, from
+// 64 channels on.
 enum class AttnKernel { rows8, rows16, prompt };
 struct AttnPlan {
     AttnKernel kernel;
@@ -857,7 +857,8 @@ AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, 
         }
         return a;
     };
-    if (most > 16 && (D == 64 || D == 128)) return make(AttnKernel::prompt, 1, PromptShare{});
+    if (most > 16 && D == 256) return make(AttnKernel::prompt, 1, PromptShape<256>::Share{});
+    if (most > 16 && D >= 64) return make(AttnKernel::prompt, 1, PromptShape<128>::Share{});
     if (most > 8) return make(AttnKernel::rows16, 1, RowsShare<2>{});
     return make(AttnKernel::rows8, D == 256 ? 1 : 2, RowsShare<1>{});
 }
@@ -917,9 +918,9 @@ extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_row
                 return GLQ_ERR_CUDA;
             return join(RowsShare<NB>{});
         };
-        if constexpr (HD == 64 || HD == 128)
+        if constexpr (HD >= 64)
             if (plan.kernel == AttnKernel::prompt)
-                return launch_paged_prompt(HD, DT, p, plan.grid, st) == cudaSuccess ? join(PromptShare{}) : GLQ_ERR_CUDA;
+                return launch_paged_prompt(HD, DT, p, plan.grid, st) == cudaSuccess ? join(typename PromptShape<HD>::Share{}) : GLQ_ERR_CUDA;
         return plan.kernel == AttnKernel::rows8 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
     });
 }

@@ -304,8 +304,12 @@ __device__ __forceinline__ float rcp_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Blocks of rows of paged_prompt_kernel (paged_prompt.cu): head sizes 64 and 128, many rows a head.
-using PromptShare = ShareOf<256, 128, 4, 8>;
+// Blocks of rows of paged_prompt_kernel (paged_prompt.cu): many rows a head.  Two tiles of 128 rows and steps of 128 tokens; with 256 channels one tile and
+// 64 tokens, which is what tensor memory and shared memory hold.
+template <int HD> struct PromptShape {
+    static constexpr int TILES = HD == 256 ? 1 : 2, STEP = HD == 256 ? 64 : 128;
+    using Share = ShareOf<128 * TILES, STEP, 4, 8>;
+};
 cudaError_t launch_paged_prompt(int head_dim, int dtype, const AttnParams& p, int grid, cudaStream_t st);
 
 // what weighted values are multiplied by; a row that saw nothing is zero, not-a-number stays

@@ -1,6 +1,7 @@
 // Attention of many rows a key/value head (pieces of prompts) over the paged 8-bit cache, on tcgen05.
 //
-// Segment: 256 rows (token of the call, head of the group), two tiles of 128, of one (sequence, key/value head); step: 128 tokens.
+// Segment: 256 rows (token of the call, head of the group), two tiles of 128, of one (sequence, key/value head); step: 128 tokens.  (Heads of 256
+// channels: one tile, 64 tokens; the warps of the other tile only give stages back.)
 // A step's products are S = Q K^T (operands in shared memory) and O += P V (P in tensor memory, over the scores that it is made of; V as it
 // lies, tokens by channels, which is the MN-major form of the operand).  Tensor memory: S of both tiles, O of both tiles.
 //
@@ -42,11 +43,14 @@ constexpr int kRegsSoftmax = 168, kRegsProducer = 104, kRegsMma = 72;
 static_assert((kPromptSoftmax * kRegsSoftmax + kPromptProducers * kRegsProducer + 4 * kRegsMma) * 32 <= kPromptThreads * 128, "registers");
 // every so many pairs of exponentials one is taken by exp2_poly
 constexpr int kPolyEvery = 4;
-constexpr int kStepTokens = PromptShare::STEP, kGroups = kStepTokens / 16;
 
+// Operands: [64-channel block][rows][128 B], 16-byte piece c of row r at c ^ (r & 7).
 template <int HD> struct PromptCfg {
-    static constexpr int TILE = 128 * HD * 2;            // an operand: [64-channel block][128 rows][128 B], 16-byte piece c of row r at c ^ (r & 7)
-    static constexpr size_t SMEM = 6 * TILE + 1024;      // Q of two tiles, K and V of two stages
+    using Share = typename PromptShape<HD>::Share;
+    static constexpr int TILES = PromptShape<HD>::TILES, STEP = Share::STEP, GROUPS = STEP / 16;
+    static constexpr int Q_BLOCK = 128 * 128, KV_BLOCK = STEP * 128, BLOCKS = HD / 64;
+    static constexpr int Q_TILE = BLOCKS * Q_BLOCK, KV_TILE = BLOCKS * KV_BLOCK;
+    static constexpr size_t SMEM = TILES * Q_TILE + 4 * KV_TILE + 1024;       // K and V of two stages
     static constexpr uint32_t S_COL = 0, O_COL = 256;
 };
 
@@ -97,9 +101,9 @@ __device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint
         "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-// MN-major operand, 128-byte swizzle: 64-channel blocks 128 rows apart, groups of 8 tokens 1024 B apart
-__device__ __forceinline__ uint64_t value_desc(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+// MN-major operand, 128-byte swizzle: 64-channel blocks `block` bytes apart, groups of 8 tokens 1024 B apart
+__device__ __forceinline__ uint64_t value_desc(uint32_t saddr, int block) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
            ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
@@ -180,6 +184,8 @@ constexpr int kPieceQueue = 4, kPieceReaders = kPromptSoftmax + kPromptProducers
 template <int HD, int DT>
 __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const AttnParams p) {
     using C = PromptCfg<HD>;
+    using Share = typename C::Share;
+    constexpr int kStepTokens = C::STEP, kGroups = C::GROUPS;
     extern __shared__ unsigned char prompt_smem[];
     __shared__ __align__(8) unsigned long long bars[2 * 11 + 2 * kPieceQueue];
     __shared__ PromptPiece s_piece[kPieceQueue];
@@ -189,7 +195,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     __shared__ int s_dead;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(prompt_smem) + 1023u) & ~1023u;
-    const uint32_t q_smem = base, k_smem = base + 2 * C::TILE, v_smem = base + 4 * C::TILE;
+    const uint32_t q_smem = base, k_smem = base + C::TILES * C::Q_TILE, v_smem = k_smem + 2 * C::KV_TILE;
     // [0], [1] of each: stages or tiles
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48, s_full = k_full + 64,
                    p_ready = k_full + 80, pv_done = k_full + 96, q_ready = k_full + 112, o_free = k_full + 128, q_free = k_full + 144,
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     __shared__ SharedRows sm_q;
     after_launch_ahead();
     const PagedRows rows_q = rows_in_shared(p.r, sm_q);
-    Pieces<PromptShare> pieces;
+    Pieces<Share> pieces;
     pieces.template begin<kPromptThreads>(p.kv, rows_q, p.group, blockIdx.x, gridDim.x, sm_plan);
     __syncthreads();
     tc_fence_after();
@@ -279,9 +285,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 tmem_ld32(s_tm, v[0]);
                 float top = -INFINITY;
 #pragma unroll 2
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < kStepTokens / 32; ++c) {
                     tmem_arrived(v[c & 1]);
-                    tmem_ld32(s_tm + 32 * ((c + 1) & 3), v[(c + 1) & 1]);         // (and the first ones again)
+                    tmem_ld32(s_tm + 32 * ((c + 1) % (kStepTokens / 32)), v[(c + 1) & 1]);         // (and the first ones again)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const uint32_t* u = v[c & 1] + 16 * half;
@@ -308,12 +314,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                         }
                 }
 #pragma unroll 1
-                for (int c2 = 0; c2 < 4; c2 += 2) {
+                for (int c2 = 0; c2 < kStepTokens / 32; c2 += 2) {
                     uint32_t w[32];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         tmem_arrived(v[c]);
-                        if (c2 + c < 3) tmem_ld32(s_tm + 32 * (c2 + c + 1), v[c ^ 1]);
+                        if (c2 + c < kStepTokens / 32 - 1) tmem_ld32(s_tm + 32 * (c2 + c + 1), v[c ^ 1]);
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const uint32_t* u = v[c] + 16 * half;
@@ -357,12 +363,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             if (!ok) break;
             tc_fence_after();
             if (m <= -1e30f) l = 0.f;         // nothing seen: the sum is of exp2_poly's smallest numbers
-            if (piece->rows > 128 * tile) {
+            if (tile < C::TILES && piece->rows > 128 * tile) {
                 const bool whole = piece->whole;
                 const float f = result_factor(l, kCodeUnit<DT>);
                 const int r = first_row + (live ? row : 0), token = r / p.group;
                 __half* out = p.out + (long long)(piece->row + token) * p.ldo + (piece->h * p.group + r - token * p.group) * HD;
-                float* part = partial_of<PromptShare, HD>(p.partial, blockIdx.x, piece->step0 == 0);
+                float* part = partial_of<Share, HD>(p.partial, blockIdx.x, piece->step0 == 0);
                 float* mine = part + (128 * tile + row) * HD;
 #pragma unroll 1
                 for (int c = 0; c < HD / 16; ++c) {
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                         for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(mine + 16 * c)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                     }
                 }
-                if (live && !whole) *reinterpret_cast<float2*>(part + PromptShare::R * HD + 2 * (128 * tile + row)) = make_float2(m, l);
+                if (live && !whole) *reinterpret_cast<float2*>(part + Share::R * HD + 2 * (128 * tile + row)) = make_float2(m, l);
             }
             tc_fence_before();
             if (steps > 0) arrive_warp(o_free + 8 * tile, lane);
@@ -395,19 +401,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     } else if (warp < kPromptMma) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsProducer));
         // ================= codes to operands =================
-        constexpr int U = HD / 32, BLOCKS = HD / 64;        // 16-byte pieces of a lane, 64-channel blocks
-        const int group0 = 2 * (warp - kPromptSoftmax);
+        constexpr int G = kGroups / kPromptProducers, U = HD / 32, BLOCKS = C::BLOCKS;        // groups of a warp, 16-byte pieces of a lane in each
+        const int group0 = G * (warp - kPromptSoftmax);
         // Piece u of lane: row lane / 4 + 8 (u / BLOCKS) of a group, piece lane % 4 of block u % BLOCKS; its halves become pieces 2c and 2c + 1 of 8 in the
         // operand's row.  Eight lanes then meet 32 banks: two rows, one even and one odd.
         const int r0 = lane >> 2, c0 = lane & 3;
         const uint32_t even = (16 * group0 + r0) * 128 + (((2 * c0) ^ (r0 & 7)) << 4), odd = (16 * group0 + r0) * 128 + (((2 * c0 + 1) ^ (r0 & 7)) << 4);
-        uint4 kc[2][U], vc[2][U];
-        float ks[2], vs[2];
-        int phys[2], phys1[2], phys2[2], h = 0;       // entries of the page table: of this step, the next and the one behind that (looked at when used)
+        uint4 kc[G][U], vc[G][U];
+        float ks[G], vs[G];
+        int phys[G], phys1[G], phys2[G], h = 0;       // entries of the page table: of this step, the next and the one behind that (looked at when used)
         uint32_t had = 0;                 // bit t: parity of the pieces that tile t had steps in
-        auto request = [&](const unsigned char* pages, const float* scales, int step, const int (&phys)[2], uint4 (&c)[2][U], float (&s)[2]) {
+        auto request = [&](const unsigned char* pages, const float* scales, int step, const int (&phys)[G], uint4 (&c)[G][U], float (&s)[G]) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < G; ++k) {
                 s[k] = 0.f;
                 if (!page_there(p.kv, phys[k])) {           // zeros
 #pragma unroll
@@ -421,9 +427,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 }
             }
         };
-        auto store = [&](uint32_t tile, const uint4 (&c)[2][U]) {
+        auto store = [&](uint32_t tile, const uint4 (&c)[G][U]) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int k = 0; k < G; ++k)
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     uint32_t h[8];
@@ -431,7 +437,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                     codes_to_half<DT>(c[k][u].y, h[2], h[3]);
                     codes_to_half<DT>(c[k][u].z, h[4], h[5]);
                     codes_to_half<DT>(c[k][u].w, h[6], h[7]);
-                    const uint32_t at = tile + 2048 * k + (u / BLOCKS) * 1024 + (u % BLOCKS) * 16384;
+                    const uint32_t at = tile + 2048 * k + (u / BLOCKS) * 1024 + (u % BLOCKS) * C::KV_BLOCK;
                     sts128(at + even, h[0], h[1], h[2], h[3]);
                     sts128(at + odd, h[4], h[5], h[6], h[7]);
                 }
@@ -439,9 +445,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         while (next_piece()) {
             const int steps = piece->most, step0 = piece->step0, b = piece->b;
             h = piece->h;
-            auto lookup = [&](int j, int (&to)[2]) {
+            auto lookup = [&](int j, int (&to)[G]) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k) to[k] = j < steps ? page_entry(p.kv, b, ((step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
+                for (int k = 0; k < G; ++k) to[k] = j < steps ? page_entry(p.kv, b, ((step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
             };
             lookup(0, phys);
             lookup(1, phys1);
@@ -451,10 +457,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 const uint32_t g = gs + j, stage = g & 1, parity = ((g >> 1) & 1) ^ 1;
                 lookup(j + 2, phys2);
                 if (!(ok = wait_warp(k_empty + 8 * stage, parity, dead, 123))) break;
-                store(k_smem + stage * C::TILE, kc);
+                store(k_smem + stage * C::KV_TILE, kc);
                 fence_async_smem();
                 arrive_warp(k_full + 8 * stage, lane);
-                const float ks0[2] = {ks[0], ks[1]};
+                float ks0[G];
+#pragma unroll
+                for (int k = 0; k < G; ++k) ks0[k] = ks[k];
                 request(p.kv.k, p.kv.k_scale, step0 + j + 1, phys1, kc, ks);
                 if (j == 0) {           // the tiles' rows, a quarter a warp
                     constexpr int LPR = HD / 8, RPP = 32 / LPR;          // lanes of a row, rows of a pass
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
 #pragma unroll 2
                         for (int i = 0; i < 32 / RPP; ++i) {
                             const int row = row0 + i * RPP;
-                            copy_async_16(q_smem + tile * C::TILE + row * 128 + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4),
+                            copy_async_16(q_smem + tile * C::Q_TILE + row * 128 + (c >> 3) * C::Q_BLOCK + (((c & 7) ^ (row & 7)) << 4),
                                           from + (row < rows ? (long long)token * p.ldq + head * HD : 0ll), row < rows);
                             token += more_tokens;
                             head += more_heads;
@@ -487,23 +495,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 }
                 if (!(ok = wait_warp(v_empty + 8 * stage, parity, dead, 124))) break;
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < G; ++k)
                     if (!(vs[k] > 0.f))           // a block without a scale: its values are zero whatever its codes
 #pragma unroll
                         for (int u = 0; u < U; ++u) vc[k][u] = make_uint4(0u, 0u, 0u, 0u);
-                store(v_smem + stage * C::TILE, vc);
-                if (lane < 2) {
-                    const float k1 = lane ? ks0[1] : ks0[0], v1 = lane ? vs[1] : vs[0];
-                    const bool there = page_there(p.kv, lane ? phys[1] : phys[0]);
-                    // (a factor above zero: -3e38 times it hides a key)
-                    s_scale[stage][group0 + lane] = make_float4(fmaxf(k1 * p.scale2, 1e-30f), !there ? -INFINITY : v1 > 0.f ? log2_fast(v1) : 0.f,
-                                                                v1 > 0.f ? rcp_fast(v1) : 1.f, 0.f);
-                }
+                store(v_smem + stage * C::KV_TILE, vc);
+#pragma unroll
+                for (int k = 0; k < G; ++k)
+                    if (lane == k)         // (a factor above zero: -3e38 times it hides a key)
+                        s_scale[stage][group0 + k] = make_float4(fmaxf(ks0[k] * p.scale2, 1e-30f), !page_there(p.kv, phys[k]) ? -INFINITY : vs[k] > 0.f ? log2_fast(vs[k]) : 0.f,
+                                                                 vs[k] > 0.f ? rcp_fast(vs[k]) : 1.f, 0.f);
                 fence_async_smem();
                 arrive_warp(v_full + 8 * stage, lane);
                 request(p.kv.v, p.kv.v_scale, step0 + j + 1, phys1, vc, vs);
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < G; ++k) {
                     phys[k] = phys1[k];
                     phys1[k] = phys2[k];
                 }
@@ -516,14 +522,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
         if (warp < kPromptMma + 2) {
             // ================= MMA issue =================
-            constexpr uint32_t s_desc = tc_idesc(128), o_desc = tc_idesc(HD) | (1u << 16);       // V: MN-major
+            constexpr uint32_t s_desc = tc_idesc(kStepTokens), o_desc = tc_idesc(HD) | (1u << 16);       // V: MN-major
             const int tile = warp - kPromptMma;
             const uint32_t s_at = tmem + C::S_COL + tile * 128, o_at = tmem + C::O_COL + tile * HD, bar = 8 * tile;
-            const uint64_t q_at = tc_smem_desc(q_smem + tile * C::TILE), k_at = tc_smem_desc(k_smem), v_at = value_desc(v_smem);
+            const uint64_t q_at = tc_smem_desc(q_smem + tile * C::Q_TILE), k_at = tc_smem_desc(k_smem), v_at = value_desc(v_smem, C::KV_BLOCK);
             auto scores = [&](uint32_t stage) {
-                const uint64_t k = k_at + stage * (C::TILE >> 4);
-                mma4_ss(s_at, q_at, k, s_desc, 0);
-                if (HD == 128) mma4_ss(s_at, q_at + (16384 >> 4), k + (16384 >> 4), s_desc, 1);
+                const uint64_t k = k_at + stage * (C::KV_TILE >> 4);
+#pragma unroll
+                for (int blk = 0; blk < C::BLOCKS; ++blk) mma4_ss(s_at, q_at + blk * (C::Q_BLOCK >> 4), k + blk * (C::KV_BLOCK >> 4), s_desc, blk > 0);
                 commit_warp(s_full + bar);
             };
             uint32_t done = 0, had = 0;           // steps, pieces that the tile had steps in
@@ -542,11 +548,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                          (j + 1 == n || wait_warp(k_full + 8 * (stage ^ 1), ((g + 1) >> 1) & 1, dead, 126)) && wait_warp(p_half + bar, done & 1, dead, 127);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t v = v_at + stage * (C::TILE >> 4);
+                    const uint64_t v = v_at + stage * (C::KV_TILE >> 4);
                     mma4_ts(o_at, s_at, v, o_desc, j > 0);
                     if (!(ok = wait_warp(p_ready + bar, done & 1, dead, 129))) break;
                     tc_fence_after();
-                    mma4_ts(o_at, s_at + 32, v + (8192 >> 4), o_desc, 1);
+                    if (kStepTokens == 128) mma4_ts(o_at, s_at + 32, v + (8192 >> 4), o_desc, 1);
                     commit_warp(pv_done + bar);
                     if (lane == 0) {
                         mbar_arrive(k_empty + 8 * stage);
@@ -590,7 +596,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                     x.step0 = pieces.step0;
                     x.whole = pieces.whole();
                     for (int tile = 0; tile < 2; ++tile) {
-                        const int rows = min(x.rows - 128 * tile, 128);
+                        const int rows = tile < C::TILES ? min(x.rows - 128 * tile, 128) : 0;
                         const int last = min(x.start + (x.r0 + 128 * tile + rows - 1) / p.group, p.kv.capacity - 1);
                         x.steps[tile] = rows > 0 ? max(0, min(pieces.step1, last / kStepTokens + 1) - x.step0) : 0;
                     }
@@ -599,7 +605,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 if (lane == 0 && ok) s_piece[n_piece % kPieceQueue] = x;
                 arrive_warp(piece_full + 8 * (n_piece % kPieceQueue), lane);
             }
-            if (lane == 0) p.join[blockIdx.x] = join_item<PromptShare>(pieces.total, gridDim.x, blockIdx.x, sm_plan);
+            if (lane == 0) p.join[blockIdx.x] = join_item<Share>(pieces.total, gridDim.x, blockIdx.x, sm_plan);
         }
     }
     __syncthreads();
@@ -619,6 +625,7 @@ template <int HD, int DT> cudaError_t launch_prompt(const AttnParams& p, int gri
 }  // namespace
 
 cudaError_t launch_paged_prompt(int head_dim, int dtype, const AttnParams& p, int grid, cudaStream_t st) {
+    if (head_dim == 256) return dtype == kI8 ? launch_prompt<256, kI8>(p, grid, st) : launch_prompt<256, kE4M3>(p, grid, st);
     if (head_dim == 64) return dtype == kI8 ? launch_prompt<64, kI8>(p, grid, st) : launch_prompt<64, kE4M3>(p, grid, st);
     return dtype == kI8 ? launch_prompt<128, kI8>(p, grid, st) : launch_prompt<128, kE4M3>(p, grid, st);
 }
