@@ -813,8 +813,7 @@ extern "C" int glq_paged_read(const glq_paged_kv_t* kv, const glq_paged_rows_t* 
     });
 }
 
-// How a call runs, from what the host knows.  More than 16 rows a key/value head: 256 (128) of them at once on the 5th-generation tensor cores, from
-// 64 channels on.
+// How a call runs, from what the host knows: the lengths are on the device, what it has is the room of the table.
 enum class AttnKernel { rows8, rows16, prompt };
 struct AttnPlan {
     AttnKernel kernel;
@@ -857,8 +856,14 @@ AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, 
         }
         return a;
     };
-    if (most > 16 && D == 256) return make(AttnKernel::prompt, 1, PromptShape<256>::Share{});
-    if (most > 16 && D >= 64) return make(AttnKernel::prompt, 1, PromptShape<128>::Share{});
+    // From 64 channels on, 256 (128) rows of a head at once on the 5th-generation tensor cores, where that is much work: those tiles multiply four times
+    // as fast, but a call begins and joins slower, and a tile that is not full costs as much as a full one.  Measured (graph, us, tiles of 16 / prompt
+    // kernel; 128 channels, 8 heads, 4 rows of q a token): 16 tokens after 1000 8.9 / 30, 64 after 4000 39 / 45, 128 after 1000 27 / 45 and after 4000
+    // 64 / 46, 256 after none 28 / 31 and after 4000 117 / 50, 512 after 4000 222 / 73; 16 sequences of 32 tokens, 16 heads of their own (32 rows), after
+    // 1000 55 / 63 and after 4000 119 / 150, of 64 tokens 98 / 64 and 220 / 151.
+    const long long every = most * rows->B * kv->n_kv;
+    if (D >= 64 && most > 32 && (every > 4096 || every * D > (1ll << 31) / ((long long)kv->max_pages * kv->page)))
+        return D == 256 ? make(AttnKernel::prompt, 1, PromptShape<256>::Share{}) : make(AttnKernel::prompt, 1, PromptShape<128>::Share{});
     if (most > 8) return make(AttnKernel::rows16, 1, RowsShare<2>{});
     return make(AttnKernel::rows8, D == 256 ? 1 : 2, RowsShare<1>{});
 }

@@ -71,8 +71,11 @@ def test_attention_of_a_decoded_token(dev, dtype, heads, kv, D, P, held):
     assert torch.equal(got, paged_attention(q, *long, i64(held, dev)))
 
 
+MUCH = 1 << 22              # tokens of room at which more than 32 rows a head go to the kernel of prompts, however few
+
+
 def wide(cache, tokens):
-    """The cache with a table of that many tokens a sequence, the new places empty."""
+    """The cache with a table of that many tokens a sequence, the new places empty: kernels are chosen by its room."""
     table = torch.full((cache[4].shape[0], tokens // cache[0].shape[2] + 1), -1, dtype=torch.int32, device=cache[4].device)
     table[:, : cache[4].shape[1]] = cache[4]
     return [*cache[:4], table]
@@ -95,22 +98,24 @@ def test_attention_of_several_tokens(dev, dtype, heads, kv, D, P, held, new):
     assert torch.equal(got, paged_attention(q, *cache, i64(held, dev), q_starts(new, dev), max_new=max(new)))
     # the most rows of a sequence not told: perhaps another kernel
     check_attention(paged_attention(q, *cache, i64(held, dev), q_starts(new, dev)), cache, held, new, q)
-    check_attention(paged_attention(q, *wide(cache, 40000), i64(held, dev), q_starts(new, dev), max_new=max(new)), cache, held, new, q)
+    for room in (40000, MUCH):
+        check_attention(paged_attention(q, *wide(cache, room), i64(held, dev), q_starts(new, dev), max_new=max(new)), cache, held, new, q)
     if len(set(new)) == 1:
         assert torch.equal(got, paged_attention(q, *cache, i64(held, dev)))
 
 
-@pytest.mark.parametrize("heads,D,new", [(4, 128, 1), (2, 128, 150), (4, 64, 1), (4, 64, 70), (2, 256, 1), (2, 256, 30)])
+@pytest.mark.parametrize("heads,D,new", [(4, 128, 1), (2, 128, 150), (4, 64, 1), (4, 64, 70), (2, 256, 1), (2, 256, 30), (2, 256, 50)])
 def test_rows_of_no_sequence_are_left_as_they_were(dev, heads, D, new):
     from glorcq_b200.paged_cache import paged_attention
     held, counts = [20, 0, 35], [new, 0, max(1, new // 2)]
     cache = make_cache(5, "int8", 2, D, 16, [a + n for a, n in zip(held, counts)], dev)
     n = 3 + sum(counts) + 5
     q = torch.randn(n, heads, D, generator=torch.Generator().manual_seed(1)).half().to(dev)
-    out = torch.full((n, heads, D), 7.0, dtype=torch.float16, device=dev)
-    paged_attention(q, *cache, i64(held, dev), q_starts(counts, dev, at=3), max_new=new, out=out)
-    assert (out[:3] == 7).all() and (out[3 + sum(counts):] == 7).all()
-    check_attention(out, cache, held, counts, q, rows=[3, 3 + new, 3 + new])
+    for c in (cache, wide(cache, MUCH)):
+        out = torch.full((n, heads, D), 7.0, dtype=torch.float16, device=dev)
+        paged_attention(q, *c, i64(held, dev), q_starts(counts, dev, at=3), max_new=new, out=out)
+        assert (out[:3] == 7).all() and (out[3 + sum(counts):] == 7).all()
+        check_attention(out, cache, held, counts, q, rows=[3, 3 + new, 3 + new])
 
 
 @pytest.mark.parametrize("D,new", [(128, 1), (128, 140), (64, 40), (32, 1)])
@@ -123,12 +128,13 @@ def test_pages_that_are_not_there_are_hidden(dev, D, new):
     table[1, 0] = cache[0].shape[0]                   # the first
     table[2] = -1                                     # all of them: nothing to see
     q = torch.randn(3 * new, 4, D, generator=torch.Generator().manual_seed(1)).half().to(dev)
-    got = paged_attention(q, *cache, i64(held, dev))
-    assert not got[2 * new:].any()
-    check_attention(got, cache, held, [new] * 3, q)
+    for c in (cache, wide(cache, MUCH)):
+        got = paged_attention(q, *c, i64(held, dev))
+        assert not got[2 * new:].any()
+        check_attention(got, cache, held, [new] * 3, q)
 
 
-@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("new", [1, 50, 1100])
 def test_positions_outside_the_table(dev, new):
     """A length below zero counts as none, one behind the table as the table's: such rows see all that is."""
     from glorcq_b200.paged_cache import paged_append, paged_attention
@@ -152,9 +158,11 @@ def test_attention_takes_rows_of_any_distance_and_its_scale(dev, new):
     cache = make_cache(9, "int8", 2, 128, 32, [40 + new, 7 + new], dev)
     both = torch.randn(2 * new, 12, 128, generator=torch.Generator().manual_seed(4)).half().to(dev)
     q, out = both[:, 4:8], torch.zeros(2 * new, 9, 128, dtype=torch.float16, device=dev)
-    paged_attention(q, *cache, i64([40, 7], dev), scale=0.21, out=out[:, 2:6])
-    check_attention(out[:, 2:6], cache, [40, 7], [new] * 2, q, scale=0.21)
-    assert not out[:, :2].any() and not out[:, 6:].any()
+    for c in (cache, wide(cache, MUCH)):
+        out[:, 2:6] = 1
+        paged_attention(q, *c, i64([40, 7], dev), scale=0.21, out=out[:, 2:6])
+        check_attention(out[:, 2:6], cache, [40, 7], [new] * 2, q, scale=0.21)
+        assert not out[:, :2].any() and not out[:, 6:].any()
 
 
 @pytest.mark.parametrize("new", [1, 33])
@@ -169,14 +177,17 @@ def test_scales_of_any_size(dev, new):
         t[table[3]] = 0.0
         cache[i].view(torch.uint8)[table[3]] = 0
     q = torch.randn(new, 4, 64, generator=torch.Generator().manual_seed(4)).half().to(dev)
-    got = paged_attention(q, *cache, i64([96], dev))
-    check_attention(got, cache, [96], [new], q)
+    for c in (cache, wide(cache, MUCH)):
+        check_attention(paged_attention(q, *c, i64([96], dev)), cache, [96], [new], q)
 
 
+@pytest.mark.parametrize("room", [0, 40000, MUCH])
 @pytest.mark.parametrize("new", [1, 20])
-def test_not_a_number_in_a_query_stays_in_its_row(dev, new):
+def test_not_a_number_in_a_query_stays_in_its_row(dev, new, room):
     from glorcq_b200.paged_cache import paged_attention
     cache = make_cache(11, "e4m3", 2, 128, 32, [70 + new] * 2, dev)
+    if room:
+        cache = wide(cache, room)
     q = torch.randn(2 * new, 4, 128, generator=torch.Generator().manual_seed(4)).half().to(dev)
     want = paged_attention(q, *cache, i64([70], dev))
     q[0, 1, 5] = float("nan")
@@ -200,6 +211,8 @@ def test_pages_behind_two_gigabytes_and_shared_ones(dev, new):
     small[4][1, :2] = small[4][0, :2]
     cache.append(torch.where(small[4] >= 0, small[4] + pool - 8, small[4]).to(torch.int32))
     q = torch.randn(2 * new, 16, D, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    for room in (40000, MUCH):
+        assert torch.equal(paged_attention(q, *wide(cache, room), i64([300], dev)), paged_attention(q, *wide(small, room), i64([300], dev)))
     got = paged_attention(q, *cache, i64([300], dev))
     assert torch.equal(got, paged_attention(q, *small, i64([300], dev)))
     check_attention(got[:, :1], [t[:, :1] if t.dim() > 2 or t.shape[1] == kv else t for t in small], [300, 300], [new] * 2, q[:, :1])
@@ -424,13 +437,13 @@ def step(cache, q, k, v, cos, sin, start):
     return paged_attention(paged_append(q, k, v, cos, sin, *cache, start), *cache, start)
 
 
-@pytest.mark.parametrize("new", [1, 30])
-def test_captured_calls_follow_lengths_and_pages(dev, new):
+@pytest.mark.parametrize("new,width", [(1, 32), (30, 32), (30, 2500)])
+def test_captured_calls_follow_lengths_and_pages(dev, new, width):
     """Two graphs over one cache replayed on two streams, lengths and table changed in between: as eager calls, also while those run
     on a third stream."""
-    cache = make_cache(1, "e4m3", 2, 128, 16, [400, 300], dev, width=32, pool=70)
+    cache = make_cache(1, "e4m3", 2, 128, 16, [400, 300], dev, width=width, pool=70)
     spare = [p for p in range(70) if p not in sum(cache[4].tolist(), [])]
-    cos, sin = tables(128, 512, dev)
+    cos, sin = tables(128, 16 * width, dev)
     q, k, v = rows_for([new, new], 8, 2, 128, dev)
     for j, b in ((25, 0), (26, 0), (27, 0), (19, 1), (20, 1), (21, 1)):
         cache[4][b, j] = spare.pop()
