@@ -165,6 +165,29 @@ __device__ __forceinline__ void exp2_poly(unsigned long long x, float& a, float&
     a = __int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23));
     b = __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23));
 }
+// A 4 by 4 transposition among four lanes: x[s] becomes piece lane % 4 of lane s's row, so that four lanes write one row's 64 bytes beside one another
+// (each lane writing its own row: 32 lines a store, and the results of both tiles took 6500 cycles, partial ones 11500, against 3800 and 5500).
+__device__ __forceinline__ void quad_transpose(uint4 (&x)[4], int lane) {
+    auto swap = [&](uint4& a, uint4& b, int bit) {        // the lane without the bit keeps a
+        const bool up = lane & bit;
+        uint4 send = up ? a : b;
+        send.x = __shfl_xor_sync(0xffffffffu, send.x, bit);
+        send.y = __shfl_xor_sync(0xffffffffu, send.y, bit);
+        send.z = __shfl_xor_sync(0xffffffffu, send.z, bit);
+        send.w = __shfl_xor_sync(0xffffffffu, send.w, bit);
+        (up ? a : b) = send;
+    };
+    swap(x[0], x[1], 1);
+    swap(x[2], x[3], 1);
+    swap(x[0], x[2], 2);
+    swap(x[1], x[3], 2);
+}
+// has the phase ended?  (a look, no wait)
+__device__ __forceinline__ bool test_warp(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return __all_sync(0xffffffffu, done != 0);
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -366,29 +389,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             if (tile < C::TILES && piece->rows > 128 * tile) {
                 const bool whole = piece->whole;
                 const float f = result_factor(l, kCodeUnit<DT>);
-                const int r = first_row + (live ? row : 0), token = r / p.group;
-                __half* out = p.out + (long long)(piece->row + token) * p.ldo + (piece->h * p.group + r - token * p.group) * HD;
+                const int row4 = row & ~3, n_rows = piece->rows - 128 * tile;          // the first of the four rows of a lane and its neighbours
+                __half* out[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = first_row + min(row4 + i, n_rows - 1), token = r / p.group;
+                    out[i] = p.out + (long long)(piece->row + token) * p.ldo + (piece->h * p.group + r - token * p.group) * HD + 8 * (lane & 3);
+                }
                 float* part = partial_of<Share, HD>(p.partial, blockIdx.x, piece->step0 == 0);
-                float* mine = part + (128 * tile + row) * HD;
+                float* mine = part + (128 * tile + row4) * HD + 4 * (lane & 3);
 #pragma unroll 1
-                for (int c = 0; c < HD / 16; ++c) {
-                    uint32_t v[16];
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t v[32];
                     if (steps > 0) {
-                        tc_ld16(o_tm + 16 * c, v);
+                        tmem_ld32(o_tm + 32 * c, v);
                         tmem_arrived(v);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = 0u;
+                        for (int i = 0; i < 32; ++i) v[i] = 0u;
                     }
-                    if (live && whole) {
-                        uint32_t o[8];
+                    uint4 x[4];
+                    if (whole) {
+                        uint32_t o[16];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) o[i] = pack_half2(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f);
-                        *reinterpret_cast<uint4*>(out + 16 * c) = make_uint4(o[0], o[1], o[2], o[3]);
-                        *reinterpret_cast<uint4*>(out + 16 * c + 8) = make_uint4(o[4], o[5], o[6], o[7]);
-                    } else if (live) {
+                        for (int i = 0; i < 16; ++i) o[i] = pack_half2(__uint_as_float(v[2 * i]) * f, __uint_as_float(v[2 * i + 1]) * f);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(mine + 16 * c)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                        for (int i = 0; i < 4; ++i) x[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        quad_transpose(x, lane);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (row4 + i < n_rows) *reinterpret_cast<uint4*>(out[i] + 32 * c) = x[i];
+                    } else {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) x[i] = make_uint4(v[16 * half + 4 * i], v[16 * half + 4 * i + 1], v[16 * half + 4 * i + 2], v[16 * half + 4 * i + 3]);
+                            quad_transpose(x, lane);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (row4 + i < n_rows) *reinterpret_cast<uint4*>(mine + i * HD + 32 * c + 16 * half) = x[i];
+                        }
                     }
                 }
                 if (live && !whole) *reinterpret_cast<float2*>(part + Share::R * HD + 2 * (128 * tile + row)) = make_float2(m, l);
@@ -449,8 +489,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
 #pragma unroll
                 for (int k = 0; k < G; ++k) to[k] = j < steps ? page_entry(p.kv, b, ((step0 + j) * kStepTokens + 16 * (group0 + k)) >> p.kv.page_shift) : -1;
             };
+            // The tiles' rows, a quarter a warp: where a place is free already, ahead of the first keys.
+            constexpr int LPR = HD / 8, RPP = 32 / LPR;          // lanes of a row, rows of a pass
+            const int c = lane % LPR, row0 = (warp - kPromptSoftmax) * 32 + lane / LPR;
+            const int more_tokens = RPP / p.group, more_heads = RPP - more_tokens * p.group;
+            const __half* from = p.q + (long long)piece->row * p.ldq + h * p.group * HD + 8 * c;
+            uint32_t rows_missing = (piece->steps[0] > 0) | (piece->steps[1] > 0) << 1, rows_coming = 0;
+            auto copy_rows = [&](int tile) {
+                had ^= 1u << tile;
+                rows_missing ^= 1u << tile;
+                rows_coming |= 1u << tile;
+                int token = (piece->r0 + 128 * tile + row0) / p.group, head = piece->r0 + 128 * tile + row0 - token * p.group;
+                const int rows = piece->rows - 128 * tile;
+#pragma unroll 2
+                for (int i = 0; i < 32 / RPP; ++i) {
+                    const int row = row0 + i * RPP;
+                    copy_async_16(q_smem + tile * C::Q_TILE + row * 128 + (c >> 3) * C::Q_BLOCK + (((c & 7) ^ (row & 7)) << 4),
+                                  from + (row < rows ? (long long)token * p.ldq + head * HD : 0ll), row < rows);
+                    token += more_tokens;
+                    head += more_heads;
+                    if (head >= p.group) {
+                        head -= p.group;
+                        ++token;
+                    }
+                }
+            };
+            auto rows_there = [&]() {
+                if (!rows_coming) return;
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem();
+                for (int tile = 0; tile < 2; ++tile)
+                    if (rows_coming >> tile & 1) arrive_warp(q_ready + 8 * tile, lane);
+                rows_coming = 0;
+            };
             lookup(0, phys);
             lookup(1, phys1);
+#pragma unroll 1
+            for (int tile = 0; tile < 2; ++tile)
+                if ((rows_missing >> tile & 1) && test_warp(q_free + 8 * tile, ((had >> tile) & 1) ^ 1)) copy_rows(tile);
             request(p.kv.k, p.kv.k_scale, step0, phys, kc, ks);
             request(p.kv.v, p.kv.v_scale, step0, phys, vc, vs);
             for (int j = 0; j < steps; ++j) {
@@ -464,34 +540,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
 #pragma unroll
                 for (int k = 0; k < G; ++k) ks0[k] = ks[k];
                 request(p.kv.k, p.kv.k_scale, step0 + j + 1, phys1, kc, ks);
-                if (j == 0) {           // the tiles' rows, a quarter a warp
-                    constexpr int LPR = HD / 8, RPP = 32 / LPR;          // lanes of a row, rows of a pass
-                    const int c = lane % LPR, row0 = (warp - kPromptSoftmax) * 32 + lane / LPR;
-                    const int more_tokens = RPP / p.group, more_heads = RPP - more_tokens * p.group;
-                    const __half* from = p.q + (long long)piece->row * p.ldq + h * p.group * HD + 8 * c;
+                if (j == 0) {
 #pragma unroll 1
                     for (int tile = 0; tile < 2; ++tile) {
-                        if (!ok || piece->steps[tile] == 0 || !(ok = wait_warp(q_free + 8 * tile, ((had >> tile) & 1) ^ 1, dead, 130))) continue;
-                        had ^= 1u << tile;
-                        int token = (piece->r0 + 128 * tile + row0) / p.group, head = piece->r0 + 128 * tile + row0 - token * p.group;
-                        const int rows = piece->rows - 128 * tile;
-#pragma unroll 2
-                        for (int i = 0; i < 32 / RPP; ++i) {
-                            const int row = row0 + i * RPP;
-                            copy_async_16(q_smem + tile * C::Q_TILE + row * 128 + (c >> 3) * C::Q_BLOCK + (((c & 7) ^ (row & 7)) << 4),
-                                          from + (row < rows ? (long long)token * p.ldq + head * HD : 0ll), row < rows);
-                            token += more_tokens;
-                            head += more_heads;
-                            if (head >= p.group) {
-                                head -= p.group;
-                                ++token;
-                            }
-                        }
-                        asm volatile("cp.async.wait_all;" ::: "memory");
-                        fence_async_smem();
-                        arrive_warp(q_ready + 8 * tile, lane);
+                        if (!(rows_missing >> tile & 1)) continue;
+                        rows_there();
+                        if (!(ok = wait_warp(q_free + 8 * tile, ((had >> tile) & 1) ^ 1, dead, 130))) break;
+                        copy_rows(tile);
                     }
                     if (!ok) break;
+                    rows_there();
                 }
                 if (!(ok = wait_warp(v_empty + 8 * stage, parity, dead, 124))) break;
 #pragma unroll
