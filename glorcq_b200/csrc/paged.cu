@@ -858,10 +858,10 @@ AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, 
     };
     // From 64 channels on, 256 (128) rows of a head at once on the 5th-generation tensor cores, where that is much work: those tiles multiply four times
     // as fast, but a call begins and joins slower, and a tile that is not full costs as much as a full one.  Measured (graph, us, tiles of 16 / prompt
-    // kernel; 128 channels, 8 heads, 4 rows of q a token): 16 tokens after 1000 8.9 / 30, 64 after 4000 39 / 45, 128 after 1000 27 / 45 and after 4000
-    // 64 / 46, 256 after none 28 / 31 and after 4000 117 / 50, 512 after 4000 222 / 73; 16 sequences of 32 tokens, 16 heads of their own (32 rows), after
-    // 1000 55 / 63 and after 4000 119 / 150, of 64 tokens 98 / 64 and 220 / 151.  256 channels, 2 heads: 64 tokens after 4000 21 / 51, 256 after 4000
-    // 68 / 60; 64 channels, 4 heads: 128 after 4000 27 / 36, 256 after 4000 44 / 37 (a row there costs tiles of 16 nearly what one of 128 does).
+    // kernel; 128 channels, 8 heads, 4 rows of q a token): 16 tokens after 1000 8.8 / 25, 64 after 4000 39 / 38, 128 after 1000 27 / 35 and after 4000
+    // 64 / 40, 256 after none 28 / 18 and after 4000 117 / 47; 16 sequences of 32 tokens, 16 heads of their own (32 rows), after 1000 55 / 66 and after
+    // 4000 119 / 147, of 64 tokens 98 / 67 and 220 / 146.  256 channels, 2 heads: 64 tokens after 4000 22 / 47, 256 after 4000 67 / 59; 64 channels,
+    // 4 heads: 128 after 4000 27 / 32, 256 after 4000 44 / 35 (a row there costs tiles of 16 nearly what one of 128 does).
     const long long every = most * rows->B * kv->n_kv;
     if (D >= 64 && most > 32 && (every > 4096 || every * std::max(D, 128) > (1ll << 31) / ((long long)kv->max_pages * kv->page)))
         return D == 256 ? make(AttnKernel::prompt, 1, PromptShape<256>::Share{}) : make(AttnKernel::prompt, 1, PromptShape<128>::Share{});

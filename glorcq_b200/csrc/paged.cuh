@@ -98,10 +98,14 @@ __device__ __forceinline__ void after_launch_ahead() {
 // (sequence, block of rows, head), are cut into equal shares, one for each CTA, whatever the lengths: these are on the device, and a batch of
 // 64 sequences of 800 to 8192 tokens takes as long as its sum, not as its longest.  A cut that falls into a segment's EXTRA units parts nothing;
 // another leaves partial results, at most two of them per CTA, which paged_join_kernel joins.
+// Where shares of LEAST units do not go round, a segment's units are rounded up to a multiple of LEAST, so that no CTA has the end of one and the
+// beginning of the next.
 // Blocks of rows are numbered so that nobody has to count those of the sequences before: sequence b's are rows * group / R + b and on.
 template <int R_, int STEP_, int EXTRA_, int LEAST_> struct ShareOf {
     static constexpr int R = R_, STEP = STEP_, EXTRA = EXTRA_;
     static constexpr int LEAST = LEAST_;      // units of a share, so long as there are fewer shares than CTAs
+    // units of a segment
+    static __host__ __device__ __forceinline__ int units(int steps, int grain) { return LEAST == 1 || grain == 1 ? steps + EXTRA : (steps + EXTRA + LEAST - 1) / LEAST * LEAST; }
 };
 // Units are counted in 32 bits (the host refuses what might not fit: 64-bit divisions took longer than the rest of a small call's planning).
 __device__ __forceinline__ int share_begin(int total, int cta, int n_cta) { return total / n_cta * cta + total % n_cta * cta / n_cta; }
@@ -133,8 +137,8 @@ template <class S> __device__ __forceinline__ RowBlock row_block(const PagedKv& 
     x.steps = x.n_rows > 0 ? min(x.start + (x.r0 + x.n_rows - 1) / group, kv.capacity - 1) / S::STEP + 1 : 0;
     return x;
 }
-template <class S> __device__ __forceinline__ int block_units(const PagedKv& kv, const RowBlock& x) {
-    return x.n_rows > 0 ? kv.n_kv * (x.steps + S::EXTRA) : 0;
+template <class S> __device__ __forceinline__ int block_units(const PagedKv& kv, const RowBlock& x, int grain) {
+    return x.n_rows > 0 ? kv.n_kv * S::units(x.steps, grain) : 0;
 }
 template <class S> inline bool units_fit(int rows, int B, int group, int n_kv, int capacity) {
     return ((double)rows * group / S::R + B) * n_kv * ((double)capacity / S::STEP + 1 + S::EXTRA) < 2147483647.0;
@@ -143,10 +147,10 @@ template <class S> __host__ __device__ __forceinline__ int block_count(int rows,
     return (int)((long long)rows * group / S::R) + B;
 }
 
-// Where a CTA's share begins: in block i, x, off units of which belong to shares before; the units of all.
+// Where a CTA's share begins: in block i, x, off units of which belong to shares before; what units are rounded to (1 or LEAST).
 struct ShareStart {
     RowBlock x;
-    int i, off;
+    int i, off, grain;
     int sums[32];
 };
 // All threads of the block; `sm` in shared memory.  Returns the units of all; what it says of the beginning holds where `cta` has a share.
@@ -164,30 +168,37 @@ __device__ __forceinline__ int paged_plan(const PagedKv& kv, const PagedRows& r,
             if (f(i, row_block<S>(kv, r, group, i, b))) return;
         }
     };
-    int mine = 0;
+    int mine, before, total, grain = 1;       // units of the thread's blocks, of those before them, of all
     RowBlock x{};
-    each([&](int, const RowBlock& y) {
-        x = y;
-        mine += block_units<S>(kv, y);
-        return false;
-    });
-    int incl = mine;
+    for (;; grain = S::LEAST) {
+        mine = 0;
+        each([&](int, const RowBlock& y) {
+            x = y;
+            mine += block_units<S>(kv, y, grain);
+            return false;
+        });
+        int incl = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += o;
-    }
-    if (lane == 31) sm.sums[warp] = incl;
-    __syncthreads();
-    int before = 0, total = 0;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 31) sm.sums[warp] = incl;
+        __syncthreads();
+        before = incl - mine;
+        total = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        if (w < warp) before += sm.sums[w];
-        total += sm.sums[w];
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) before += sm.sums[w];
+            total += sm.sums[w];
+        }
+        if (S::LEAST == 1 || grain > 1 || total > n_cta * S::LEAST) break;
+        __syncthreads();
     }
+    if (tid == 0) sm.grain = grain;
     const int n = share_ctas<S>(total, n_cta);
     const int u0 = cta < n ? share_begin(total, cta, n) : total;
-    int at = before + incl - mine;
+    int at = before;
     if (u0 >= at && u0 < at + mine) {
         if (per == 1) {
             sm.x = x;
@@ -195,7 +206,7 @@ __device__ __forceinline__ int paged_plan(const PagedKv& kv, const PagedRows& r,
             sm.off = u0 - at;
         } else {
             each([&](int i, const RowBlock& y) {
-                const int w = block_units<S>(kv, y);
+                const int w = block_units<S>(kv, y, grain);
                 if (u0 < at + w) {
                     sm.x = y;
                     sm.i = i;
@@ -223,7 +234,7 @@ template <class S> struct Pieces {
     int left, off, i;
     RowBlock x;                  // block i
     int h, step0, step1;         // the piece: steps step0 .. step1 of head h of it
-    int total, n_cta;
+    int total, n_cta, grain;
     template <int THREADS> __device__ __forceinline__ void begin(const PagedKv& kv, const PagedRows& r, int group, int cta, int most_ctas, ShareStart& sm) {
         total = paged_plan<S, THREADS>(kv, r, group, cta, most_ctas, sm);
         n_cta = share_ctas<S>(total, most_ctas);
@@ -231,10 +242,11 @@ template <class S> struct Pieces {
         i = sm.i;
         off = sm.off;
         x = sm.x;
+        grain = sm.grain;
     }
     __device__ __forceinline__ bool next(const PagedKv& kv, const PagedRows& r, int group) {
         while (left > 0) {
-            if (off >= block_units<S>(kv, x)) {
+            if (off >= block_units<S>(kv, x, grain)) {
                 ++i;
                 off = 0;
                 int b = x.b;
@@ -242,13 +254,13 @@ template <class S> struct Pieces {
                 x = row_block<S>(kv, r, group, i, b);
                 continue;
             }
-            const int units = x.steps + S::EXTRA;
+            const int units = S::units(x.steps, grain);
             h = off / units;
             const int v0 = off - h * units, v1 = min(units, v0 + left);
             off += v1 - v0;
             left -= v1 - v0;
             step0 = max(v0 - S::EXTRA, 0);
-            step1 = max(v1 - S::EXTRA, 0);
+            step1 = min(max(v1 - S::EXTRA, 0), x.steps);
             if (step1 > step0) return true;
         }
         return false;
@@ -260,11 +272,11 @@ template <class S> __device__ __forceinline__ JoinItem join_item(int total, int 
     JoinItem j{};
     const int n = share_ctas<S>(total, most_ctas);
     if (cta >= n || share_begin(total, cta, n) == share_begin(total, cta + 1, n)) return j;
-    const int units = sm.x.steps + S::EXTRA, h = sm.off / units, v0 = sm.off - h * units;
-    if (v0 <= S::EXTRA) return j;
+    const int units = S::units(sm.x.steps, sm.grain), h = sm.off / units, v0 = sm.off - h * units;
+    if (v0 <= S::EXTRA || v0 - S::EXTRA >= sm.x.steps) return j;
     const int u0 = share_begin(total, cta, n) - v0, c0 = share_of(total, u0 + S::EXTRA, n);
     if (c0 + 1 != cta) return j;
-    j.parts = share_of(total, u0 + units - 1, n) - c0 + 1;
+    j.parts = share_of(total, u0 + S::EXTRA + sm.x.steps - 1, n) - c0 + 1;
     j.first_cta = c0;
     j.row = sm.x.own.x;
     j.r0 = sm.x.r0;
@@ -305,10 +317,12 @@ __device__ __forceinline__ float rcp_fast(float x) {
     return y;
 }
 // Blocks of rows of paged_prompt_kernel (paged_prompt.cu): many rows a head.  Two tiles of 128 rows and steps of 128 tokens; with 256 channels one tile and
-// 64 tokens, which is what tensor memory and shared memory hold.
+// 64 tokens, which is what tensor memory and shared memory hold.  A segment's beginning and end count as two steps, the least share is six.  Measured (us,
+// shares rounded up to (extra, least) = (2, 4) / (2, 6) / (4, 8)): 16 heads, 512 tokens 26.8 / 23.0 / 23.1; 32 heads on 8, 256 tokens after 1000 34.9 /
+// 39.2 / 39.1, 1024 tokens 41.0 / 44.6 / 45.6; 32 on 4, 4096 tokens 209 / 211 / 214; not rounded up, (4, 8): 24.1, 44.5, 44.4, 217.
 template <int HD> struct PromptShape {
     static constexpr int TILES = HD == 256 ? 1 : 2, STEP = HD == 256 ? 64 : 128;
-    using Share = ShareOf<128 * TILES, STEP, 4, 8>;
+    using Share = ShareOf<128 * TILES, STEP, 2, 6>;
 };
 cudaError_t launch_paged_prompt(int head_dim, int dtype, const AttnParams& p, int grid, cudaStream_t st);
 
