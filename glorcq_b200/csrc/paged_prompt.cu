@@ -3,7 +3,10 @@
 // Segment: 256 rows (token of the call, head of the group), two tiles of 128, of one (sequence, key/value head); step: 128 tokens.  (Heads of 256
 // channels: one tile, 64 tokens; the warps of the other tile only give stages back.)
 // A step's products are S = Q K^T (operands in shared memory) and O += P V (P in tensor memory, over the scores that it is made of; V as it
-// lies, tokens by channels, which is the MN-major form of the operand).  Tensor memory: S of both tiles, O of both tiles.
+// lies, tokens by channels, which is the MN-major form of the operand), each in half steps of 64 tokens.  Tensor memory: a tile has two places
+// for S, which half steps take in turn, and O.  While the softmax of one half step runs, P V of the one before and S of the one after do: the
+// softmax, which takes longest, hardly ever waits (a step of 128 tokens in one piece, whose next scores had to wait for its P V: 4 heads,
+// 4096 tokens, 211 us against 183).
 //
 // Warps, which keep their roles over all segments of a CTA:
 //   0..3, 4..7  softmax of tile 0 and 1: a thread has a row; writes P as fp16, multiplies O where m has grown, writes the result
@@ -11,13 +14,11 @@
 //               warp's at a time; a segment's rows
 //   12, 13      issue the MMAs of tile 0 and 1 (one warp for both needed longer for it than the MMAs themselves)
 //   15          works out the CTA's pieces of segments and hands them to the others through a small queue
-// P takes half of the columns of the scores that it is made of, so the next scores of a tile wait for its P V; the other tile's products run
-// meanwhile, and while this one's softmax does.
 // Scales and m as in paged_attention_rows_kernel: w = 2^(ks s + log2 vs - m) in fp16, the sum of w / vs in fp32, m raised only when a score exceeds it
-// by 2^8.  Keys that a row does not see get a score of -3e38 in tensor memory, in the steps that have such keys, and the common path has no masks.
+// by 2^8.  Keys that a row does not see get a score of -3e38, in the half steps that have such keys, and the common path has no masks.
 //
-// The loops are rolled where they can be: every warp of a scheduler runs another role's code, and what the instruction cache does not hold costs the
-// one warp that issues the MMAs more than the MMAs (134 cycles an MMA with unrolled loops everywhere).
+// The loops around it all are rolled: every warp of a scheduler runs another role's code, and what the instruction cache does not hold costs the
+// warps that issue the MMAs more than the MMAs (134 cycles an MMA with unrolled loops everywhere).
 //
 // Every wait is bounded (tc_wait); a wait that runs out marks the CTA dead, all roles leave their loops and the kernel ends.
 #include "paged.cuh"
@@ -38,9 +39,10 @@ namespace {
 
 constexpr int kPromptSoftmax = 8, kPromptProducers = 4, kPromptMma = kPromptSoftmax + kPromptProducers;
 constexpr int kPromptThreads = (kPromptMma + 4) * 32;
-// Registers of a thread: 128 at launch.
-constexpr int kRegsSoftmax = 168, kRegsProducer = 104, kRegsMma = 72;
+// Registers of a thread: 128 at launch.  (168, 104 and 72 made the MMA warps reload what they had put away: 219 us where this split takes 183.)
+constexpr int kRegsSoftmax = 152, kRegsProducer = 128, kRegsMma = 80;
 static_assert((kPromptSoftmax * kRegsSoftmax + kPromptProducers * kRegsProducer + 4 * kRegsMma) * 32 <= kPromptThreads * 128, "registers");
+static_assert(kRegsSoftmax >= 128 && kRegsProducer <= 128 && kRegsMma <= 128, "the softmax takes what the others give");
 // every so many pairs of exponentials one is taken by exp2_poly
 constexpr int kPolyEvery = 4;
 
@@ -208,9 +210,9 @@ template <int HD, int DT>
 __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const AttnParams p) {
     using C = PromptCfg<HD>;
     using Share = typename C::Share;
-    constexpr int kStepTokens = C::STEP, kGroups = C::GROUPS;
+    constexpr int kStepTokens = C::STEP, kGroups = C::GROUPS, kHalves = kStepTokens / 64;
     extern __shared__ unsigned char prompt_smem[];
-    __shared__ __align__(8) unsigned long long bars[2 * 11 + 2 * kPieceQueue];
+    __shared__ __align__(8) unsigned long long bars[26 + 2 * kPieceQueue];
     __shared__ PromptPiece s_piece[kPieceQueue];
     __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs
     __shared__ ShareStart sm_plan;
@@ -219,10 +221,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(prompt_smem) + 1023u) & ~1023u;
     const uint32_t q_smem = base, k_smem = base + C::TILES * C::Q_TILE, v_smem = k_smem + 2 * C::KV_TILE;
-    // [0], [1] of each: stages or tiles
+    // [0], [1] of each: stages or tiles; of s_full, p_ready and pv_done four: [tile][place of the scores]
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48, s_full = k_full + 64,
-                   p_ready = k_full + 80, pv_done = k_full + 96, q_ready = k_full + 112, o_free = k_full + 128, q_free = k_full + 144,
-                   p_half = k_full + 160, piece_full = k_full + 176, piece_empty = piece_full + 8 * kPieceQueue;
+                   p_ready = k_full + 96, pv_done = k_full + 128, q_ready = k_full + 160, o_free = k_full + 176, q_free = k_full + 192,
+                   piece_full = k_full + 208, piece_empty = piece_full + 8 * kPieceQueue;
     volatile int* dead = &s_dead;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -230,13 +232,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             mbar_init(v_full + 8 * i, kPromptProducers);
             mbar_init(k_empty + 8 * i, 2);
             mbar_init(v_empty + 8 * i, 2);
-            mbar_init(s_full + 8 * i, 1);
-            mbar_init(pv_done + 8 * i, 1);
-            mbar_init(p_ready + 8 * i, 4);
-            mbar_init(p_half + 8 * i, 4);
             mbar_init(q_ready + 8 * i, kPromptProducers);
             mbar_init(q_free + 8 * i, 1);
             mbar_init(o_free + 8 * i, 4);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_ready + 8 * i, 4);
+            mbar_init(pv_done + 8 * i, 1);
         }
         for (int i = 0; i < kPieceQueue; ++i) {
             mbar_init(piece_full + 8 * i, 1);
@@ -276,56 +279,49 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         const int tile = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t s_tm = trow + C::S_COL + tile * 128, o_tm = trow + C::O_COL + tile * HD;
-        uint32_t done = 0;               // this tile's steps of the pieces before
+        uint32_t t = 0;                  // the tile's half steps so far: half step t has its scores, and P, at place t % 2
         while (next_piece()) {
             const int steps = piece->steps[tile], first_row = piece->r0 + 128 * tile;
             const bool live = row < piece->rows - 128 * tile;
             const int limit = live ? min(piece->start + (first_row + row) / p.group, p.kv.capacity - 1) : -1;      // the last key that the row sees
             const int limit_low = min(piece->start + first_row / p.group, p.kv.capacity - 1);                      // that every row of the tile sees
+            const uint32_t t0 = t;
             int first = piece->step0 * kStepTokens;
             float m = -1e30f, l = 0.f;
-            for (int j = 0; j < steps && ok; ++j, first += kStepTokens) {
-                const uint32_t g = gs + j;
-                ok = wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121) && wait_warp(s_full + 8 * tile, done & 1, dead, 120);
+#pragma unroll 1
+            for (; t < t0 + kHalves * steps; ++t, first += 64) {
+                const uint32_t half = (t - t0) % kHalves, g = gs + (t - t0) / kHalves, bar = 16 * tile + 8 * (t & 1), s_at = s_tm + 64 * (t & 1);
+                ok = (half > 0 || wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121)) && wait_warp(s_full + bar, (t >> 1) & 1, dead, 120);
                 if (!ok) break;
                 tc_fence_after();
-                const float4* scale = s_scale[g & 1];
-                if (first + kStepTokens - 1 > limit_low) {
-#pragma unroll 1
-                    for (int c = max(0, (limit_low - first) / 16); c < kGroups; ++c) {
-                        uint32_t v[16];
-                        tc_ld16(s_tm + 16 * c, v);
-                        tmem_arrived(v);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (first + 16 * c + i > limit) v[i] = __float_as_uint(-3e38f);
-                        tmem_st<16>(s_tm + 16 * c, v);
-                    }
-                    tmem_st_wait();
-                }
-                // 32 columns at a time, the next ones on their way
                 uint32_t v[2][32];
-                tmem_ld32(s_tm, v[0]);
+                tmem_ld32(s_at, v[0]);
+                tmem_ld32(s_at + 32, v[1]);
+                tmem_arrived(v[0]);
+                tmem_arrived(v[1]);
+                const float4* scale = s_scale[g & 1] + 4 * half;
+                if (first + 63 > limit_low) {
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (first + i > limit) v[i / 32][i % 32] = __float_as_uint(-3e38f);
+                }
                 float top = -INFINITY;
-#pragma unroll 2
-                for (int c = 0; c < kStepTokens / 32; ++c) {
-                    tmem_arrived(v[c & 1]);
-                    tmem_ld32(s_tm + 32 * ((c + 1) % (kStepTokens / 32)), v[(c + 1) & 1]);         // (and the first ones again)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t* u = v[c & 1] + 16 * half;
-                        const float4 sc = scale[2 * c + half];
-                        float x = max3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t* u = v[q / 2] + 16 * (q % 2);
+                    const float4 sc = scale[q];
+                    float x = max3(__uint_as_float(u[0]), __uint_as_float(u[1]), __uint_as_float(u[2]));
 #pragma unroll
-                        for (int i = 3; i < 15; i += 2) x = max3(x, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
-                        top = fmaxf(top, fmaf(fmaxf(x, __uint_as_float(u[15])), sc.x, sc.y));
-                    }
+                    for (int i = 3; i < 15; i += 2) x = max3(x, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+                    top = fmaxf(top, fmaf(fmaxf(x, __uint_as_float(u[15])), sc.x, sc.y));
                 }
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float up = fmaxf(m, top), f = exp2_fast(m - up);
                     m = up;
                     l *= f;
-                    if (j > 0)            // (the product before this step's scores has been added)
+                    if (t > t0) {         // the products so far, the last of which may be running
+                        if (!(ok = wait_warp(pv_done + 16 * tile + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1, dead, 122))) break;
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < HD / 16; ++c) {
                             uint32_t x[16];
@@ -335,54 +331,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                             for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
                             tmem_st<16>(o_tm + 16 * c, x);
                         }
+                    }
                 }
-#pragma unroll 1
-                for (int c2 = 0; c2 < kStepTokens / 32; c2 += 2) {
-                    uint32_t w[32];
+                uint32_t w[16];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        tmem_arrived(v[c]);
-                        if (c2 + c < kStepTokens / 32 - 1) tmem_ld32(s_tm + 32 * (c2 + c + 1), v[c ^ 1]);
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t* u = v[q / 2] + 16 * (q % 2);
+                    const float4 sc = scale[q];
+                    const float off = sc.y - m;
+                    const unsigned long long cs2 = pack2(sc.x, sc.x), off2 = pack2(off, off);
+                    unsigned long long sum2 = 0ull;
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint32_t* u = v[c] + 16 * half;
-                            const float4 sc = scale[2 * (c2 + c) + half];
-                            const float off = sc.y - m;
-                            const unsigned long long cs2 = pack2(sc.x, sc.x), off2 = pack2(off, off);
-                            unsigned long long sum2 = 0ull;
-#pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                const unsigned long long x = fma2(pack2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), cs2, off2);
-                                float a, b;
-                                if (i / 2 % kPolyEvery == kPolyEvery - 1) {
-                                    exp2_poly(x, a, b);
-                                } else {
-                                    unpack2(x, a, b);
-                                    a = exp2_fast(a);
-                                    b = exp2_fast(b);
-                                }
-                                sum2 = add2(sum2, pack2(a, b));
-                                w[16 * c + 8 * half + i / 2] = pack_half2(a, b);
-                            }
-                            float a, b;
-                            unpack2(sum2, a, b);
-                            l += (a + b) * sc.z;
+                    for (int i = 0; i < 16; i += 2) {
+                        const unsigned long long x = fma2(pack2(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), cs2, off2);
+                        float a, b;
+                        if (i / 2 % kPolyEvery == kPolyEvery - 1) {
+                            exp2_poly(x, a, b);
+                        } else {
+                            unpack2(x, a, b);
+                            a = exp2_fast(a);
+                            b = exp2_fast(b);
                         }
+                        sum2 = add2(sum2, pack2(a, b));
+                        w[8 * (q % 2) + i / 2] = pack_half2(a, b);
                     }
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) tmem_st<16>(s_tm + 16 * (c2 + c), w + 16 * c);
-                    if (c2 == 0) {          // P V of the first 64 tokens may begin
-                        tmem_st_wait();
-                        tc_fence_before();
-                        arrive_warp(p_half + 8 * tile, lane);
-                    }
+                    float a, b;
+                    unpack2(sum2, a, b);
+                    l += (a + b) * sc.z;
+                    if (q % 2) tmem_st<16>(s_at + 16 * (q / 2), w);
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                arrive_warp(p_ready + 8 * tile, lane);
-                ++done;
+                arrive_warp(p_ready + bar, lane);
             }
-            if (ok && steps > 0) ok = wait_warp(pv_done + 8 * tile, (done - 1) & 1, dead, 122);
+            if (ok && steps > 0) ok = wait_warp(pv_done + 16 * tile + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1, dead, 122);
             if (!ok) break;
             tc_fence_after();
             if (m <= -1e30f) l = 0.f;         // nothing seen: the sum is of exp2_poly's smallest numbers
@@ -580,51 +562,47 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
         if (warp < kPromptMma + 2) {
             // ================= MMA issue =================
-            constexpr uint32_t s_desc = tc_idesc(kStepTokens), o_desc = tc_idesc(HD) | (1u << 16);       // V: MN-major
+            constexpr uint32_t s_desc = tc_idesc(64), o_desc = tc_idesc(HD) | (1u << 16);       // V: MN-major
             const int tile = warp - kPromptMma;
-            const uint32_t s_at = tmem + C::S_COL + tile * 128, o_at = tmem + C::O_COL + tile * HD, bar = 8 * tile;
+            const uint32_t s_at = tmem + C::S_COL + tile * 128, o_at = tmem + C::O_COL + tile * HD, bar = 8 * tile, bar2 = 16 * tile;
             const uint64_t q_at = tc_smem_desc(q_smem + tile * C::Q_TILE), k_at = tc_smem_desc(k_smem), v_at = value_desc(v_smem, C::KV_BLOCK);
-            auto scores = [&](uint32_t stage) {
-                const uint64_t k = k_at + stage * (C::KV_TILE >> 4);
-#pragma unroll
-                for (int blk = 0; blk < C::BLOCKS; ++blk) mma4_ss(s_at, q_at + blk * (C::Q_BLOCK >> 4), k + blk * (C::KV_BLOCK >> 4), s_desc, blk > 0);
-                commit_warp(s_full + bar);
-            };
-            uint32_t done = 0, had = 0;           // steps, pieces that the tile had steps in
+            uint32_t t = 0, had = 0;              // half steps as in the softmax, pieces that the tile had steps in
             while (next_piece()) {
-                const int n = piece->steps[tile], steps = piece->most;
-                if (n > 0) {
-                    ok = wait_warp(q_ready + bar, had & 1, dead, 125) && wait_warp(k_full + 8 * (gs & 1), (gs >> 1) & 1, dead, 126);
-                    if (!ok) break;
+                const int n = kHalves * piece->steps[tile], steps = piece->most;
+                auto scores = [&](int i) {        // of the piece's half step i, t + i
+                    const uint32_t g = gs + i / kHalves, place = (t + i) & 1;
+                    if (i % kHalves == 0 && !wait_warp(k_full + 8 * (g & 1), (g >> 1) & 1, dead, 126)) return false;
                     tc_fence_after();
-                    scores(gs & 1);
-                }
-                for (int j = 0; j < n; ++j, ++done) {
-                    const uint32_t g = gs + j, stage = g & 1;
-                    // (who has written P has waited for V; the next K is usually there long before P)
-                    ok = (j > 0 || wait_warp(o_free + bar, (had & 1) ^ 1, dead, 128)) &&
-                         (j + 1 == n || wait_warp(k_full + 8 * (stage ^ 1), ((g + 1) >> 1) & 1, dead, 126)) && wait_warp(p_half + bar, done & 1, dead, 127);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t v = v_at + stage * (C::KV_TILE >> 4);
-                    mma4_ts(o_at, s_at, v, o_desc, j > 0);
-                    if (!(ok = wait_warp(p_ready + bar, done & 1, dead, 129))) break;
-                    tc_fence_after();
-                    if (kStepTokens == 128) mma4_ts(o_at, s_at + 32, v + (8192 >> 4), o_desc, 1);
-                    commit_warp(pv_done + bar);
-                    if (lane == 0) {
-                        mbar_arrive(k_empty + 8 * stage);
-                        if (j + 1 == n) mbar_arrive(q_free + bar);
-                    }
-                    if (!(ok = wait_warp(pv_done + bar, done & 1, dead, 122))) break;
-                    if (j + 1 < n) {
+                    const uint64_t k = k_at + (g & 1) * (C::KV_TILE >> 4) + i % kHalves * (8192 >> 4);
+#pragma unroll
+                    for (int blk = 0; blk < C::BLOCKS; ++blk) mma4_ss(s_at + 64 * place, q_at + blk * (C::Q_BLOCK >> 4), k + blk * (C::KV_BLOCK >> 4), s_desc, blk > 0);
+                    commit_warp(s_full + bar2 + 8 * place);
+                    return true;
+                };
+                if (n > 0) ok = wait_warp(q_ready + bar, had & 1, dead, 125);
+#pragma unroll 1
+                for (int i = -2; i < n && ok; ++i) {
+                    if (i >= 0) {
+                        const uint32_t g = gs + i / kHalves, stage = g & 1, place = (t + i) & 1, parity = ((t + i) >> 1) & 1;
+                        const bool last = i % kHalves == kHalves - 1;         // of its step
+                        ok = (i > 0 || wait_warp(o_free + bar, (had & 1) ^ 1, dead, 128)) && wait_warp(p_ready + bar2 + 8 * place, parity, dead, 129);
+                        if (!ok) break;
                         tc_fence_after();
-                        scores(stage ^ 1);
+                        // (who has written P has waited for V)
+                        mma4_ts(o_at, s_at + 64 * place, v_at + stage * (C::KV_TILE >> 4) + i % kHalves * (8192 >> 4), o_desc, i > 0);
+                        commit_warp(pv_done + bar2 + 8 * place);
+                        if (lane == 0) {                                      // the step's scores have all been read
+                            if (last) mbar_arrive(k_empty + 8 * stage);
+                            if (i + 1 == n) mbar_arrive(q_free + bar);
+                        }
+                        if (!(ok = wait_warp(pv_done + bar2 + 8 * place, parity, dead, 122))) break;
+                        if (last && lane == 0) mbar_arrive(v_empty + 8 * stage);
                     }
-                    if (lane == 0) mbar_arrive(v_empty + 8 * stage);
+                    if (i + 2 < n) ok = scores(i + 2);
                 }
+                t += n;
                 // steps that only the other tile takes part in
-                for (int j = n; j < steps && ok; ++j) {
+                for (int j = piece->steps[tile]; j < steps && ok; ++j) {
                     const uint32_t g = gs + j, stage = 8 * (g & 1);
                     ok = wait_warp(k_full + stage, (g >> 1) & 1, dead, 126) && wait_warp(v_full + stage, (g >> 1) & 1, dead, 121);
                     if (ok && lane == 0) {
