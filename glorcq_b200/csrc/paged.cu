@@ -665,56 +665,98 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
     if (!CLUSTER && threadIdx.x == 0) p.join[blockIdx.x] = join_item<Share>(piece.total, gridDim.x, blockIdx.x, sm_plan);
 }
 
-// Joins the partial results of segments that several CTAs shared: 32 rows of one a CTA, a warp a row.  Lane c looks at the maximum and sum of
-// the c-th part, the values are added in the order of the shares, eight parts requested together.
+// Joins the partial results of segments that several CTAs shared: 32 rows of one a CTA.  Lane c looks at the maximum and sum of the c-th part, the
+// values are added in the order of the shares.  A warp takes a row, and requests eight parts together; a prompt's segment has two parts as a rule and 256
+// rows, and a warp requests two parts of four rows together (four chunks of 700 rows after 2900, 38 MB of partial results: 66 us with one row at a time,
+// 62 with four).
 template <int HD, int DT, class S>
 __global__ void __launch_bounds__(kRowsThreads) paged_join_kernel(const AttnParams p) {
     constexpr int VPL = HD / 32;                     // channels of a lane
+    constexpr int ROWS = S::R >= 128 ? 4 : 1, PARTS = 8 / ROWS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     after_launch_ahead();
     const JoinItem x = p.join[blockIdx.x];
-    const int r0 = x.r0, n_rows = min(x.n_rows, (int)blockIdx.y * 32 + 32), c0 = x.first_cta, c1 = c0 + x.parts - 1, h = x.h;
+    const int n_rows = min(x.n_rows, (int)blockIdx.y * 32 + 32), c0 = x.first_cta, c1 = c0 + x.parts - 1;
     if (x.parts == 0) return;
-    constexpr int R = S::R;
     auto part_of = [&](int c) { return partial_of<S, HD>(p.partial, c, c == c0); };
-    for (int r = blockIdx.y * 32 + warp; r < n_rows; r += kRowsWarps) {
-        float mx = -1e30f, sum = 0.f, acc[VPL];
+    for (int r0 = blockIdx.y * 32 + warp; r0 < n_rows; r0 += kRowsWarps * ROWS) {
+        float mx[ROWS], sum[ROWS], acc[ROWS][VPL];
+        int row[ROWS];
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) acc[i] = 0.f;
+        for (int k = 0; k < ROWS; ++k) {
+            row[k] = min(r0 + k * kRowsWarps, n_rows - 1);          // (the last row again where there are no more)
+            mx[k] = -1e30f;
+            sum[k] = 0.f;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) acc[k][i] = 0.f;
+        }
         for (int base = c0; base <= c1; base += 32) {
-            const int c = base + lane;
-            const bool live = c <= c1;
-            const float2 ml = live ? *reinterpret_cast<const float2*>(part_of(c) + R * HD + 2 * r) : make_float2(-1e30f, 0.f);
-            float top = fmaxf(ml.x, mx);
+            const int c = base + lane, n = min(32, c1 - base + 1);
+            float2 ml[ROWS];
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float f = exp2_fast(mx - top), w = exp2_fast(ml.x - top);
-            mx = top;
-            sum = sum * f + warp_sum(ml.y * w);
+            for (int k = 0; k < ROWS; ++k) ml[k] = c <= c1 ? *reinterpret_cast<const float2*>(part_of(c) + S::R * HD + 2 * row[k]) : make_float2(-1e30f, 0.f);
+            float w[ROWS];
 #pragma unroll
-            for (int i = 0; i < VPL; ++i) acc[i] *= f;
-            const unsigned there = __ballot_sync(0xffffffffu, live);
-            const int n = min(32, c1 - base + 1);
-            for (int k = 0; k < n; k += 8) {
-                float v[8][VPL];
+            for (int k = 0; k < ROWS; ++k) {
+                float top = fmaxf(ml[k].x, mx[k]);
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const float* src = part_of(base + k + u) + r * HD + lane * VPL;
+                for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float f = exp2_fast(mx[k] - top);
+                w[k] = exp2_fast(ml[k].x - top);
+                mx[k] = top;
+                sum[k] = sum[k] * f + warp_sum(ml[k].y * w[k]);
 #pragma unroll
-                    for (int i = 0; i < VPL; ++i) v[u][i] = there >> (k + u) & 1u ? src[i] : 0.f;
-                }
+                for (int i = 0; i < VPL; ++i) acc[k][i] *= f;
+            }
+            for (int u0 = 0; u0 < n; u0 += PARTS) {
+                float v[ROWS][PARTS][VPL];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const float wu = __shfl_sync(0xffffffffu, w, k + u);
+                for (int k = 0; k < ROWS; ++k)
 #pragma unroll
-                    for (int i = 0; i < VPL; ++i) acc[i] += v[u][i] * wu;
-                }
+                    for (int u = 0; u < PARTS; ++u) {
+                        const float* src = part_of(base + u0 + u) + row[k] * HD + lane * VPL;
+#pragma unroll
+                        for (int i = 0; i < VPL; i += VPL < 4 ? VPL : 4) {
+                            float* to = v[k][u] + i;
+                            const bool there = u0 + u < n;
+                            if constexpr (VPL >= 4) {
+                                const float4 t = there ? *reinterpret_cast<const float4*>(src + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                to[0] = t.x, to[1] = t.y, to[2] = t.z, to[3] = t.w;
+                            } else if constexpr (VPL == 2) {
+                                const float2 t = there ? *reinterpret_cast<const float2*>(src) : make_float2(0.f, 0.f);
+                                to[0] = t.x, to[1] = t.y;
+                            } else {
+                                to[0] = there ? *src : 0.f;
+                            }
+                        }
+                    }
+#pragma unroll
+                for (int k = 0; k < ROWS; ++k)
+#pragma unroll
+                    for (int u = 0; u < PARTS; ++u) {
+                        const float wu = __shfl_sync(0xffffffffu, w[k], u0 + u);
+#pragma unroll
+                        for (int i = 0; i < VPL; ++i) acc[k][i] += v[k][u][i] * wu;
+                    }
             }
         }
-        const float inv = result_factor(sum, kCodeUnit<DT>);
-        __half* dst = p.out + (long long)(x.row + (r0 + r) / p.group) * p.ldo + (h * p.group + (r0 + r) % p.group) * HD + lane * VPL;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) dst[i] = __float2half_rn(acc[i] * inv);
+        for (int k = 0; k < ROWS; ++k) {
+            if (r0 + k * kRowsWarps >= n_rows) break;
+            const float inv = result_factor(sum[k], kCodeUnit<DT>);
+            const int r = x.r0 + row[k];
+            __half* dst = p.out + (long long)(x.row + r / p.group) * p.ldo + (x.h * p.group + r % p.group) * HD + lane * VPL;
+            if constexpr (VPL == 1) {
+                *dst = __float2half_rn(acc[k][0] * inv);
+            } else {
+                uint32_t o[VPL / 2];
+#pragma unroll
+                for (int i = 0; i < VPL / 2; ++i) o[i] = pack_half2(acc[k][2 * i] * inv, acc[k][2 * i + 1] * inv);
+                if constexpr (VPL == 2) *reinterpret_cast<uint32_t*>(dst) = o[0];
+                if constexpr (VPL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
+                if constexpr (VPL == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
     }
 }
 
