@@ -201,7 +201,7 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 struct PromptPiece {
     int b, h, row, r0, rows, start;      // sequence, head; the sequence's first row in the batch, the block's first and number of rows; tokens before the call
     int step0;
-    int steps[2], most;                  // steps that a tile takes part in, the larger of them; most < 0 ends the list
+    int halves[2], most;                 // half steps that a tile takes part in; steps of both; most < 0 ends the list
     int whole;                           // the segment is this CTA's alone
 };
 constexpr int kPieceQueue = 4, kPieceReaders = kPromptSoftmax + kPromptProducers + 2;
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
         const uint32_t s_tm = trow + C::S_COL + tile * 128, o_tm = trow + C::O_COL + tile * HD;
         uint32_t t = 0;                  // the tile's half steps so far: half step t has its scores, and P, at place t % 2
         while (next_piece()) {
-            const int steps = piece->steps[tile], first_row = piece->r0 + 128 * tile;
+            const int halves = piece->halves[tile], first_row = piece->r0 + 128 * tile;
             const bool live = row < piece->rows - 128 * tile;
             const int limit = live ? min(piece->start + (first_row + row) / p.group, p.kv.capacity - 1) : -1;      // the last key that the row sees
             const int limit_low = min(piece->start + first_row / p.group, p.kv.capacity - 1);                      // that every row of the tile sees
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             int first = piece->step0 * kStepTokens;
             float m = -1e30f, l = 0.f;
 #pragma unroll 1
-            for (; t < t0 + kHalves * steps; ++t, first += 64) {
+            for (; t < t0 + halves; ++t, first += 64) {
                 const uint32_t half = (t - t0) % kHalves, g = gs + (t - t0) / kHalves, bar = 16 * tile + 8 * (t & 1), s_at = s_tm + 64 * (t & 1);
                 ok = (half > 0 || wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121)) && wait_warp(s_full + bar, (t >> 1) & 1, dead, 120);
                 if (!ok) break;
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 tc_fence_before();
                 arrive_warp(p_ready + bar, lane);
             }
-            if (ok && steps > 0) ok = wait_warp(pv_done + 16 * tile + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1, dead, 122);
+            if (ok && halves > 0) ok = wait_warp(pv_done + 16 * tile + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1, dead, 122);
             if (!ok) break;
             tc_fence_after();
             if (m <= -1e30f) l = 0.f;         // nothing seen: the sum is of exp2_poly's smallest numbers
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {
                     uint32_t v[32];
-                    if (steps > 0) {
+                    if (halves > 0) {
                         tmem_ld32(o_tm + 32 * c, v);
                         tmem_arrived(v);
                     } else {
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 if (live && !whole) *reinterpret_cast<float2*>(part + Share::R * HD + 2 * (128 * tile + row)) = make_float2(m, l);
             }
             tc_fence_before();
-            if (steps > 0) arrive_warp(o_free + 8 * tile, lane);
+            if (halves > 0) arrive_warp(o_free + 8 * tile, lane);
             gs += piece->most;
             done_piece();
         }
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             const int c = lane % LPR, row0 = (warp - kPromptSoftmax) * 32 + lane / LPR;
             const int more_tokens = RPP / p.group, more_heads = RPP - more_tokens * p.group;
             const __half* from = p.q + (long long)piece->row * p.ldq + h * p.group * HD + 8 * c;
-            uint32_t rows_missing = (piece->steps[0] > 0) | (piece->steps[1] > 0) << 1, rows_coming = 0;
+            uint32_t rows_missing = (piece->halves[0] > 0) | (piece->halves[1] > 0) << 1, rows_coming = 0;
             auto copy_rows = [&](int tile) {
                 had ^= 1u << tile;
                 rows_missing ^= 1u << tile;
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             const uint64_t q_at = tc_smem_desc(q_smem + tile * C::Q_TILE), k_at = tc_smem_desc(k_smem), v_at = value_desc(v_smem, C::KV_BLOCK);
             uint32_t t = 0, had = 0;              // half steps as in the softmax, pieces that the tile had steps in
             while (next_piece()) {
-                const int n = kHalves * piece->steps[tile], steps = piece->most;
+                const int n = piece->halves[tile], steps = piece->most;
                 auto scores = [&](int i) {        // of the piece's half step i, t + i
                     const uint32_t g = gs + i / kHalves, place = (t + i) & 1;
                     if (i % kHalves == 0 && !wait_warp(k_full + 8 * (g & 1), (g >> 1) & 1, dead, 126)) return false;
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 for (int i = -2; i < n && ok; ++i) {
                     if (i >= 0) {
                         const uint32_t g = gs + i / kHalves, stage = g & 1, place = (t + i) & 1, parity = ((t + i) >> 1) & 1;
-                        const bool last = i % kHalves == kHalves - 1;         // of its step
+                        const bool last = i % kHalves == kHalves - 1 || i + 1 == n;         // of its step
                         ok = (i > 0 || wait_warp(o_free + bar, (had & 1) ^ 1, dead, 128)) && wait_warp(p_ready + bar2 + 8 * place, parity, dead, 129);
                         if (!ok) break;
                         tc_fence_after();
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 }
                 t += n;
                 // steps that only the other tile takes part in
-                for (int j = piece->steps[tile]; j < steps && ok; ++j) {
+                for (int j = (n + kHalves - 1) / kHalves; j < steps && ok; ++j) {
                     const uint32_t g = gs + j, stage = 8 * (g & 1);
                     ok = wait_warp(k_full + stage, (g >> 1) & 1, dead, 126) && wait_warp(v_full + stage, (g >> 1) & 1, dead, 121);
                     if (ok && lane == 0) {
@@ -634,9 +634,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                     for (int tile = 0; tile < 2; ++tile) {
                         const int rows = tile < C::TILES ? min(x.rows - 128 * tile, 128) : 0;
                         const int last = min(x.start + (x.r0 + 128 * tile + rows - 1) / p.group, p.kv.capacity - 1);
-                        x.steps[tile] = rows > 0 ? max(0, min(pieces.step1, last / kStepTokens + 1) - x.step0) : 0;
+                        x.halves[tile] = rows > 0 ? max(0, min(kHalves * pieces.step1, last / 64 + 1) - kHalves * x.step0) : 0;
                     }
-                    x.most = max(x.steps[0], x.steps[1]);
+                    x.most = (max(x.halves[0], x.halves[1]) + kHalves - 1) / kHalves;
                 }
                 if (lane == 0 && ok) s_piece[n_piece % kPieceQueue] = x;
                 arrive_warp(piece_full + 8 * (n_piece % kPieceQueue), lane);
