@@ -900,12 +900,12 @@ AttnPlan plan_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, 
     };
     // From 64 channels on, 256 (128) rows of a head at once on the 5th-generation tensor cores, where that is much work: those tiles multiply four times
     // as fast, but a call begins and joins slower, and a tile that is not full costs as much as a full one.  Measured (graph, us, tiles of 16 / prompt
-    // kernel; 128 channels, 8 heads, 4 rows of q a token): 16 tokens after 1000 8.8 / 25, 64 after 4000 39 / 38, 128 after 1000 27 / 35 and after 4000
-    // 64 / 40, 256 after none 28 / 18 and after 4000 117 / 47; 16 sequences of 32 tokens, 16 heads of their own (32 rows), after 1000 55 / 66 and after
-    // 4000 119 / 147, of 64 tokens 98 / 67 and 220 / 146.  256 channels, 2 heads: 64 tokens after 4000 22 / 47, 256 after 4000 67 / 59; 64 channels,
-    // 4 heads: 128 after 4000 27 / 32, 256 after 4000 44 / 35 (a row there costs tiles of 16 nearly what one of 128 does).
+    // kernel; 128 channels, 8 heads, 4 rows of q a token): 16 tokens after 1000 8.8 / 21, 64 after 1000 14 / 27 and after 4000 39 / 30, 128 after 1000
+    // 27 / 28 and after 4000 64 / 32, 256 after none 28 / 19 and after 4000 117 / 40; 16 sequences of 32 tokens, 16 heads of their own (32 rows), after
+    // 1000 55 / 62 and after 4000 119 / 147, of 64 tokens 98 / 63 and 220 / 147.  256 channels, 2 heads: 64 tokens after 4000 22 / 31, 128 after 4000
+    // 45 / 32; 64 channels, 4 heads: 128 after 4000 27 / 24, 256 after 4000 44 / 26 (a row there costs tiles of 16 nearly what one of 128 does).
     const long long every = most * rows->B * kv->n_kv;
-    if (D >= 64 && most > 32 && (every > 4096 || every * std::max(D, 128) > (1ll << 31) / ((long long)kv->max_pages * kv->page)))
+    if (D >= 64 && most > 32 && (every > 4096 || every * std::max(D, 128) > (1ll << 30) / ((long long)kv->max_pages * kv->page)))
         return D == 256 ? make(AttnKernel::prompt, 1, PromptShape<256>::Share{}) : make(AttnKernel::prompt, 1, PromptShape<128>::Share{});
     if (most > 8) return make(AttnKernel::rows16, 1, RowsShare<2>{});
     return make(AttnKernel::rows8, D == 256 ? 1 : 2, RowsShare<1>{});

@@ -317,12 +317,12 @@ __device__ __forceinline__ float rcp_fast(float x) {
     return y;
 }
 // Blocks of rows of paged_prompt_kernel (paged_prompt.cu): many rows a head.  Two tiles of 128 rows and steps of 128 tokens; with 256 channels one tile and
-// 64 tokens, which is what tensor memory and shared memory hold.  A segment's beginning and end count as two steps, the least share is six.  Measured (us,
-// shares rounded up to (extra, least) = (2, 4) / (2, 6) / (4, 8)): 16 heads, 512 tokens 26.8 / 23.0 / 23.1; 32 heads on 8, 256 tokens after 1000 34.9 /
-// 39.2 / 39.1, 1024 tokens 41.0 / 44.6 / 45.6; 32 on 4, 4096 tokens 209 / 211 / 214; not rounded up, (4, 8): 24.1, 44.5, 44.4, 217.
+// 64 tokens, which is what tensor memory and shared memory hold.  A segment's beginning and end count as two steps, the least share is four.
+// Measured (us, (extra, least) = (2, 4) / (2, 6) / (2, 3) / (1, 4)): 16 heads, 512 tokens 22.5 / 22.3 / 24.7 / 24.8; 32 heads on 8, 512 tokens 24.3 / 22.9 /
+// 27.8 / 25.2, 256 tokens after 1000 29.3 / 32.9 / 27.8 / 29.3, 1024 tokens 37.5 / 40.2 / 37.3 / 38.8; 32 on 4, 4096 tokens 180 / 178 / 179 / 212.
 template <int HD> struct PromptShape {
     static constexpr int TILES = HD == 256 ? 1 : 2, STEP = HD == 256 ? 64 : 128;
-    using Share = ShareOf<128 * TILES, STEP, 2, 6>;
+    using Share = ShareOf<128 * TILES, STEP, 2, 4>;
 };
 cudaError_t launch_paged_prompt(int head_dim, int dtype, const AttnParams& p, int grid, cudaStream_t st);
 
