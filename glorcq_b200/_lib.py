@@ -183,6 +183,7 @@ def native():
             raise RuntimeError("glorcq_b200/_native is missing or was built for another torch: build it with "
                                "`python -m glorcq_b200._build`") from e
         mod.bind({n: C.cast(getattr(L, n), vp).value for n in mod.names()})
+        mod.paged_bind({n: C.cast(getattr(L, n), vp).value for n in mod.paged_names()})
         _native = mod
     return _native
 

@@ -50,12 +50,15 @@ struct Api {
     GLQ_FN(glq_moe_workspace_bytes)                                                                                 \
     GLQ_FN(glq_moe_counters)                                                                                        \
     GLQ_FN(glq_moe_forward_ep)                                                                                      \
-    GLQ_FN(glq_add_rmsnorm)                                                                                         \
+    GLQ_FN(glq_add_rmsnorm)
+    GLQ_FNS
+// the cache in pages: a table of its own, so that either can be bound without the other
+#define GLQ_PAGED_FNS                                                                                               \
     GLQ_FN(glq_paged_append)                                                                                        \
     GLQ_FN(glq_paged_attention_workspace_bytes)                                                                     \
     GLQ_FN(glq_paged_attention)                                                                                     \
     GLQ_FN(glq_paged_read)
-    GLQ_FNS
+    GLQ_PAGED_FNS
 #undef GLQ_FN
 } api;
 
@@ -768,18 +771,20 @@ PyObject* py_paged_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-PyObject* py_bind(PyObject*, PyObject* d) {   // {entry point: address}
+// {entry point: address} for the entry points that names / paged_names lists
 #define GLQ_FN(name)                                                                              \
     if (PyObject* v = PyDict_GetItemString(d, #name)) api.name = reinterpret_cast<decltype(api.name)>(PyLong_AsVoidPtr(v)); \
     else return PyErr_Format(PyExc_RuntimeError, "the library has no entry point %s", #name);
+PyObject* py_bind(PyObject*, PyObject* d) {
     GLQ_FNS
-#undef GLQ_FN
     Py_RETURN_NONE;
 }
-PyObject* py_names(PyObject*, PyObject*) {
-#define GLQ_FN(name) #name,
-    const char* names[] = {GLQ_FNS};
+PyObject* py_paged_bind(PyObject*, PyObject* d) {
+    GLQ_PAGED_FNS
+    Py_RETURN_NONE;
+}
 #undef GLQ_FN
+PyObject* list_of(std::initializer_list<const char*> names) {
     PyObject* l = PyList_New(0);
     for (const char* s : names) {
         PyObject* u = PyUnicode_FromString(s);
@@ -788,12 +793,17 @@ PyObject* py_names(PyObject*, PyObject*) {
     }
     return l;
 }
+#define GLQ_FN(name) #name,
+PyObject* py_names(PyObject*, PyObject*) { return list_of({GLQ_FNS}); }
+PyObject* py_paged_names(PyObject*, PyObject*) { return list_of({GLQ_PAGED_FNS}); }
+#undef GLQ_FN
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(workspace), FAST(layer), FAST(linear), FAST(group), FAST(grouped_linear), FAST(turbo_matmul),
                          FAST(turbo_grouped_gemv), FAST(gptq_matmul), FAST(block), FAST(block_scratch), FAST(moe), FAST(add_rmsnorm),
                          FAST(paged_append), FAST(paged_attention), FAST(paged_read),
                          {"bind", py_bind, METH_O, nullptr}, {"names", py_names, METH_NOARGS, nullptr},
+                         {"paged_bind", py_paged_bind, METH_O, nullptr}, {"paged_names", py_paged_names, METH_NOARGS, nullptr},
                          {"clear_workspaces", py_clear_workspaces, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "glorcq_b200._native", nullptr, -1, methods};
 

@@ -432,6 +432,32 @@ def test_refusals(dev):
     torch.cuda.synchronize()
 
 
+def test_calls_run_without_the_interpreter_lock(dev):
+    """The library's entry points are replaced by PyGILState_Check: 0, a success, when the calling thread does not hold the interpreter lock, and by
+    Py_IsInitialized, which is 1, an unknown status."""
+    import ctypes as C
+    from glorcq_b200 import _lib
+    from glorcq_b200.paged_cache import paged_append, paged_attention, paged_read
+    cache = make_cache(1, "int8", 2, 64, 16, [20], dev)
+    q = torch.zeros(1, 4, 64, dtype=torch.float16, device=dev)
+    start = i64([19], dev)
+    calls = {"glq_paged_append": lambda: paged_append(None, q[:, :2], q[:, :2], None, None, *cache, start),
+             "glq_paged_attention": lambda: paged_attention(q, *cache, start), "glq_paged_read": lambda: paged_read(*cache, start, None, 1)}
+    nat = _lib.native()
+    real = {e: C.cast(getattr(_lib.lib(), e), C.c_void_p).value for e in nat.paged_names()}
+    assert set(real) == {*calls, "glq_paged_attention_workspace_bytes"} and not set(real) & set(nat.names())
+    probe, fails = (C.cast(f, C.c_void_p).value for f in (C.pythonapi.PyGILState_Check, C.pythonapi.Py_IsInitialized))
+    try:
+        for e, call in calls.items():
+            nat.paged_bind({**real, e: probe})
+            call()
+            nat.paged_bind({**real, e: fails})
+            with pytest.raises(RuntimeError):
+                call()
+    finally:
+        nat.paged_bind(real)
+
+
 def step(cache, q, k, v, cos, sin, start):
     from glorcq_b200.paged_cache import paged_append, paged_attention
     return paged_attention(paged_append(q, k, v, cos, sin, *cache, start), *cache, start)
