@@ -528,10 +528,10 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
 #pragma unroll
                 for (int n = 0; n < NB; ++n) mma16816(s[n], a0, a1, a2, a3, qf[n][w][0], qf[n][w][1]);
             }
-            const float c = ks * p.scale2, lv = vscale > 0.f ? log2_fast(vscale) : 0.f, iv = vscale > 0.f ? rcp_fast(vscale) : 1.f;
+            const bool there = page_there(p.kv, phys), masked = tile * 16 + 15 > limit_low || !there, live = there && live_scale(vscale);
+            const float c = ks * p.scale2, lv = live ? log2_fast(vscale) : 0.f, iv = live ? rcp_fast(vscale) : 1.f;
             // w of token g (+ 8) and rows 2t, 2t + 1 of each block of rows
             uint32_t pf[NB][2];
-            const bool there = page_there(p.kv, phys), masked = tile * 16 + 15 > limit_low || !there;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 const int tok = tile * 16 + g;
@@ -565,8 +565,8 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
                 for (int e = 0; e < 4; ++e) s[n][e] = exp2_fast(s[n][e] - m[n][e & 1]);
                 l[n][0] += (s[n][0] + s[n][2]) * iv;
                 l[n][1] += (s[n][1] + s[n][3]) * iv;
-                pf[n][0] = transpose8x8(vscale > 0.f ? pack_half2(s[n][0], s[n][1]) : 0u);
-                pf[n][1] = transpose8x8(vscale > 0.f ? pack_half2(s[n][2], s[n][3]) : 0u);
+                pf[n][0] = transpose8x8(live ? pack_half2(s[n][0], s[n][1]) : 0u);
+                pf[n][1] = transpose8x8(live ? pack_half2(s[n][2], s[n][3]) : 0u);
             }
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
@@ -929,7 +929,7 @@ extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_row
     const int bad = check_attention(kv, rows, n_heads);
     if (bad != GLQ_OK) return bad;
     if (rows->rows == 0 || rows->B == 0) return GLQ_OK;
-    if (!q || !out || !(scale >= 0.f) || ldq < (int64_t)n_heads * kv->head_dim || ldo < (int64_t)n_heads * kv->head_dim) return GLQ_ERR_ARG;
+    if (!q || !out || !(scale >= 0.f && scale <= FLT_MAX) || ldq < (int64_t)n_heads * kv->head_dim || ldo < (int64_t)n_heads * kv->head_dim) return GLQ_ERR_ARG;
     if (ldq % 8 || ldo % 8 || !aligned16(q) || !aligned16(out)) return GLQ_ERR_ALIGN;
     const AttnPlan plan = plan_attention(kv, rows, n_heads);
     if (!plan.fits) return GLQ_ERR_UNSUPPORTED;

@@ -316,6 +316,8 @@ __device__ __forceinline__ float rcp_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// A block's scale whose logarithm and reciprocal may be taken.  A block without one (0; also what nobody has written yet) has values that are zero.
+__device__ __forceinline__ bool live_scale(float s) { return s >= FLT_MIN && s <= FLT_MAX; }
 // Blocks of rows of paged_prompt_kernel (paged_prompt.cu): many rows a head.  Two tiles of 128 rows and steps of 128 tokens; with 256 channels one tile and
 // 64 tokens, which is what tensor memory and shared memory hold.  A segment's beginning and end count as two steps, the least share is four.
 // Measured (us, (extra, least) = (2, 4) / (2, 6) / (2, 3) / (1, 4)): 16 heads, 512 tokens 22.5 / 22.3 / 24.7 / 24.8; 32 heads on 8, 512 tokens 24.3 / 22.9 /

@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
 #pragma unroll 1
             for (; t < t0 + halves; ++t, first += 64) {
                 const uint32_t half = (t - t0) % kHalves, g = gs + (t - t0) / kHalves, bar = 16 * tile + 8 * (t & 1), s_at = s_tm + 64 * (t & 1);
-                ok = (half > 0 || wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121)) && wait_warp(s_full + bar, (t >> 1) & 1, dead, 120);
+                // (the scores first: a tile that had no part in many steps knows by them that V's stage is not two phases behind, which looks the same)
+                ok = wait_warp(s_full + bar, (t >> 1) & 1, dead, 120) && (half > 0 || wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t v[2][32];
@@ -536,15 +537,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 if (!(ok = wait_warp(v_empty + 8 * stage, parity, dead, 124))) break;
 #pragma unroll
                 for (int k = 0; k < G; ++k)
-                    if (!(vs[k] > 0.f))           // a block without a scale: its values are zero whatever its codes
+                    if (!live_scale(vs[k]))       // a block without a scale: its values are zero whatever its codes
 #pragma unroll
                         for (int u = 0; u < U; ++u) vc[k][u] = make_uint4(0u, 0u, 0u, 0u);
                 store(v_smem + stage * C::KV_TILE, vc);
 #pragma unroll
                 for (int k = 0; k < G; ++k)
                     if (lane == k)         // (a factor above zero: -3e38 times it hides a key)
-                        s_scale[stage][group0 + k] = make_float4(fmaxf(ks0[k] * p.scale2, 1e-30f), !page_there(p.kv, phys[k]) ? -INFINITY : vs[k] > 0.f ? log2_fast(vs[k]) : 0.f,
-                                                                 vs[k] > 0.f ? rcp_fast(vs[k]) : 1.f, 0.f);
+                        s_scale[stage][group0 + k] = make_float4(fmaxf(ks0[k] * p.scale2, 1e-30f), !page_there(p.kv, phys[k]) ? -INFINITY : live_scale(vs[k]) ? log2_fast(vs[k]) : 0.f,
+                                                                 live_scale(vs[k]) ? rcp_fast(vs[k]) : 1.f, 0.f);
                 fence_async_smem();
                 arrive_warp(v_full + 8 * stage, lane);
                 request(p.kv.v, p.kv.v_scale, step0 + j + 1, phys1, vc, vs);

@@ -31,7 +31,8 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_tab
 
     Sequence b holds ``start[b]`` tokens ((B,) or (1,) int64, on the device) and gets rows ``q_start[b] .. q_start[b + 1]`` ((B + 1,)
     int32; None: N / B each).  ``cos`` / ``sin`` ((positions, D / 2) fp32) may be None (no rotation), ``q_norm`` / ``k_norm`` ((D,) fp16) are the
-    weights of per-head RMS norms, ``q`` may be None (returns None), ``q_out`` may be q itself."""
+    weights of per-head RMS norms, ``q`` may be None (returns None), ``q_out`` may be q itself.  Rows of no sequence are not written.  A page that
+    the call writes belongs to one sequence."""
     return _lib.native().paged_append(q, k, v, cos, sin, k_pages, v_pages, k_scale, v_scale, page_table, start, q_start, q_norm, k_norm,
                                       eps, q_out)
 
@@ -47,7 +48,7 @@ def paged_attention(q, k_pages, v_pages, k_scale, v_scale, page_table, start, q_
 
 def paged_read(k_pages, v_pages, k_scale, v_scale, page_table, start, q_start, rows):
     """Keys and values (rows, kv heads, D) fp16 of positions ``start[b] ..`` of every sequence: rows ``q_start[b] .. q_start[b + 1]``
-    are sequence b's (None: rows / B each)."""
+    are sequence b's (None: rows / B each); rows of no sequence are not written."""
     return _lib.native().paged_read(k_pages, v_pages, k_scale, v_scale, page_table, start, q_start, rows)
 
 

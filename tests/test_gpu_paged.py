@@ -104,6 +104,25 @@ def test_attention_of_several_tokens(dev, dtype, heads, kv, D, P, held, new):
         assert torch.equal(got, paged_attention(q, *cache, i64(held, dev)))
 
 
+@pytest.mark.parametrize("dtype,D", [("e4m3", 128), ("int8", 64), ("int8", 256)])
+def test_blocks_with_one_tile_of_rows_and_with_two_in_turn(dev, dtype, D):
+    """Sequences whose last block of 256 rows has rows in its first tile alone, for many steps, and then blocks that have both: the results are
+    right and the same every time."""
+    from glorcq_b200.paged_cache import paged_attention
+    held, new = [700, 1500, 300, 900, 1300, 0], [40, 90, 31, 100, 20, 70]
+    cache = make_cache(D, dtype, 4, D, 16, [a + n for a, n in zip(held, new)], dev)
+    q = torch.randn(sum(new), 16, D, generator=torch.Generator().manual_seed(D)).half().to(dev)
+    want = paged_attention(q, *cache, i64(held, dev), q_starts(new, dev), max_new=max(new))
+    check_attention(want, cache, held, new, q)
+    many = 24                                        # the sequences again and again: every CTA has several blocks
+    table, q = cache[4].repeat(many, 1), q.repeat(many, 1, 1)
+    first = paged_attention(q, *cache[:4], table, i64(held * many, dev), q_starts(new * many, dev), max_new=max(new))
+    for _ in range(10):
+        assert torch.equal(first, paged_attention(q, *cache[:4], table, i64(held * many, dev), q_starts(new * many, dev), max_new=max(new)))
+    for i in (0, 7, many - 1):
+        check_attention(first[i * sum(new):(i + 1) * sum(new)], cache, held, new, q[:sum(new)])
+
+
 @pytest.mark.parametrize("heads,D,new", [(4, 128, 1), (2, 128, 150), (4, 64, 1), (4, 64, 70), (2, 256, 1), (2, 256, 30), (2, 256, 50)])
 def test_rows_of_no_sequence_are_left_as_they_were(dev, heads, D, new):
     from glorcq_b200.paged_cache import paged_attention
@@ -179,6 +198,47 @@ def test_scales_of_any_size(dev, new):
     q = torch.randn(new, 4, 64, generator=torch.Generator().manual_seed(4)).half().to(dev)
     for c in (cache, wide(cache, MUCH)):
         check_attention(paged_attention(q, *c, i64([96], dev)), cache, [96], [new], q)
+
+
+@pytest.mark.parametrize("dtype,D,new", [("int8", 128, 1), ("e4m3", 128, 12), ("int8", 128, 40), ("e4m3", 64, 40), ("int8", 256, 40), ("int8", 32, 20)])
+def test_what_lies_behind_the_tokens_does_not_matter(dev, dtype, D, new):
+    """Pages that are a sequence's already but hold nothing yet, and the slots behind its last token: any codes, any scales."""
+    from glorcq_b200.paged_cache import paged_attention
+    held = [21, 100]
+    clean = make_cache(6, dtype, 2, D, 16, [a + new for a in held], dev, width=16, pool=32)
+    q = torch.randn(2 * new, 4, D, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    dirty = [t.clone() for t in clean]
+    spare = [p for p in range(32) if p not in sum(clean[4].tolist(), [])]
+    for b, a in enumerate(held):
+        used = (a + new + 15) // 16
+        for j in range(used, min(used + 5, 16)):
+            dirty[4][b, j] = spare.pop()
+        if (a + new) % 16:
+            for t in dirty[:2]:
+                t.view(torch.uint8)[dirty[4][b, used - 1], :, (a + new) % 16:] = 0xff
+    for x in (float("nan"), float("inf"), -1.0, 1e-42, 1e30):
+        for p in range(32):
+            if p not in sum(clean[4].tolist(), []):
+                for t in dirty[:2]:
+                    t.view(torch.uint8)[p] = 0x7f
+                for t in dirty[2:4]:
+                    t[p] = x
+        for room in (0, 40000, MUCH):
+            a, b = ([*c[:4], wide(c, room)[4] if room else c[4]] for c in (clean, dirty))
+            assert torch.equal(paged_attention(q, *b, i64(held, dev)), paged_attention(q, *a, i64(held, dev))), (x, room)
+    check_attention(paged_attention(q, *dirty, i64(held, dev)), clean, held, [new] * 2, q)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_scale_of_zero_means_the_mean(dev, new):
+    from glorcq_b200.paged_cache import paged_attention
+    cache = make_cache(6, "int8", 2, 128, 16, [90 + new], dev)
+    q = torch.randn(new, 4, 128, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    for c in (cache, wide(cache, 40000), wide(cache, MUCH)):
+        check_attention(paged_attention(q, *c, i64([90], dev), scale=0.0), cache, [90], [new], q, scale=0.0)
+    for bad in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(RuntimeError):
+            paged_attention(q, *cache, i64([90], dev), scale=bad)
 
 
 @pytest.mark.parametrize("room", [0, 40000, MUCH])
@@ -427,6 +487,8 @@ def test_refusals(dev):
         paged_read(*cache, start, None, 3)
     with pytest.raises(RuntimeError):
         paged_read(*cache, start, None, -1)
+    with pytest.raises(RuntimeError, match="not supported"):             # rows times tokens beyond 32 bits
+        paged_attention(torch.zeros(1 << 16, 64, 64, device=dev).half(), *cache[:4], torch.full((2, 1 << 24), -1, dtype=torch.int32, device=dev), start)
     with pytest.raises(RuntimeError, match="multiple of the cache's heads"):
         paged_attention(torch.zeros(2, 3, 64, device=dev).half(), *cache, start)
     torch.cuda.synchronize()
