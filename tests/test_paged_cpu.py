@@ -68,6 +68,11 @@ def test_arguments_are_checked_on_the_host(L):
         assert attention(**bad) == -1, bad
     for bad in (dict(ldq=260), dict(ldo=260), dict(q=PTR + 8), dict(out=PTR + 8)):
         assert attention(**bad) == -2, bad
+    for scale in (-0.125, float("nan"), float("inf")):
+        assert L.glq_paged_attention(k, r, PTR, 256, PTR, 256, 4, scale, PTR, 1 << 40, None) == -1, scale
+    # rows times tokens that 32 bits do not count
+    many = descriptors(max_pages=1 << 25, table_stride=1 << 25, rows=1 << 20, max_new=1 << 20)
+    assert L.glq_paged_attention(C.byref(many[0]), C.byref(many[1]), PTR, 256, PTR, 256, 4, 0.125, PTR, 1 << 40, None) == -3
     ragged = descriptors(q_start=PTR, max_new=-1)[1]
     assert attention(r=C.byref(ragged)) == -1
     assert L.glq_paged_read(k, r, None, PTR, None) == L.glq_paged_read(k, r, PTR, None, None) == -1
