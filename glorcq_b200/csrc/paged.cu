@@ -12,7 +12,7 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // Append.  A block of a page and head is one CTA's: its scale needs the largest value of all new tokens before a code can be written.  Up to four rows a
 // lane stay in registers in between; of larger blocks the values are computed twice (the second time from the caches).  Two halves of a row that the
-// rotation mixes belong to one lane: lane c of HD / 16 has channels 8c .. 8c+7 and HD/2 + 8c .. .  Queries: a CTA a row, whose lanes use a
+// rotation mixes belong to one lane: lane c of HD / 16 has channels 8c .. 8c+7 and HD/2 + 8c .. .  Queries: a CTA a row or two, whose lanes use a
 // position's angles for all their heads.  Bound by memory: what counts is that a lane's loads are all requested before the first is used.
 // ---------------------------------------------------------------------------------------------
 constexpr int kAppendThreads = 128, kAppendCtas = 4;       // CTAs an SM: with five, registers spill
@@ -24,10 +24,10 @@ struct AppendParams {
     __half* q_out;
     const float *cos, *sin;
     long long ldq, ldk, ldv, ldqo;
-    int n_heads, page_items, cos_rows, query_rows, stride;       // (rows of queries that a CTA takes at once; every so many CTAs one has a block)
+    int n_heads, page_items, cos_rows, query_rows, query_turns, stride;       // (rows of queries that a CTA takes at once, how often; every so many CTAs one has a block)
     float eps;
 };
-constexpr int kAppendHeld = 4;
+constexpr int kAppendHeld = 4, kQueryTurns = 2;
 
 struct __align__(16) RowHalves {
     float a[8], b[8];      // first half's channels, second half's
@@ -98,48 +98,63 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kern
         widen8(*reinterpret_cast<const uint4*>(w + HD / 2 + 8 * c), weight.b);
     };
     if (!is_block) {                                    // queries
-        // one row, the heads of which go round the slots, or as many whole rows as there are slots for
-        const int row = work * p.query_rows + (p.query_rows > 1 ? slot / p.n_heads : 0);
+        // One row, the heads of which go round the slots, or as many whole rows as there are slots for; that again for `query_turns` of them, whose loads are
+        // requested together.
         const int first = p.query_rows > 1 ? slot % p.n_heads : slot;
-        const bool there = row < p.r.N && (p.query_rows == 1 || slot < p.query_rows * p.n_heads);
-        // row b is usually sequence b's where a sequence has one token
-        int b = min(there ? row : 0, rows.B - 1);
-        int2 own = rows_of(rows, b);
-        if (row < own.x || row - own.x >= own.y) {
-            b = last_from(rows.B, there ? row : 0, [&](int b) { return rows_from(rows, b); });
-            own = rows_of(rows, b);
-        }
-        // rows in front of the first sequence or behind the last are not touched
-        const bool mine = there && row >= own.x && row - own.x < own.y;
-        RowHalves cs = {};
-        if (mine && p.cos) {
-            const long long at = (long long)start_of(rows, b, p.kv.capacity) + (row - own.x);
-            load_angles<HD>(cs, p.cos, p.sin, (int)min(at, (long long)p.cos_rows - 1), c);
-        }
-        if (p.q_norm) load_weight(p.q_norm);
         const int rounds = p.query_rows > 1 ? 1 : (p.n_heads + RPP - 1) / RPP;       // (alike for all threads, who stay together for the norm's shuffles)
-        for (int k = 0; k < rounds; k += 2) {
-            uint4 raw[2][2];
+        if (p.q_norm) load_weight(p.q_norm);
+        int row[kQueryTurns];
+        bool mine[kQueryTurns];
+        RowHalves cs[kQueryTurns] = {};
+        uint4 raw[kQueryTurns][2][2];
+        auto request = [&](int t, int k) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int h = first + (k + u) * RPP;
-                const bool live = mine && k + u < rounds && h < p.n_heads;
-                const __half* src = p.q + row * p.ldq + h * HD + 8 * c;
-                raw[u][0] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
-                raw[u][1] = live ? *reinterpret_cast<const uint4*>(src + HD / 2) : make_uint4(0u, 0u, 0u, 0u);
+                const bool live = mine[t] && k + u < rounds && h < p.n_heads;
+                const __half* src = p.q + row[t] * p.ldq + h * HD + 8 * c;
+                raw[t][u][0] = live ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+                raw[t][u][1] = live ? *reinterpret_cast<const uint4*>(src + HD / 2) : make_uint4(0u, 0u, 0u, 0u);
             }
+        };
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int h = first + (k + u) * RPP;
-                RowHalves x;
-                widen8(raw[u][0], x.a);
-                widen8(raw[u][1], x.b);
-                if (p.q_norm) norm_row<HD>(x, weight, p.eps);
-                if (p.cos) rotate(x, cs);
-                if (mine && k + u < rounds && h < p.n_heads) {
-                    __half* dst = p.q_out + row * p.ldqo + h * HD + 8 * c;
-                    *reinterpret_cast<uint4*>(dst) = narrow8(x.a);
-                    *reinterpret_cast<uint4*>(dst + HD / 2) = narrow8(x.b);
+        for (int t = 0; t < kQueryTurns; ++t) {
+            if (t >= p.query_turns) break;
+            row[t] = (work * p.query_turns + t) * p.query_rows + (p.query_rows > 1 ? slot / p.n_heads : 0);
+            const bool there = row[t] < p.r.N && (p.query_rows == 1 || slot < p.query_rows * p.n_heads);
+            // row b is usually sequence b's where a sequence has one token
+            int b = min(there ? row[t] : 0, rows.B - 1);
+            int2 own = rows_of(rows, b);
+            if (row[t] < own.x || row[t] - own.x >= own.y) {
+                b = last_from(rows.B, there ? row[t] : 0, [&](int b) { return rows_from(rows, b); });
+                own = rows_of(rows, b);
+            }
+            // rows in front of the first sequence or behind the last are not touched
+            mine[t] = there && row[t] >= own.x && row[t] - own.x < own.y;
+            if (mine[t] && p.cos) {
+                const long long at = (long long)start_of(rows, b, p.kv.capacity) + (row[t] - own.x);
+                load_angles<HD>(cs[t], p.cos, p.sin, (int)min(at, (long long)p.cos_rows - 1), c);
+            }
+            request(t, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < kQueryTurns; ++t) {
+            if (t >= p.query_turns) break;
+            for (int k = 0; k < rounds; k += 2) {
+                if (k > 0) request(t, k);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int h = first + (k + u) * RPP;
+                    RowHalves x;
+                    widen8(raw[t][u][0], x.a);
+                    widen8(raw[t][u][1], x.b);
+                    if (p.q_norm) norm_row<HD>(x, weight, p.eps);
+                    if (p.cos) rotate(x, cs[t]);
+                    if (mine[t] && k + u < rounds && h < p.n_heads) {
+                        __half* dst = p.q_out + row[t] * p.ldqo + h * HD + 8 * c;
+                        *reinterpret_cast<uint4*>(dst) = narrow8(x.a);
+                        *reinterpret_cast<uint4*>(dst + HD / 2) = narrow8(x.b);
+                    }
                 }
             }
         }
@@ -827,10 +842,15 @@ extern "C" int glq_paged_append(const glq_paged_kv_t* kv, const glq_paged_rows_t
         constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
         AppendParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<const __half*>(k),
                        static_cast<const __half*>(v), static_cast<const __half*>(q_norm), static_cast<const __half*>(k_norm),
-                       static_cast<__half*>(q_out), cos, sin, ldq, ldk, ldv, ldqo, n_heads, 0, cos_rows, 1, 1, eps};
+                       static_cast<__half*>(q_out), cos, sin, ldq, ldk, ldv, ldqo, n_heads, 0, cos_rows, 1, 1, 1, eps};
         if (q) p.query_rows = std::max(1, kAppendThreads / (HD / 16) / n_heads);
+        // Two turns where the queries are several waves of CTAs: more loads are on their way.  Measured (graph, us, one / two): four sequences of 1024 tokens,
+        // 32 heads on 4, 25.4 / 21.0; 4096 tokens, 16 heads of their own 30.7 / 27.9, 8 on 2 of 256 channels 21.9 / 19.0, 32 on 8 23.8 / 23.7, with norms
+        // into e4m3 30.4 / 32.0; 512 tokens, 16 heads 5.7 / 5.8.
+        if (q && rows->rows / p.query_rows >= 2 * kAppendCtas * sm_count()) p.query_turns = kQueryTurns;
         const long long items = (long long)rows->rows / kv->page + 2ll * rows->B;
-        const long long grid = items * 2 * kv->n_kv + (q ? (rows->rows + p.query_rows - 1) / p.query_rows : 0);
+        const int query_rows = p.query_rows * p.query_turns;          // of a CTA
+        const long long grid = items * 2 * kv->n_kv + (q ? (rows->rows + query_rows - 1) / query_rows : 0);
         if (items * 2 * kv->n_kv > 0x3fffffffll || grid > 0x7fffffffll) return GLQ_ERR_UNSUPPORTED;
         p.page_items = (int)items;
         p.stride = (int)std::max<long long>(1, grid / (items * 2 * kv->n_kv));

@@ -396,6 +396,34 @@ def test_append_with_norms(dev, D):
     assert ((kk.cpu().double() - ref).abs() <= (0.5 + 2.0 ** -10) * step.double() + 2.0 ** -11 * ref.abs() + rel * size).all()
 
 
+@pytest.mark.parametrize("heads,D", [(17, 128), (5, 256), (3, 64), (32, 32)])
+def test_append_of_many_rows_turns_queries_as_of_few(dev, heads, D):
+    """A CTA takes more rows of queries where there are many: the same values as from calls of 300 rows each."""
+    from glorcq_b200.paged_cache import paged_append
+    n = 1250 * max(1, 128 // (D // 16) // heads) + 37
+    held, new = [3, 50], [n - 401, 401]
+    pages = [(a + m + 127) // 128 for a, m in zip(held, new)]
+    cache = make_cache(3, "int8", 1, D, 128, [0, 0], dev, width=max(pages), pool=sum(pages) + 1)
+    cache[4].fill_(-1)
+    cache[4][0, :pages[0]] = torch.arange(pages[0])
+    cache[4][1, :pages[1]] = torch.arange(pages[0], sum(pages))
+    cos, sin = tables(D, max(pages) * 128, dev)
+    g = torch.Generator().manual_seed(D)
+    q, k = (torch.randn(n + 5, h, D, generator=g).half().to(dev) for h in (heads, 1))
+    qw, kw = ((torch.rand(D, generator=g) + 0.5).half().to(dev) for _ in range(2))
+    for norms in ({}, dict(q_norm=qw, k_norm=kw)):
+        out = torch.full_like(q, 7.0)
+        paged_append(q, k, k, cos, sin, *cache, i64(held, dev), q_starts(new, dev, at=2), q_out=out, **norms)
+        assert (out[:2] == 7).all() and (out[2 + n:] == 7).all()
+        for b, first in ((0, 2), (1, 2 + new[0])):
+            for i in range(0, new[b], 300):
+                m = min(300, new[b] - i)
+                rows = slice(first + i, first + i + m)
+                one = [*cache[:4], cache[4][b:b + 1]]
+                got = paged_append(q[rows], k[rows], k[rows], cos, sin, *one, i64([held[b] + i], dev), **norms)
+                assert torch.equal(got, out[rows]), (b, i)
+
+
 def test_append_of_values_that_are_not_finite(dev):
     from glorcq_b200.paged_cache import paged_append
     for dtype in ("int8", "e4m3"):
