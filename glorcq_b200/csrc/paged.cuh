@@ -245,8 +245,12 @@ template <class S> struct Pieces {
         grain = sm.grain;
     }
     __device__ __forceinline__ bool next(const PagedKv& kv, const PagedRows& r, int group) {
+        return next(kv, r, group, [] {});
+    }
+    template <class F> __device__ __forceinline__ bool next(const PagedKv& kv, const PagedRows& r, int group, F&& looking) {      // looking(): at each block
         while (left > 0) {
             if (off >= block_units<S>(kv, x, grain)) {
+                looking();
                 ++i;
                 off = 0;
                 int b = x.b;

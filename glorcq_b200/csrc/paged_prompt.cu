@@ -20,7 +20,10 @@
 // The loops around it all are rolled: every warp of a scheduler runs another role's code, and what the instruction cache does not hold costs the
 // warps that issue the MMAs more than the MMAs (134 cycles an MMA with unrolled loops everywhere).
 //
-// Every wait is bounded (tc_wait); a wait that runs out marks the CTA dead, all roles leave their loops and the kernel ends.
+// Every wait is bounded; a wait that runs out marks the CTA dead, all roles leave their loops and the kernel ends.  What lasts a step at most has
+// tc_wait's 2 ms.  Three waits last as long as a piece of a segment or several (a place in the queue of pieces; the next piece; the scores of a tile
+// that had no rows in the pieces before), which behind 100000 tokens is more than that, and so may the search for a piece among thousands of sequences
+// without rows: their 2 ms begin anew with every step of the CTA and every block of rows that is looked at (wait_steps).
 #include "paged.cuh"
 #include "tc_mm.cuh"
 
@@ -58,6 +61,40 @@ template <int HD> struct PromptCfg {
 
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* dead, int code) {
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || tc_wait(bar, parity, dead, code));
+}
+// What moves while a CTA does (addresses in shared memory): the last step in either stage, the blocks of rows that warp 15 has looked at.
+struct Progress {
+    uint32_t step0, step1, looked;
+    static __device__ __forceinline__ uint32_t word(uint32_t a) {
+        uint32_t x;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(x) : "r"(a) : "memory");
+        return x;
+    }
+    __device__ __forceinline__ uint32_t now() const { return word(step0) + word(step1) + word(looked); }
+};
+// The same for what may last many steps.
+__device__ __forceinline__ bool wait_steps(uint32_t bar, uint32_t parity, volatile int* dead, int code, const Progress& progress) {
+    uint32_t seen = progress.now();
+    unsigned long long t0 = global_ns();
+    for (bool late = false;;) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*dead) return false;
+        const uint32_t now = progress.now();
+        if (now != seen) {
+            seen = now;
+            t0 = global_ns();
+            late = false;
+        } else if (late) {
+            glq_ok(false, code, bar, parity);
+            *dead = 1;
+            return false;
+        } else {
+            late = global_ns() - t0 > 2000000ull;
+        }
+    }
+}
+__device__ __forceinline__ bool wait_warp_steps(uint32_t bar, uint32_t parity, volatile int* dead, int code, const Progress& progress) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || wait_steps(bar, parity, dead, code, progress));
 }
 __device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, bool live) {       // not live: zeros, nothing is read
     const int bytes = live ? 16 : 0;
@@ -214,10 +251,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     extern __shared__ unsigned char prompt_smem[];
     __shared__ __align__(8) unsigned long long bars[26 + 2 * kPieceQueue];
     __shared__ PromptPiece s_piece[kPieceQueue];
-    __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs
+    __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs, number of the step
     __shared__ ShareStart sm_plan;
     __shared__ uint32_t s_tmem;
     __shared__ int s_dead;
+    __shared__ uint32_t s_looked;                      // blocks of rows that warp 15 has looked at
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = (smem_u32(prompt_smem) + 1023u) & ~1023u;
     const uint32_t q_smem = base, k_smem = base + C::TILES * C::Q_TILE, v_smem = k_smem + 2 * C::KV_TILE;
@@ -226,6 +264,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                    p_ready = k_full + 96, pv_done = k_full + 128, q_ready = k_full + 160, o_free = k_full + 176, q_free = k_full + 192,
                    piece_full = k_full + 208, piece_empty = piece_full + 8 * kPieceQueue;
     volatile int* dead = &s_dead;
+    const Progress progress{smem_u32(&s_scale[0][0].w), smem_u32(&s_scale[1][0].w), smem_u32(&s_looked)};
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + 8 * i, kPromptProducers);
@@ -246,6 +285,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             mbar_init(piece_empty + 8 * i, kPieceReaders);
         }
         s_dead = 0;
+        s_scale[0][0].w = s_scale[1][0].w = 0.f;
+        s_looked = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kPromptMma) tc_alloc(smem_u32(&s_tmem), 512);
@@ -265,7 +306,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     const PromptPiece* piece = s_piece;
     auto next_piece = [&]() {
         piece = s_piece + n_piece % kPieceQueue;
-        ok = wait_warp(piece_full + 8 * (n_piece % kPieceQueue), (n_piece / kPieceQueue) & 1, dead, 131);
+        ok = wait_warp_steps(piece_full + 8 * (n_piece % kPieceQueue), (n_piece / kPieceQueue) & 1, dead, 131, progress);
         return ok && piece->most >= 0;
     };
     auto done_piece = [&]() {
@@ -292,7 +333,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             for (; t < t0 + halves; ++t, first += 64) {
                 const uint32_t half = (t - t0) % kHalves, g = gs + (t - t0) / kHalves, bar = 16 * tile + 8 * (t & 1), s_at = s_tm + 64 * (t & 1);
                 // (the scores first: a tile that had no part in many steps knows by them that V's stage is not two phases behind, which looks the same)
-                ok = wait_warp(s_full + bar, (t >> 1) & 1, dead, 120) && (half > 0 || wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121));
+                ok = wait_warp_steps(s_full + bar, (t >> 1) & 1, dead, 120, progress) && (half > 0 || wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t v[2][32];
@@ -545,7 +586,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 for (int k = 0; k < G; ++k)
                     if (lane == k)         // (a factor above zero: -3e38 times it hides a key)
                         s_scale[stage][group0 + k] = make_float4(fmaxf(ks0[k] * p.scale2, 1e-30f), !page_there(p.kv, phys[k]) ? -INFINITY : live_scale(vs[k]) ? log2_fast(vs[k]) : 0.f,
-                                                                 live_scale(vs[k]) ? rcp_fast(vs[k]) : 1.f, 0.f);
+                                                                 live_scale(vs[k]) ? rcp_fast(vs[k]) : 1.f, __uint_as_float(g));
                 fence_async_smem();
                 arrive_warp(v_full + 8 * stage, lane);
                 request(p.kv.v, p.kv.v_scale, step0 + j + 1, phys1, vc, vs);
@@ -618,9 +659,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             }
         } else if (warp == kPromptMma + 3) {
             // ================= pieces =================
+            uint32_t looked = 0;
             for (bool more = true; more && ok; ++n_piece) {
-                ok = wait_warp(piece_empty + 8 * (n_piece % kPieceQueue), ((n_piece / kPieceQueue) & 1) ^ 1, dead, 132);
-                more = ok && pieces.next(p.kv, rows_q, p.group);
+                ok = wait_warp_steps(piece_empty + 8 * (n_piece % kPieceQueue), ((n_piece / kPieceQueue) & 1) ^ 1, dead, 132, progress);
+                more = ok && pieces.next(p.kv, rows_q, p.group, [&] {
+                    if (lane == 0) *const_cast<volatile uint32_t*>(&s_looked) = ++looked;
+                });
                 PromptPiece x{};
                 x.most = -1;
                 if (more) {

@@ -1,0 +1,110 @@
+"""The paged 8-bit cache where it is easily got wrong: prompts behind contexts that take long, blocks and rows of which little is left."""
+
+import pytest
+import torch
+
+from tests.paged_ref import TYPES
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available()
+    from glorcq_b200 import _build
+    _build.build()
+    return torch.device("cuda:0")
+
+
+def i64(v, dev):
+    return torch.tensor(v, dtype=torch.int64, device=dev)
+
+
+def q_starts(new, dev):
+    return torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device=dev)
+
+
+def long_cache(dtype, kv, D, P, tokens, dev):
+    """One sequence's `tokens` tokens in pages in random order: keys of about one in size, values of about one half."""
+    g = torch.Generator(device=dev).manual_seed(D + kv)
+    n = -(-tokens // P)
+    size = 80.0 if dtype == "int8" else 160.0
+    codes = [(torch.randn(n, kv, P, D, generator=g, device=dev) * size / 2.5).clamp(-size, size) for _ in range(2)]
+    codes = [(t.round() if dtype == "int8" else t).to(TYPES[dtype]) for t in codes]
+    scale = [(0.75 + 0.5 * torch.rand(n, kv, generator=g, device=dev)) * 2.5 / size * x for x in (1.0, 0.5)]
+    return [*codes, *scale, torch.randperm(n, generator=g, device=dev).to(torch.int32)[None]]
+
+
+def exact_rows(cache, b, held, q, rows):
+    """Attention in 64 bits of the rows `rows` of sequence b's q (n, heads, D), the first of which is at position `held`, and the bound of a kernel's
+    error: that of paged_ref.attention, and for as many tokens one rounding of 2^-23 of the sum so far for every 16 tokens that are added to it, which
+    counts for the sum of the values as for that of the weights."""
+    k_pages, v_pages, k_scale, v_scale, table = cache
+    D, heads, kv, P = q.shape[-1], q.shape[1], k_pages.shape[1], k_pages.shape[2]
+    pages = table[b].long()
+    total = min(held + len(q), len(pages) * P)
+    out, tol = (torch.zeros(len(rows), heads, D, dtype=torch.float64, device=q.device) for _ in range(2))
+    for h in range(kv):
+        k, v = ((t[pages, h].double() * s[pages, h].double()[:, None, None]).reshape(-1, D)[:total] for t, s in ((k_pages, k_scale), (v_pages, v_scale)))
+        vs = v_scale[pages, h].double().repeat_interleave(P)[:total]
+        for i, r in enumerate(rows):
+            n = min(held + r + 1, total)
+            x = q[r, h * heads // kv:(h + 1) * heads // kv].double()
+            p = torch.softmax(x @ k[:n].T * D ** -0.5, dim=1)
+            size = (x.abs() @ k[:n].abs().T).amax(dim=1) * D ** -0.5
+            rel = 2.0 ** -11 + 2 * ((D + 16) * 2.0 ** -23 * size + 2.0 ** -18) + 2 * n / 16 * 2.0 ** -23
+            y, mag = p @ v[:n], p @ v[:n].abs()
+            floor = 2.0 ** -25 * (p * vs[:n]).amax(dim=1)[:, None] * (v[:n] / vs[:n, None]).abs().sum(dim=0)
+            at = slice(h * heads // kv, (h + 1) * heads // kv)
+            out[i, at], tol[i, at] = y, 2.0 ** -11 * y.abs() + rel[:, None] * mag + floor + 2.0 ** -25
+    return out, tol
+
+
+def check_rows(got, cache, b, held, q, rows):
+    ref, tol = exact_rows(cache, b, held, q, rows)
+    err = (got[rows].double() - ref).abs()
+    assert (err <= tol).all(), f"sequence {b}: {(err / tol).max()} of the bound"
+    # (the rows tell their keys apart: a result that has missed some of them, or that nobody wrote, is not within the bound)
+    assert tol.max() < 0.2 * ref.abs().max()
+
+
+LONG = [  # dtype, heads, kv heads, D, sequences that share the pages, tokens held, new tokens of each
+    ("int8", 32, 8, 128, 1, 131072, 4096), ("e4m3", 16, 8, 256, 1, 65536, 4096), ("int8", 8, 8, 128, 50, 200000, 100), ("e4m3", 8, 8, 128, 20, 200000, 300)]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,D,batch,held,new", LONG)
+def test_prompts_behind_contexts_that_take_long(dev, dtype, heads, kv, D, batch, held, new):
+    """Pieces of the work that take milliseconds each: no wait for one of them runs out, and no row is left out.  (Many keys, few of which weigh: q is
+    large, so that the scores' deviation is 3.)"""
+    from glorcq_b200 import tiled
+    from glorcq_b200.paged_cache import paged_attention
+    cache = long_cache(dtype, kv, D, 128, held + new, dev)
+    cache[4] = cache[4].repeat(batch, 1)
+    q = (torch.randn(batch * new, heads, D, generator=torch.Generator(device=dev).manual_seed(1), device=dev) * 3).half()
+    out = torch.full_like(q, 7.0)
+    paged_attention(q, *cache, i64([held], dev), max_new=new, out=out)
+    torch.cuda.synchronize()
+    assert tiled.debug_error() is None
+    assert not (out == 7.0).all(dim=-1).any()
+    for b in {0, batch // 2, batch - 1}:
+        rows = sorted({0, 31, new // 2, new - 30, new - 1})
+        check_rows(out[b * new:(b + 1) * new], cache, b, held, q[b * new:(b + 1) * new], rows)
+
+
+def test_prompts_among_thousands_of_sequences_without_rows(dev):
+    """What finds a CTA's next rows looks at every sequence in between; who waits for it does not give up."""
+    from glorcq_b200 import tiled
+    from glorcq_b200.paged_cache import paged_attention
+    B, held = 8000, 1000
+    cache = long_cache("int8", 2, 128, 64, held + 40, dev)
+    cache[4] = cache[4].repeat(B, 1)
+    new = [0] * B
+    for b in (0, 1, 4000, B - 1):
+        new[b] = 40
+    q = (torch.randn(sum(new), 4, 128, generator=torch.Generator(device=dev).manual_seed(1), device=dev) * 3).half()
+    out = torch.full_like(q, 7.0)
+    paged_attention(q, *cache, i64([held], dev), q_starts(new, dev), max_new=40, out=out)
+    torch.cuda.synchronize()
+    assert tiled.debug_error() is None
+    for i in range(4):
+        check_rows(out[40 * i:40 * i + 40], cache, 0, held, q[40 * i:40 * i + 40], [0, 17, 39])
