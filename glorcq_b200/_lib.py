@@ -143,6 +143,7 @@ _SIGS = {
     "glq_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedKv), C.POINTER(PagedRows), C.c_int]),
     "glq_paged_attention": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedRows), vp, C.c_int64, vp, C.c_int64, C.c_int, C.c_float, vp,
                                       C.c_size_t, vp]),
+    "glq_paged_error": (C.c_int, [vp, C.c_int]),
     "glq_paged_read": (C.c_int, [C.POINTER(PagedKv), C.POINTER(PagedRows), vp, vp, vp]),
 }
 

@@ -1274,7 +1274,6 @@ extern "C" int glq_rht_forward(const void* x, int x_is_f32, int64_t ldx, const f
 }
 
 int glq_moe_error_words(unsigned long long* out4, int clear);   // moe.cu: the error word of that translation unit
-int glq_paged_error_words(unsigned long long* out4, int clear); // paged_prompt.cu
 
 // First bounds violation or timed-out wait recorded by a kernel: {code, index, limit, block<<32|thread};
 // all zero when there was none.  Synchronises the device.
@@ -1285,7 +1284,7 @@ extern "C" int glq_debug_error(unsigned long long* out4, int clear) {
         unsigned long long z[4] = {0, 0, 0, 0};
         GLQ_CUDA(cudaMemcpyToSymbol(g_glq_err, z, sizeof(z)));
     }
-    for (auto* words : {glq_moe_error_words, glq_paged_error_words}) {
+    for (auto* words : {glq_moe_error_words, glq_paged_error}) {
         unsigned long long m[4] = {0, 0, 0, 0};
         const int rc = words(m, clear);
         if (rc != GLQ_OK) return rc;

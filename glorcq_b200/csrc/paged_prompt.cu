@@ -28,7 +28,8 @@
 #include "tc_mm.cuh"
 
 // error word of this translation unit, merged by glq_debug_error
-int glq_paged_error_words(unsigned long long* out4, int clear) {
+extern "C" int glq_paged_error(unsigned long long* out4, int clear) {
+    if (!out4) return GLQ_ERR_ARG;
     if (cudaMemcpyFromSymbol(out4, glq::g_glq_err, 4 * sizeof(unsigned long long)) != cudaSuccess) return GLQ_ERR_CUDA;
     if (clear) {
         const unsigned long long z[4] = {0, 0, 0, 0};

@@ -145,6 +145,8 @@ class GLoRCQGraphWrapper:
         torch.cuda.synchronize()
         end = time.time()
         PeerExchange.check_all()      # expert parallel: a wait for another rank that ran out invalidates the tokens
+        if self.paged:
+            self.static_cache.raise_on_error()
         self.last_prefill_seconds, self.last_decode_seconds = prefill_end - start, end - prefill_end
         return output_ids, end - start
 

@@ -17,6 +17,8 @@ glq_paged_attention and glq_paged_read in include/glorcq_b200.h.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -147,6 +149,15 @@ class PagedKVCache:
         ids, values = kept
         for t, x in zip(self._tensors(), values):
             t[:, ids] = x
+
+    def raise_on_error(self):
+        """To be called where the host synchronises anyway (``GLoRCQGraphWrapper.generate`` does): raises where a wait in one of the cache's kernels
+        on this device has run out since the last look, which left rows of its call incomplete."""
+        word = (ctypes.c_ulonglong * 4)()
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.lib().glq_paged_error(word, 1), "paged_error")
+        if word[0]:
+            raise RuntimeError(f"paged cache: a wait ran out (code {word[0]}, thread {word[3] & 0xffffffff} of block {word[3] >> 32}); results since the last look may be incomplete")
 
     def _tensors(self):
         return self.k.view(torch.uint8), self.v.view(torch.uint8), self.k_scale, self.v_scale

@@ -488,6 +488,10 @@ int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, 
  * sequence b. */
 int glq_paged_read(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, void* k_out, void* v_out, void* stream);
 
+/* glq_debug_error of the paged cache's kernels alone (on the current device).  The kernel for many rows a head gives a wait up after 2 ms without
+ * progress, which is a fault of its own or of the machine: results of the call are then incomplete, and this word says so. */
+int glq_paged_error(unsigned long long* out4, int clear);
+
 #ifdef __cplusplus
 }
 #endif

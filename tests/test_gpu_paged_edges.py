@@ -108,3 +108,21 @@ def test_prompts_among_thousands_of_sequences_without_rows(dev):
     assert tiled.debug_error() is None
     for i in range(4):
         check_rows(out[40 * i:40 * i + 40], cache, 0, held, q[40 * i:40 * i + 40], [0, 17, 39])
+
+
+SMALL = dict(hidden_size=256, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, head_dim=64, vocab_size=512, num_experts=4,
+             num_experts_per_tok=4, moe_intermediate_size=128, norm_topk_prob=True, rms_norm_eps=1e-6, rope_theta=10000.0, max_position_embeddings=128)
+
+
+def test_generate_looks_for_waits_that_ran_out(dev, monkeypatch):
+    from glorcq_b200.graph_wrapper import GLoRCQGraphWrapper
+    from glorcq_b200.synthetic import make_decoder
+    w = GLoRCQGraphWrapper(make_decoder(SMALL, dev, seed=3, rank=16, attn_rank=16), max_batch_size=1, max_seq_len=64, kv_cache="int8", page_size=16)
+    ids = torch.arange(20, device=dev)[None]
+    w.generate(ids, max_new_tokens=4)                       # nothing is wrong: the word of this device is clear
+
+    def found():
+        raise RuntimeError("a wait ran out")
+    monkeypatch.setattr(w.static_cache, "raise_on_error", found)
+    with pytest.raises(RuntimeError, match="a wait ran out"):
+        w.generate(ids, max_new_tokens=4)
