@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<HD, NB>::CTAS) paged_att
                 for (int n = 0; n < NB; ++n) mma16816(s[n], a0, a1, a2, a3, qf[n][w][0], qf[n][w][1]);
             }
             const bool there = page_there(p.kv, phys), masked = tile * 16 + 15 > limit_low || !there, live = there && live_scale(vscale);
-            const float c = ks * p.scale2, lv = live ? log2_fast(vscale) : 0.f, iv = live ? rcp_fast(vscale) : 1.f;
+            const float c = ks * p.scale2, lv = scale_log(vscale), iv = scale_inverse(vscale);
             // w of token g (+ 8) and rows 2t, 2t + 1 of each block of rows
             uint32_t pf[NB][2];
 #pragma unroll

@@ -320,8 +320,15 @@ __device__ __forceinline__ float rcp_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// A block's scale whose logarithm and reciprocal may be taken.  A block without one (0; also what nobody has written yet) has values that are zero.
-__device__ __forceinline__ bool live_scale(float s) { return s >= FLT_MIN && s <= FLT_MAX; }
+// Scales of values.  A block whose scale is below kLeastScale (0 above all; also what nobody has written yet) has values that are zero: what it could add
+// to a result is below 448 kLeastScale, zero in fp16.  Its scores count in the sum of the softmax and must not set the maximum, relative to which
+// the other blocks' weights are rounded: they count as if its scale were kLeastScale, so that it raises the maximum only above scores that weigh 2^-60 of its own,
+// whose part of the result is zero in fp16 whatever the values.  (As if its scale were 1: values of 1e-4 beside a block of zeros off by 1 %.)
+constexpr float kLeastScaleLog = -60.f, kLeastScale = 0x1p-60f;
+__device__ __forceinline__ bool live_scale(float s) { return s >= kLeastScale && s <= FLT_MAX; }
+// log2 of a block's scale, and its reciprocal, as the softmax has them
+__device__ __forceinline__ float scale_log(float s) { return live_scale(s) ? log2_fast(s) : kLeastScaleLog; }
+__device__ __forceinline__ float scale_inverse(float s) { return live_scale(s) ? rcp_fast(s) : 1.f / kLeastScale; }
 // Blocks of rows of paged_prompt_kernel (paged_prompt.cu): many rows a head.  Two tiles of 128 rows and steps of 128 tokens; with 256 channels one tile and
 // 64 tokens, which is what tensor memory and shared memory hold.  A segment's beginning and end count as two steps, the least share is four.
 // Measured (us, (extra, least) = (2, 4) / (2, 6) / (2, 3) / (1, 4)): 16 heads, 512 tokens 22.5 / 22.3 / 24.7 / 24.8; 32 heads on 8, 512 tokens 24.3 / 22.9 /

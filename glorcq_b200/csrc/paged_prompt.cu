@@ -586,8 +586,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
 #pragma unroll
                 for (int k = 0; k < G; ++k)
                     if (lane == k)         // (a factor above zero: -3e38 times it hides a key)
-                        s_scale[stage][group0 + k] = make_float4(fmaxf(ks0[k] * p.scale2, 1e-30f), !page_there(p.kv, phys[k]) ? -INFINITY : live_scale(vs[k]) ? log2_fast(vs[k]) : 0.f,
-                                                                 live_scale(vs[k]) ? rcp_fast(vs[k]) : 1.f, __uint_as_float(g));
+                        s_scale[stage][group0 + k] = make_float4(fmaxf(ks0[k] * p.scale2, 1e-30f), page_there(p.kv, phys[k]) ? scale_log(vs[k]) : -INFINITY,
+                                                                 page_there(p.kv, phys[k]) ? scale_inverse(vs[k]) : 0.f, __uint_as_float(g));
                 fence_async_smem();
                 arrive_warp(v_full + 8 * stage, lane);
                 request(p.kv.v, p.kv.v_scale, step0 + j + 1, phys1, vc, vs);

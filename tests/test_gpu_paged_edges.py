@@ -3,7 +3,9 @@
 import pytest
 import torch
 
+from glorcq_b200.paged_cache import paged_attention
 from tests.paged_ref import TYPES
+from tests.test_gpu_paged import MUCH, i64, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -14,10 +16,6 @@ def dev():
     from glorcq_b200 import _build
     _build.build()
     return torch.device("cuda:0")
-
-
-def i64(v, dev):
-    return torch.tensor(v, dtype=torch.int64, device=dev)
 
 
 def q_starts(new, dev):
@@ -54,7 +52,8 @@ def exact_rows(cache, b, held, q, rows):
             size = (x.abs() @ k[:n].abs().T).amax(dim=1) * D ** -0.5
             rel = 2.0 ** -11 + 2 * ((D + 16) * 2.0 ** -23 * size + 2.0 ** -18) + 2 * n / 16 * 2.0 ** -23
             y, mag = p @ v[:n], p @ v[:n].abs()
-            floor = 2.0 ** -25 * (p * vs[:n]).amax(dim=1)[:, None] * (v[:n] / vs[:n, None]).abs().sum(dim=0)
+            codes = (v[:n] / torch.where(vs > 0, vs, torch.ones_like(vs))[:n, None]).abs()
+            floor = 2.0 ** -25 * (p * vs[:n]).amax(dim=1)[:, None] * codes.sum(dim=0)
             at = slice(h * heads // kv, (h + 1) * heads // kv)
             out[i, at], tol[i, at] = y, 2.0 ** -11 * y.abs() + rel[:, None] * mag + floor + 2.0 ** -25
     return out, tol
@@ -77,7 +76,6 @@ def test_prompts_behind_contexts_that_take_long(dev, dtype, heads, kv, D, batch,
     """Pieces of the work that take milliseconds each: no wait for one of them runs out, and no row is left out.  (Many keys, few of which weigh: q is
     large, so that the scores' deviation is 3.)"""
     from glorcq_b200 import tiled
-    from glorcq_b200.paged_cache import paged_attention
     cache = long_cache(dtype, kv, D, 128, held + new, dev)
     cache[4] = cache[4].repeat(batch, 1)
     q = (torch.randn(batch * new, heads, D, generator=torch.Generator(device=dev).manual_seed(1), device=dev) * 3).half()
@@ -94,7 +92,6 @@ def test_prompts_behind_contexts_that_take_long(dev, dtype, heads, kv, D, batch,
 def test_prompts_among_thousands_of_sequences_without_rows(dev):
     """What finds a CTA's next rows looks at every sequence in between; who waits for it does not give up."""
     from glorcq_b200 import tiled
-    from glorcq_b200.paged_cache import paged_attention
     B, held = 8000, 1000
     cache = long_cache("int8", 2, 128, 64, held + 40, dev)
     cache[4] = cache[4].repeat(B, 1)
@@ -126,3 +123,30 @@ def test_generate_looks_for_waits_that_ran_out(dev, monkeypatch):
     monkeypatch.setattr(w.static_cache, "raise_on_error", found)
     with pytest.raises(RuntimeError, match="a wait ran out"):
         w.generate(ids, max_new_tokens=4)
+
+
+# ---- blocks and rows of which little is left ------------------------------------------------------------------------------------
+
+ROOMS = (0, 40000, MUCH)
+
+
+@pytest.mark.parametrize("new", [1, 12, 40])
+@pytest.mark.parametrize("dtype,D", [("int8", 128), ("e4m3", 128), ("e4m3", 64), ("int8", 256), ("int8", 32)])
+@pytest.mark.parametrize("size", [1e-3, 1e-4])
+def test_values_of_zero_beside_small_ones_keep_the_others_bits(dev, dtype, D, size, new):
+    """Pages whose values are all zero (scale 0) take their part of the softmax and nothing else: values of 1e-3 and 1e-4 in the other pages, none larger,
+    come out as exactly as without them.  Sequences that share pages: as many as give every warp several tiles of 16 tokens."""
+    held, batch = 2000, 24
+    cache = long_cache(dtype, 2, D, 16, held + new, dev)
+    cache[3] *= 2 * size
+    empty = cache[4][0, torch.randperm(held // 16, generator=torch.Generator().manual_seed(D))[:30].to(dev)].long()
+    cache[3][empty] = 0.0
+    cache[1].view(torch.uint8)[empty] = 0
+    cache[4] = cache[4].repeat(batch, 1)
+    q = torch.randn(batch * new, 4, D, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    for room in ROOMS:
+        got = paged_attention(q, *(wide(cache, room) if room else cache), i64([held], dev))
+        for b in (0, batch - 1):
+            ref, tol = exact_rows(cache, b, held, q[b * new:(b + 1) * new], [0, new // 2, new - 1])
+            err = (got[[b * new, b * new + new // 2, b * new + new - 1]].double() - ref).abs()
+            assert (err <= tol).all(), (room, b, (err / tol).max())
