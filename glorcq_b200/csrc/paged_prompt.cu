@@ -15,7 +15,7 @@
 //   12, 13      issue the MMAs of tile 0 and 1 (one warp for both needed longer for it than the MMAs themselves)
 //   15          works out the CTA's pieces of segments and hands them to the others through a small queue
 // Scales and m as in paged_attention_rows_kernel: w = 2^(ks s + log2 vs - m) in fp16, the sum of w / vs in fp32, m raised only when a score exceeds it
-// by 2^8.  Keys that a row does not see get a score of -3e38, in the half steps that have such keys, and the common path has no masks.
+// by 2^8.  Keys that a row does not see get a score of -inf, in the half steps that have such keys, and the common path has no masks.
 //
 // The loops around it all are rolled: every warp of a scheduler runs another role's code, and what the instruction cache does not hold costs the
 // warps that issue the MMAs more than the MMAs (134 cycles an MMA with unrolled loops everywhere).
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 if (first + 63 > limit_low) {
 #pragma unroll
                     for (int i = 0; i < 64; ++i)
-                        if (first + i > limit) v[i / 32][i % 32] = __float_as_uint(-3e38f);
+                        if (first + i > limit) v[i / 32][i % 32] = __float_as_uint(-INFINITY);
                 }
                 float top = -INFINITY;
 #pragma unroll
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 store(v_smem + stage * C::KV_TILE, vc);
 #pragma unroll
                 for (int k = 0; k < G; ++k)
-                    if (lane == k)         // (a factor above zero: -3e38 times it hides a key)
+                    if (lane == k)         // (a factor above zero: -inf times it hides a key)
                         s_scale[stage][group0 + k] = make_float4(fmaxf(ks0[k] * p.scale2, 1e-30f), page_there(p.kv, phys[k]) ? scale_log(vs[k]) : -INFINITY,
                                                                  page_there(p.kv, phys[k]) ? scale_inverse(vs[k]) : 0.f, __uint_as_float(g));
                 fence_async_smem();

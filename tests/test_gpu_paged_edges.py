@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from glorcq_b200.paged_cache import paged_attention
-from tests.paged_ref import TYPES
+from tests.paged_ref import TYPES, make_cache
 from tests.test_gpu_paged import MUCH, i64, wide
 
 pytestmark = pytest.mark.gpu
@@ -150,3 +150,17 @@ def test_values_of_zero_beside_small_ones_keep_the_others_bits(dev, dtype, D, si
             ref, tol = exact_rows(cache, b, held, q[b * new:(b + 1) * new], [0, new // 2, new - 1])
             err = (got[[b * new, b * new + new // 2, b * new + new - 1]].double() - ref).abs()
             assert (err <= tol).all(), (room, b, (err / tol).max())
+
+def test_rows_that_see_no_key_are_zero_whatever_lies_behind_them(dev):
+    """The rows' own page is not there, and the one behind them has keys of zero or nearly: they are behind the rows all the same."""
+    for dtype, D in (("int8", 128), ("e4m3", 64), ("int8", 256)):
+        cache = make_cache(3, dtype, 1, D, 16, [100], dev)
+        q = torch.randn(16, 4, D, generator=torch.Generator().manual_seed(4)).half().to(dev)
+        first, second = int(cache[4][0, 0]), int(cache[4][0, 1])
+        cache[4][0, 0] = -1
+        for k_scale in (0.0, 1e-30, 1e-10, 1.0):
+            cache[2][second] = k_scale
+            for scale in (None, 0.0):
+                for room in ROOMS:
+                    c = wide(cache, room) if room else cache
+                    assert not paged_attention(q, *c, i64([0], dev), scale=scale).any(), (dtype, D, k_scale, scale, room)
