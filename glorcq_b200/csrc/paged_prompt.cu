@@ -43,8 +43,9 @@ namespace {
 
 constexpr int kPromptSoftmax = 8, kPromptProducers = 4, kPromptMma = kPromptSoftmax + kPromptProducers;
 constexpr int kPromptThreads = (kPromptMma + 4) * 32;
-// Registers of a thread: 128 at launch.  (168, 104 and 72 made the MMA warps reload what they had put away: 219 us where this split takes 183.)
-constexpr int kRegsSoftmax = 152, kRegsProducer = 128, kRegsMma = 80;
+// Registers of a thread: 128 at launch.  Measured (4096 tokens, 32 heads on 4, us): this split 180.7; 136, 120, 120 180; 144, 112, 112 181.2; 152, 128, 80 and
+// 152, 112, 96 and 144, 128, 96 182.7; 152, 120, 88 184.3.  (With too few the MMA warps reload what they had put away.)
+constexpr int kRegsSoftmax = 144, kRegsProducer = 120, kRegsMma = 104;
 static_assert((kPromptSoftmax * kRegsSoftmax + kPromptProducers * kRegsProducer + 4 * kRegsMma) * 32 <= kPromptThreads * 128, "registers");
 static_assert(kRegsSoftmax >= 128 && kRegsProducer <= 128 && kRegsMma <= 128, "the softmax takes what the others give");
 // every so many pairs of exponentials one is taken by exp2_poly
@@ -165,8 +166,13 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
 }
 template <int N> __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* v) {
-    static_assert(N == 16, "");
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+    static_assert(N == 8 || N == 16, "");
+    if constexpr (N == 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                     "r"(v[5]), "r"(v[6]), "r"(v[7])
+                     : "memory");
+    else
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
                  "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
                  "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
@@ -360,6 +366,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 }
                 if (__any_sync(0xffffffffu, top > m + 8.f)) {
                     const float up = fmaxf(m, top), f = exp2_fast(m - up);
+                    if (__any_sync(0xffffffffu, fabsf(up) > 0x1p20f && up > -1e30f)) break;
                     m = up;
                     l *= f;
                     if (t > t0) {         // the products so far, the last of which may be running
@@ -402,6 +409,66 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                     unpack2(sum2, a, b);
                     l += (a + b) * sc.z;
                     if (q % 2) tmem_st<16>(s_at + 16 * (q / 2), w);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                arrive_warp(p_ready + bar, lane);
+            }
+            // Scores that are very large.  Above, 2^(u ks + (log2 vs - m)) has u ks unrounded, and m, a rounded score, is off by up to 2^-24 of it: from
+            // 2^27 on the weights overflow fp16 or nothing is left of them.  Here a score is rounded as m was before m is taken from it.  (In the loop above the
+            // operations that this takes cost 6 of 180 us whether they are needed or not.)
+#pragma unroll 1
+            for (; ok && t < t0 + halves; ++t, first += 64) {
+                const uint32_t half = (t - t0) % kHalves, g = gs + (t - t0) / kHalves, bar = 16 * tile + 8 * (t & 1), s_at = s_tm + 64 * (t & 1);
+                ok = wait_warp(s_full + bar, (t >> 1) & 1, dead, 120) && (half > 0 || wait_warp(v_full + 8 * (g & 1), (g >> 1) & 1, dead, 121));
+                if (!ok) break;
+                tc_fence_after();
+                auto scores = [&](int q, float (&y)[16]) {          // returns 1 / vs
+                    uint32_t u[16];
+                    tc_ld16(s_at + 16 * q, u);
+                    tmem_arrived(u);
+                    const float4 sc = s_scale[g & 1][4 * half + q];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = first + 16 * q + i > limit ? -INFINITY : fmaf(__uint_as_float(u[i]), sc.x, sc.y);
+                    return sc.z;
+                };
+                float y[16], top = m;
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    scores(q, y);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, y[i]);
+                }
+                const float f = exp2_fast(m - top);
+                m = top;
+                l *= f;
+                if (t > t0 && __any_sync(0xffffffffu, f != 1.f)) {
+                    if (!(ok = wait_warp(pv_done + 16 * tile + 8 * ((t - 1) & 1), ((t - 1) >> 1) & 1, dead, 122))) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; ++c) {
+                        uint32_t x[16];
+                        tc_ld16(o_tm + 16 * c, x);
+                        tmem_arrived(x);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
+                        tmem_st<16>(o_tm + 16 * c, x);
+                    }
+                }
+                // P of 16 tokens takes the columns of 8 scores: those of tokens that have been read
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    const float inverse = scores(q, y);
+                    uint32_t w[8];
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float a = exp2_fast(y[2 * i] - m), b = exp2_fast(y[2 * i + 1] - m);
+                        sum += a + b;
+                        w[i] = pack_half2(a, b);
+                    }
+                    l += sum * inverse;
+                    tmem_st<8>(s_at + 8 * q, w);
                 }
                 tmem_st_wait();
                 tc_fence_before();

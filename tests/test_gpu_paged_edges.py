@@ -164,3 +164,66 @@ def test_rows_that_see_no_key_are_zero_whatever_lies_behind_them(dev):
                 for room in ROOMS:
                     c = wide(cache, room) if room else cache
                     assert not paged_attention(q, *c, i64([0], dev), scale=scale).any(), (dtype, D, k_scale, scale, room)
+
+
+def test_keys_behind_a_row_stay_hidden_however_low_its_scores_are(dev):
+    """Scores of -6e10, and behind the rows keys of zero, whose scores would be 0: the results are those without them.  (What the results are is not asked:
+    at 6e10 a score in fp32 is rounded by 2^-24 of it, 4000, and log2 of the values' scale, which is added to it, is lost.)"""
+    cache = make_cache(3, "int8", 1, 128, 16, [40], dev)
+    table = cache[4][0].tolist()
+    for p in table[:2]:
+        cache[0][p], cache[2][p] = -127, 500.0
+    cache[0][table[2]], cache[2][table[2]] = 0, 0.0
+    q = torch.full((32, 4, 128), 60000.0, dtype=torch.float16, device=dev)
+    for room in ROOMS:
+        c = wide(cache, room) if room else cache
+        without = [*c[:4], c[4].clone()]
+        without[4][0, 2] = -1
+        got = paged_attention(q, *c, i64([0], dev))
+        assert got.any() and torch.equal(got, paged_attention(q, *without, i64([0], dev))), room
+
+
+@pytest.mark.parametrize("new", [1, 12, 70])
+@pytest.mark.parametrize("dtype,D", [("int8", 128), ("e4m3", 64), ("int8", 256)])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e7, 3e8])
+def test_scores_so_large_that_one_key_takes_all(dev, dtype, D, size, new):
+    """Scores with a deviation of `size`: where the two largest are further apart than fp32 can be wrong about them (D + 16 roundings of 2^-23 of the sum of
+    magnitudes, for either) by 12 at least, which leaves the second 2^-17, the row is the largest one's value.  Its weight w is rounded to fp16 as the
+    product's operand and not in the sum, both of which have it relative to a maximum that may be up to 2^8 below: off by 2^-11 w / w, then by the
+    exponential's and the quotient's few roundings of 2^-22 (2^-18 together), and the result by its own rounding to fp16, 2^-11."""
+    held = 300
+    cache = long_cache(dtype, 1, D, 32, held + new, dev)
+    width = min(15000.0, size ** 0.5)
+    cache[2] *= size / width
+    q = (torch.randn(new, 4, D, generator=torch.Generator().manual_seed(4)).clamp(-4, 4) * width).half().to(dev)
+    page = cache[4][0].long()
+    k, v = ((t[page].double() * s[page].double()[:, :, None, None]).reshape(-1, D) for t, s in ((cache[0], cache[2]), (cache[1], cache[3])))
+    e = torch.einsum("nhd,td->nht", q.double(), k) * D ** -0.5
+    far = torch.einsum("nhd,td->nht", q.double().abs(), k.abs()).amax(dim=-1) * D ** -0.5 * (D + 16) * 2.0 ** -23 * 2 + 12
+    e = e.masked_fill(torch.arange(len(k), device=dev) > held + torch.arange(new, device=dev)[:, None, None], -torch.inf)
+    top = e.topk(2, dim=-1)
+    sure = top.values[..., 0] - top.values[..., 1] > far
+    assert sure.double().mean() > 0.8
+    want = v[top.indices[..., 0]]
+    # (what the second and all others add: 2^-17 of 400 values of one, at the very most; nothing at all from 1e6 on)
+    bound = (2 * 2.0 ** -11 + 2.0 ** -18) * want.abs() + 2.0 ** -25 + (2.0 ** -17 * 2 * v.abs().amax() if size < 1e6 else 0.0)
+    for room in ROOMS:
+        got = paged_attention(q, *(wide(cache, room) if room else cache), i64([held], dev))
+        assert got.isfinite().all() and ((got.double() - want).abs() <= bound)[sure].all(), room
+
+
+def test_keys_behind_a_row_stay_hidden_however_low_its_scores_are(dev):
+    """Scores of -6e10, and behind the rows keys of zero, whose scores would be 0: the results are those without them.  (What the results are is not asked:
+    at 6e10 a score in fp32 is rounded by 2^-24 of it, 4000, and log2 of the values' scale, which is added to it, is lost.)"""
+    cache = make_cache(3, "int8", 1, 128, 16, [40], dev)
+    table = cache[4][0].tolist()
+    for p in table[:2]:
+        cache[0][p], cache[2][p] = -127, 500.0
+    cache[0][table[2]], cache[2][table[2]] = 0, 0.0
+    q = torch.full((32, 4, 128), 60000.0, dtype=torch.float16, device=dev)
+    for room in ROOMS:
+        c = wide(cache, room) if room else cache
+        without = [*c[:4], c[4].clone()]
+        without[4][0, 2] = -1
+        got = paged_attention(q, *c, i64([0], dev))
+        assert got.any() and torch.equal(got, paged_attention(q, *without, i64([0], dev))), room
