@@ -648,6 +648,7 @@ PagedCall paged_call(PyObject* const* a, int64_t n_rows, int64_t max_new) {
     const at::Tensor& start = beside(a[5], "start", at::kLong, "torch.int64", kp);
     const at::Tensor* qs = a[6] == Py_None ? nullptr : &beside(a[6], "q_start", at::kInt, "torch.int32", kp);
     const int64_t B = table.size(0), pages = kp.size(0), heads = kp.size(1);
+    if (heads < 1) fail("k_pages must have one head or more");
     if (vpg.sizes() != kp.sizes()) fail("k_pages and v_pages must have one shape");
     if (ks.dim() != 2 || ks.size(0) != pages || ks.size(1) != heads || vs.sizes() != ks.sizes()) fail("k_scale and v_scale must be (pages, heads)");
     if (start.dim() != 1 || (start.size(0) != 1 && start.size(0) != B)) fail("start must have one value, or one for each sequence");

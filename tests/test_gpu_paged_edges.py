@@ -227,3 +227,17 @@ def test_keys_behind_a_row_stay_hidden_however_low_its_scores_are(dev):
         without[4][0, 2] = -1
         got = paged_attention(q, *c, i64([0], dev))
         assert got.any() and torch.equal(got, paged_attention(q, *without, i64([0], dev))), room
+
+
+# ---- host side -------------------------------------------------------------------------------------------------------------------
+
+def test_a_cache_without_heads_is_refused(dev):
+    from glorcq_b200.paged_cache import paged_append, paged_read
+    cache = [torch.zeros(4, 0, 16, 64, dtype=torch.int8, device=dev) for _ in range(2)] + [torch.zeros(4, 0, device=dev) for _ in range(2)] + \
+            [torch.zeros(1, 4, dtype=torch.int32, device=dev)]
+    for n in (0, 1):
+        q, k = torch.zeros(n, 4, 64, device=dev).half(), torch.zeros(n, 0, 64, device=dev).half()
+        for call in (lambda: paged_attention(q, *cache, i64([0], dev)), lambda: paged_append(q, k, k, None, None, *cache, i64([0], dev)),
+                     lambda: paged_read(*cache, i64([0], dev), None, n)):
+            with pytest.raises(RuntimeError, match="one head or more"):
+                call()
