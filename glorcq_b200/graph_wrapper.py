@@ -64,7 +64,8 @@ class GLoRCQGraphWrapper:
 
     def capture_graph(self):
         """Allocation pass, three warm-up steps on a side stream, then the recorded step
-        (inference/graph_wrapper.py:69-130)."""
+        (inference/graph_wrapper.py:69-130).  These steps are at positions 0 and 10 of the cache, which is left as it was."""
+        kept = self.static_cache.snapshot(11)
         self.model.eval()
         self._set_moe_graph_mode(True)
         with torch.no_grad():
@@ -93,6 +94,7 @@ class GLoRCQGraphWrapper:
         # the model's output projection may leave the greedy token of the step beside the logits
         best = getattr(self.model, "last_argmax", None)
         self.static_next = best.view(self.max_batch_size, 1) if best is not None else None
+        self.static_cache.restore(kept)
 
     @torch.no_grad()
     def replay(self, input_ids, cache_position_val):
@@ -126,10 +128,7 @@ class GLoRCQGraphWrapper:
         prefill_end = time.time()
         self._set_moe_graph_mode(True)
         if self.graph is None:
-            # capturing runs steps at positions 0 and 10 of the static cache: keep the prompt's entries
-            kept = self.static_cache.snapshot(11)
             self.capture_graph()
-            self.static_cache.restore(kept)
             torch.cuda.synchronize()
             prefill_end = time.time()
         for i in range(max_new_tokens - 1):

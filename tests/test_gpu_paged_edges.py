@@ -241,3 +241,26 @@ def test_a_cache_without_heads_is_refused(dev):
                      lambda: paged_read(*cache, i64([0], dev), None, n)):
             with pytest.raises(RuntimeError, match="one head or more"):
                 call()
+
+
+@pytest.mark.parametrize("kv_cache", ["static", "int8", "e4m3"])
+def test_capturing_a_step_leaves_the_cache_as_it_was(dev, kv_cache):
+    """A prompt in the cache, then capture_graph(): its warm-up steps write positions 0 and 10, the first of which gives a block a new scale."""
+    from glorcq_b200.graph_wrapper import GLoRCQGraphWrapper
+    from glorcq_b200.synthetic import make_decoder
+    m = make_decoder(SMALL, dev, seed=3, rank=16, attn_rank=16)
+    w = GLoRCQGraphWrapper(m, max_batch_size=2, max_seq_len=64, kv_cache=kv_cache, page_size=16)
+    ids = torch.randint(0, 512, (2, 30), generator=torch.Generator().manual_seed(1)).to(dev)
+    with torch.no_grad():
+        m(input_ids=ids, cache_position=torch.arange(30, device=dev), past_key_values=w.static_cache)
+        c = w.static_cache
+        tensors = [c.k, c.v] if kv_cache == "static" else [c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scale, c.v_scale]
+        before = [t.clone() for t in tensors]
+        w.capture_graph()
+        assert all(torch.equal(a, b) for a, b in zip(tensors, before))
+        # and the captured step reads that prompt
+        got = w.replay(ids[:, :1], 30).clone()
+        for t, x in zip(tensors, before):
+            t.copy_(x)
+        want = m(input_ids=ids[:, :1], cache_position=torch.tensor([30], device=dev), past_key_values=c)[0]
+        assert torch.equal(got, want)
