@@ -142,7 +142,7 @@ class PagedKVCache:
     def snapshot(self, n):
         """What the first ``n`` positions of every sequence hold, for ``restore``."""
         ids = self.page_table[:, : -(-n // self.page_size)].reshape(-1).long()
-        ids = ids[ids >= 0]
+        ids = ids[(ids >= 0) & (ids < self.k.shape[1])]       # (what is no page is nobody's)
         return ids, [t[:, ids].clone() for t in self._tensors()]
 
     def restore(self, kept):
