@@ -3,8 +3,8 @@
 // A page holds `page` tokens of every key/value head as codes (heads, tokens, channels) and one fp32 scale per (page, head) for
 // the keys and one for the values: value = code * scale.  Sequence b holds start[b] tokens before a call and owns rows
 // q_start[b] .. q_start[b + 1] of the call's batch; logical page j of it is physical page table[b][j].  Numbers from device
-// memory are never trusted with an address: q_start is cut to the rows there are, start to the table's capacity, and a page id outside
-// the pool is a page that is not there (nothing is written to it, its tokens are hidden, it reads as zeros).
+// memory are never trusted with an address, nor with the end of a loop: q_start is cut to the rows there are, start to the table's capacity, and a page id
+// outside the pool is a page that is not there (nothing is written to it, its tokens are hidden, it reads as zeros).
 //
 // All of it may have been written by the launch ahead, beside which these kernels start: plain loads behind griddepcontrol.wait, and
 // dependent launches are let go behind it too.
@@ -251,7 +251,8 @@ template <class S> struct Pieces {
         while (left > 0) {
             if (off >= block_units<S>(kv, x, grain)) {
                 looking();
-                ++i;
+                // (where q_start decreases, which it must not, these blocks may not be those that were counted: the list has an end all the same)
+                if (++i >= block_count<S>(r.N, r.B, group)) left = 0;
                 off = 0;
                 int b = x.b;
                 while (b + 1 < r.B && first_block<S>(r, group, b + 1) <= i) ++b;

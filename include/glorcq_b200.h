@@ -440,7 +440,8 @@ int glq_lm_head_rows(const void* x, int64_t ldx, const void* W, int B, int V, in
  * be shared by sequences that only read them; a page that a call writes belongs to one sequence.
  *
  * Rows of a call: sequence b holds start[b * start_stride] tokens before the call (start_stride 0: the same for all) and has
- * rows q_start[b] .. q_start[b + 1] - 1 of the batch, at positions start, start + 1, ...; q_start NULL: rows / B each.
+ * rows q_start[b] .. q_start[b + 1] - 1 of the batch, at positions start, start + 1, ...; q_start NULL: rows / B each; q_start must not
+ * decrease (where it does, what the call leaves in its rows and in the sequences' pages is not defined).
  * max_new: at least the most rows of one sequence (host; with q_start NULL not read).  Rows in front of q_start[0] or behind q_start[B] are left as they
  * are.  A start below zero counts as zero, one above max_pages * page as that; tokens past it are not stored and see all that is.
  * start, q_start and table are read on the device when the call runs, so that captured calls follow them.

@@ -264,3 +264,32 @@ def test_capturing_a_step_leaves_the_cache_as_it_was(dev, kv_cache):
             t.copy_(x)
         want = m(input_ids=ids[:, :1], cache_position=torch.tensor([30], device=dev), past_key_values=c)[0]
         assert torch.equal(got, want)
+
+
+def test_numbers_of_rows_that_go_back_and_forth_end_the_call(dev):
+    """q_start must not decrease, and lies on the device: a call that is given such numbers ends, and writes nothing outside its rows and its pages."""
+    import random
+    from glorcq_b200 import tiled
+    from glorcq_b200.paged_cache import paged_append, paged_read
+    r = random.Random(1)
+    cache = long_cache("int8", 2, 128, 16, 640, dev)
+    spare = cache[0].shape[0]
+    cache = [torch.cat((t, t[:1])) for t in cache[:4]] + [cache[4]]
+    kept = [t[spare].clone() for t in cache[:4]]
+    for n in range(60):
+        B, N = r.choice([2, 9, 30, 700]), r.choice([20, 100, 400])
+        qs = torch.tensor([r.randint(-5, N + 5) for _ in range(B + 1)], dtype=torch.int32, device=dev)
+        table = cache[4].repeat(B, 1)
+        start = i64([r.randint(0, 600) for _ in range(B)], dev)
+        q = torch.randn(N, 4, 128, device=dev).half()
+        for room in ROOMS[:2 if B > 100 else 3]:
+            out = torch.full((N + 20, 4, 128), 7.0, dtype=torch.float16, device=dev)
+            c = [*cache[:4], table]
+            paged_attention(q, *(wide(c, room) if room else c), start, qs, max_new=r.choice([None, N]), out=out[10:-10])
+            assert (out[:10] == 7).all() and (out[-10:] == 7).all()
+        out = torch.full((N + 20, 4, 128), 7.0, dtype=torch.float16, device=dev)
+        paged_append(q, q[:, :2], q[:, 2:], None, None, *c, start, qs, q_out=out[10:-10])
+        assert (out[:10] == 7).all() and (out[-10:] == 7).all()
+        paged_read(*c, start, qs, N)
+    assert all(torch.equal(t[spare].view(torch.uint8), k.view(torch.uint8)) for t, k in zip(cache[:4], kept))
+    assert tiled.debug_error() is None
