@@ -960,7 +960,7 @@ extern "C" int glq_paged_attention(const glq_paged_kv_t* kv, const glq_paged_row
     return by_type(kv, [&](auto hd, auto dt) {
         constexpr int HD = decltype(hd)::value, DT = decltype(dt)::value;
         const int group = n_heads / kv->n_kv;
-        const AttnParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<__half*>(out), ldq, ldo, n_heads,
+        const AttnParams p{device_kv(kv), device_rows(rows), static_cast<const __half*>(q), static_cast<__half*>(out), ldq, ldo,
                            group, scale * 1.4426950408889634f * kCodeUnit<DT>, static_cast<JoinItem*>(workspace),
                            reinterpret_cast<float*>(static_cast<JoinItem*>(workspace) + plan.grid)};
         auto join = [&](auto share) {

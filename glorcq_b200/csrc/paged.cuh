@@ -301,7 +301,7 @@ struct AttnParams {
     const __half* q;
     __half* out;
     long long ldq, ldo;
-    int n_heads, group;
+    int group;
     float scale2;           // softmax scale * log2(e) * kCodeUnit
     JoinItem* join;         // an item for each CTA, then
     float* partial;         // two partial results for each
