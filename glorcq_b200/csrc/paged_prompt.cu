@@ -20,7 +20,8 @@
 // The loops around it all are rolled: every warp of a scheduler runs another role's code, and what the instruction cache does not hold costs the
 // warps that issue the MMAs more than the MMAs (134 cycles an MMA with unrolled loops everywhere).
 //
-// Every wait is bounded; a wait that runs out marks the CTA dead, all roles leave their loops and the kernel ends.  What lasts a step at most has
+// Every wait is bounded; a wait that runs out marks the CTA dead, all roles leave their loops, wait (2 ms again) for copies and MMAs that they have under way,
+// and the kernel ends.  What lasts a step at most has
 // tc_wait's 2 ms.  Three waits last as long as a piece of a segment or several (a place in the queue of pieces; the next piece; the scores of a tile
 // that had no rows in the pieces before), which behind 100000 tokens is more than that, and so may the search for a piece among thousands of sequences
 // without rows: their 2 ms begin anew with every step of the CTA and every block of rows that is looked at (wait_steps).
@@ -97,6 +98,11 @@ __device__ __forceinline__ bool wait_steps(uint32_t bar, uint32_t parity, volati
 }
 __device__ __forceinline__ bool wait_warp_steps(uint32_t bar, uint32_t parity, volatile int* dead, int code, const Progress& progress) {
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || wait_steps(bar, parity, dead, code, progress));
+}
+// At the end of a CTA that is dead: for what is under way, 2 ms at most.
+__device__ __forceinline__ void wait_at_the_end(uint32_t bar) {
+    for (const unsigned long long t0 = global_ns(); !mbar_try_wait(bar, 0) && global_ns() - t0 < 2000000ull;) {
+    }
 }
 __device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, bool live) {       // not live: zeros, nothing is read
     const int bytes = live ? 16 : 0;
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     using Share = typename C::Share;
     constexpr int kStepTokens = C::STEP, kGroups = C::GROUPS, kHalves = kStepTokens / 64;
     extern __shared__ unsigned char prompt_smem[];
-    __shared__ __align__(8) unsigned long long bars[26 + 2 * kPieceQueue];
+    __shared__ __align__(8) unsigned long long bars[28 + 2 * kPieceQueue];
     __shared__ PromptPiece s_piece[kPieceQueue];
     __shared__ float4 s_scale[2][kGroups];             // of a stage's groups of 16 tokens: factor of the scores, log2 vs, 1 / vs, number of the step
     __shared__ ShareStart sm_plan;
@@ -269,7 +275,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
     // [0], [1] of each: stages or tiles; of s_full, p_ready and pv_done four: [tile][place of the scores]
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_full + 32, v_empty = k_full + 48, s_full = k_full + 64,
                    p_ready = k_full + 96, pv_done = k_full + 128, q_ready = k_full + 160, o_free = k_full + 176, q_free = k_full + 192,
-                   piece_full = k_full + 208, piece_empty = piece_full + 8 * kPieceQueue;
+                   piece_full = k_full + 208, piece_empty = piece_full + 8 * kPieceQueue, mma_end = piece_empty + 8 * kPieceQueue;
     volatile int* dead = &s_dead;
     const Progress progress{smem_u32(&s_scale[0][0].w), smem_u32(&s_scale[1][0].w), smem_u32(&s_looked)};
     if (threadIdx.x == 0) {
@@ -281,6 +287,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             mbar_init(q_ready + 8 * i, kPromptProducers);
             mbar_init(q_free + 8 * i, 1);
             mbar_init(o_free + 8 * i, 4);
+            mbar_init(mma_end + 8 * i, 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(s_full + 8 * i, 1);
@@ -668,6 +675,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
             if (!ok) break;
             done_piece();
         }
+        if (!ok) asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMma));
         if (warp < kPromptMma + 2) {
@@ -724,6 +732,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged_prompt_kernel(const A
                 gs += steps;
                 had += n > 0;
                 done_piece();
+            }
+            if (!ok) {
+                commit_warp(mma_end + 8 * tile);
+                wait_at_the_end(mma_end + 8 * tile);
             }
         } else if (warp == kPromptMma + 3) {
             // ================= pieces =================
