@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const ReadPara
 //           interleaved, then expanded.
 //   P       movmatrix transposes the scores' fragment (tokens by g) into the second product's (tokens by t).
 // Scales: c = ks * scale * log2(e) multiplies a score; vs goes into the exponent, w = 2^(c s + log2 vs - m), so that probabilities are rounded
-// to fp16 relative to the largest contribution; the sum of the softmax is that of w / vs in fp32.  The maximum m is raised only when a score
+// to fp16 (the product's operand) relative to the largest contribution, which takes the results' error from 2.1e-4, their own rounding, to 2.4e-4 .. 2.9e-4
+// (w in two halves, products of both: 2.1e-4 and 2 to 5 % of the time); the sum of the softmax is that of w / vs in fp32.  The maximum m is raised only when a score
 // exceeds it by 2^8 (w stays below 256 in fp16), by a vote, so that a step has no shuffles as a rule.
 // ---------------------------------------------------------------------------------------------
 constexpr int kRowsWarps = 8, kRowsThreads = kRowsWarps * 32;
@@ -845,8 +846,9 @@ extern "C" int glq_paged_append(const glq_paged_kv_t* kv, const glq_paged_rows_t
                        static_cast<__half*>(q_out), cos, sin, ldq, ldk, ldv, ldqo, n_heads, 0, cos_rows, 1, 1, 1, eps};
         if (q) p.query_rows = std::max(1, kAppendThreads / (HD / 16) / n_heads);
         // Two turns where the queries are several waves of CTAs: more loads are on their way.  Measured (graph, us, one / two): four sequences of 1024 tokens,
-        // 32 heads on 4, 25.4 / 21.0; 4096 tokens, 16 heads of their own 30.7 / 27.9, 8 on 2 of 256 channels 21.9 / 19.0, 32 on 8 23.8 / 23.7, with norms
-        // into e4m3 30.4 / 32.0; 512 tokens, 16 heads 5.7 / 5.8.
+        // 32 heads on 4, 25.4 / 21.0; 4096 tokens, 16 heads of their own 30.7 / 27.9, 8 on 2 of 256 channels 21.9 / 19.0, 32 on 8 23.8 / 23.7; 512 tokens,
+        // 16 heads 5.7 / 5.8.  With norms: four of 1024, 32 on 4, 21.6 / 19.1; 4096 tokens, 16 heads 35.6 / 28.5, 8 on 2 of 256 22.5 / 20.1, 32 on 8 26.1 / 26.2
+        // and into e4m3 30.8 / 30.8; 64 of 128 tokens, 32 on 4, into e4m3 50.5 / 46.2.
         if (q && rows->rows / p.query_rows >= 2 * kAppendCtas * sm_count()) p.query_turns = kQueryTurns;
         const long long items = (long long)rows->rows / kv->page + 2ll * rows->B;
         const int query_rows = p.query_rows * p.query_turns;          // of a CTA

@@ -64,7 +64,9 @@ def rope_tables(head_dim, positions, theta, device):
 class PagedKVCache:
     """Pages of all layers of a model, and who has which.
 
-    ``dtype``: "int8" (an error of at most half of a block's largest magnitude / 127) or "e4m3" (a relative error of at most 2^-4).
+    ``dtype``: "int8" or "e4m3".  The error of a value, by the scale s of its block (one head's tokens of a page): below s with "int8", at most
+    s / 2 where one call wrote the whole block; at most 2^-4 of the value and 2^-9 s with "e4m3".  s is the block's largest magnitude / 127 (448) where one call
+    wrote it, and below twice that where tokens came one by one and its scale was doubled on the way.
     ``num_pages`` None: pages for every sequence's ``max_cache_len`` tokens, handed out at once; otherwise that many for all,
     and ``reserve`` / ``release`` hand them out and take them back.  The page table is device memory that captured calls read when they
     run."""

@@ -477,7 +477,8 @@ int glq_paged_append(const glq_paged_kv_t* kv, const glq_paged_rows_t* rows, con
 
 /* Causal attention of the call's rows over the cache, the call's own tokens (glq_paged_append before it) among it:
  * out = softmax(scale * q . K^T) V over the keys at positions 0 .. the row's own, head h of n_heads on key/value head
- * h / (n_heads / n_kv).  q, out fp16 (rows, n_heads, head_dim); a row that sees no key is zero.  scale finite, >= 0.  Scores, softmax and sums in fp32, the
+ * h / (n_heads / n_kv).  q, out fp16 (rows, n_heads, head_dim); a row that sees no key is zero.  scale finite, >= 0 (a score below -1e30 counts as
+ * none).  Values of a block whose scale is below 2^-60 count as zero.  Scores, softmax and sums in fp32, the
  * probabilities rounded to fp16 as the second product's operand.  What lies in the slots and pages behind a sequence's tokens does not matter,
  * scales included.  Workspace contents irrelevant; some calls need none (0 bytes, workspace may be NULL).  GLQ_ERR_UNSUPPORTED: rows times
  * tokens that the table has room for are too many to be counted in 32 bits (in steps of 64 tokens and blocks of 8 rows or more, all heads). */
