@@ -16,7 +16,8 @@
 //   15          works out the CTA's pieces of segments and hands them to the others through a small queue
 // Scales and m as in paged_attention_rows_kernel: w = 2^(ks s + log2 vs - m) in fp16 (the operand in tensor memory; the results' error becomes 2.5e-4 to 2.9e-4
 // where their own rounding is 2.1e-4; w in two halves would double P V and what the softmax packs and stores, which is the longer of the two), the sum of w / vs in fp32, m raised only when a score exceeds it
-// by 2^8.  Keys that a row does not see get a score of -inf, in the half steps that have such keys, and the common path has no masks.
+// by 2^8 (a published idea, as is taking a part of the exponentials as polynomials).  Keys that a row does not see get a score of -inf, in the half steps that
+// have such keys, and the common path has no masks.
 //
 // The loops around it all are rolled: every warp of a scheduler runs another role's code, and what the instruction cache does not hold costs the
 // warps that issue the MMAs more than the MMAs (134 cycles an MMA with unrolled loops everywhere).

@@ -368,7 +368,8 @@ class GLoRCQDecoder(nn.Module):
                 logits_to_keep=0, **_unused):
         """``logits_to_keep`` = k > 0 computes the logits of the last k positions only (the greedy loop needs
         one); 0 keeps them all, as the transformers models do by default.  ``cache_position``: the positions of the T tokens, the same
-        for all sequences; with a ``PagedKVCache`` (T > 1: consecutive ones) also (B,) for T = 1 or (B, T), a sequence's own."""
+        for all sequences; with a ``PagedKVCache`` (T > 1: consecutive ones) also (B,) for T = 1 or (B, T), a sequence's own; they are not read back, and tokens
+        at positions that the cache does not have are not stored."""
         c = self.config
         B, T = input_ids.shape
         if past_key_values is None:
